@@ -328,6 +328,106 @@ int sf_release_graphs(void);
  * ids [B1, N] int64 on the device. */
 int sf_parent_map(const int64_t* ids, int B1, int N, int64_t* par_idx, void* stream);
 
+/* ------------------------------------------------------------------ paged cache ----
+ * A pool of pages shared by many sequences, the attention that reads it and the eviction
+ * that bounds it.  No counterpart in the reference, whose running prefix is one sequence's
+ * DynamicCache (modeling_ministral.py:154-158).
+ *
+ *   k_pages, v_pages  [num_pages][Hkv][page_size][hd], hd contiguous, the other strides (in
+ *                     elements, alike for both) multiples of 16 bytes: page-major and
+ *                     token-major pools alike
+ *   mass_pages        [num_pages][Hkv][page_size] fp32, contiguous: every cached key's
+ *                     accumulated attention weight
+ *   table             [B][width] int32 page ids (row stride in elements); position x of
+ *                     sequence b is row x % page_size of page table[b][x / page_size].
+ *                     Entries of pages that no new token sees (past a sequence's last
+ *                     key, or wholly between the sinks and the window) are not read.  Any
+ *                     other id outside [0, num_pages) sets SF_DEV_INDEX: it is read as page
+ *                     0, and not written at all.
+ *   q, out            [T, H, hd], the new tokens of all sequences one after the other
+ *
+ * Sequence b has kv_lens[b] cached keys, those of its q_lens[b] new tokens included; token i
+ * of the chunk sits at position p = kv_len - q_len + i and sees key j when
+ *     j < hi(i)  and  (j > p - window  or  j < sinks),
+ *     hi(i) = min(kv_len, kv_len - q_len + (i / block + 1) * block)
+ * block = 1: causal; block = N: bidirectional inside blocks of N tokens of the chunk; block =
+ * 0: hi(i) = kv_len.  window = 0: no lower bound (sinks is then unused).  A row that sees
+ * nothing (kv_len 0, or more new tokens than cached keys) gets out = 0 and lse = -inf.
+ *
+ * head_dim 64 or 128, H / Hkv <= 16, page_size a power of two in [16, 256].               */
+typedef struct sf_paged_list {       /* one kernel's share of a plan (offsets in words) */
+  int32_t items, n_items, first, workers, merges, n_merges, slots, rows, tile_tokens, pad;
+} sf_paged_list;
+
+typedef struct sf_paged_plan {
+  /* set by the caller */
+  int32_t dtype, B, H, Hkv, hd, page_size, block, window, sinks;
+  int32_t sms;                       /* SMs to spread the work over; 0: the current device's */
+  /* set by sf_paged_plan_build */
+  int32_t T, max_kv, short_chunk;    /* short_chunk: some q_len > kv_len (nothing to append) */
+  int32_t tokens;                    /* offset of the {sequence, position} list */
+  sf_paged_list attn[2], mass;       /* [0]: few query rows per kv head, [1]: many */
+  int64_t words;                     /* words of the plan */
+  size_t ws_bytes;                   /* scratch of sf_paged_attention */
+  /* set by the caller before the first use */
+  const int32_t* dev;                /* the plan's words in device memory */
+  void* ws;                          /* ws_bytes of device memory */
+  int* err;                          /* device error word (SF_DEV_*), zeroed by the caller */
+} sf_paged_plan;
+
+/* Splits one step's work over the SMs.  The split depends on the lengths, the head counts and
+ * the mask alone, so one plan serves every layer of the step.  q_lens, kv_lens and words are
+ * HOST arrays; words must hold sf_paged_plan_words(...) words (0: an argument is wrong, see
+ * sf_last_error).  The caller copies plan->words words to device memory and sets dev, ws and
+ * err.  Calls that share a plan share its scratch: they must not overlap on the GPU. */
+int64_t sf_paged_plan_words(const sf_paged_plan* plan, const int32_t* q_lens,
+                            const int32_t* kv_lens);
+int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_t* kv_lens,
+                        int32_t* words, int64_t cap);
+
+typedef struct sf_paged_pool {
+  const void* k_pages;
+  const void* v_pages;
+  float* mass_pages;                 /* NULL where a call does not use it */
+  int64_t page_stride, head_stride, row_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t num_pages, table_width;
+} sf_paged_pool;
+
+/* The new rows of every sequence into its pages, at positions [kv_len - q_len, kv_len);
+ * mass_pages, when not NULL, is zeroed there.  k_new / v_new [T][Hkv][hd] with the given token
+ * and head strides (elements, 16-byte multiples, alike for both). */
+int sf_paged_kv_append(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* k_new,
+                       const void* v_new, int64_t new_tok_stride, int64_t new_head_stride,
+                       void* stream);
+
+/* out = softmax(scale * q K^T + mask) V and lse = ln of the softmax's denominator [T, H] fp32.
+ * q has the given token and head strides (16-byte multiples); out is contiguous.  scale > 0. */
+int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* q,
+                       int64_t q_tok_stride, int64_t q_head_stride, void* out, float* lse,
+                       float scale, void* stream);
+
+/* mass[key] += sum over the tokens that see it and the query heads of its kv head of
+ * exp(scale * q . k - lse), lse as sf_paged_attention wrote it.  Each weight is summed in one
+ * place in a fixed order: the same inputs give the same bits. */
+int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* q,
+                            int64_t q_tok_stride, int64_t q_head_stride, const float* lse,
+                            float scale, void* stream);
+
+/* Eviction: of the lens[b][0] cached keys of every (sequence, kv head) lens[b][1] stay (all,
+ * when there are no more): the first `sinks`, the last `recent`, and of the others those with
+ * the largest accumulated weight, equal weights by position, the lowest first (NaN ranks above
+ * +inf).  Their rows and weights move, in the order of their positions, to positions 0, 1, ...
+ * of the pages of dst_table, which must not be pages of a source table; kept [B][Hkv]
+ * [kept_stride] gets their old positions, -1 after the last.  lens [B][2] int32 on the device
+ * with max_len / max_keep its columns' maxima; sinks + recent <= every lens[b][1] that is below
+ * lens[b][0]; kept_stride >= min(max_len, max_keep). */
+int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_table,
+                   int64_t dst_stride, int32_t dst_width, const int32_t* lens, int32_t max_len,
+                   int32_t max_keep, int B, int Hkv, int hd, int page_size, int sinks, int recent,
+                   int32_t* kept, int64_t kept_stride, int* err, void* stream);
+
 /* ------------------------------------------------------------------ measurement ----
  * Kernels launched by this library so far (all host threads).                       */
 long long sf_launch_count(void);

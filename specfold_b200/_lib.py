@@ -17,6 +17,7 @@ _LIB = None
 
 c_void_p, c_int, c_float, c_int64, c_size_t = C.c_void_p, C.c_int, C.c_float, C.c_int64, C.c_size_t
 
+SF_ERR_ARG = 1
 SF_DTYPE_F32 = 0
 SF_DTYPE_BF16 = 1
 DEV_ERR_BITS = {1: "barrier wait timed out", 2: "index out of range", 4: "parent chain too deep",
@@ -44,6 +45,30 @@ class SfVerifyArgs(C.Structure):
         ("P_dev", c_void_p), ("commit", c_int), ("tp_peers", c_void_p), ("prefill", c_int),
     ]
 
+
+class SfPagedList(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("items", "n_items", "first", "workers", "merges", "n_merges",
+                                         "slots", "rows", "tile_tokens", "pad")]
+
+
+class SfPagedPlan(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "B", "H", "Hkv", "hd", "page_size", "block", "window",
+                                         "sinks", "sms", "T", "max_kv", "short_chunk", "tokens")] + [
+        ("attn", SfPagedList * 2), ("mass", SfPagedList), ("words", c_int64), ("ws_bytes", c_size_t),
+        ("dev", c_void_p), ("ws", c_void_p), ("err", c_void_p),
+    ]
+
+
+class SfPagedPool(C.Structure):
+    _fields_ = [
+        ("k_pages", c_void_p), ("v_pages", c_void_p), ("mass_pages", c_void_p),
+        ("page_stride", c_int64), ("head_stride", c_int64), ("row_stride", c_int64),
+        ("table", c_void_p), ("table_stride", c_int64), ("num_pages", C.c_int32),
+        ("table_width", C.c_int32),
+    ]
+
+
+_PLAN, _POOL = C.POINTER(SfPagedPlan), C.POINTER(SfPagedPool)
 
 # name -> (restype, argtypes); mirrors include/specfold_b200.h
 _SIGS = {
@@ -107,6 +132,16 @@ _SIGS = {
     "sf_release_graphs": (c_int, []),
     "sf_pack_weight_tiles": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                      c_void_p]),
+    "sf_paged_plan_words": (c_int64, [_PLAN, c_void_p, c_void_p]),
+    "sf_paged_plan_build": (c_int, [_PLAN, c_void_p, c_void_p, c_void_p, c_int64]),
+    "sf_paged_kv_append": (c_int, [_PLAN, _POOL, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "sf_paged_attention": (c_int, [_PLAN, _POOL, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                   c_float, c_void_p]),
+    "sf_paged_attention_mass": (c_int, [_PLAN, _POOL, c_void_p, c_int64, c_int64, c_void_p, c_float,
+                                        c_void_p]),
+    "sf_paged_evict": (c_int, [c_int, _POOL, c_void_p, c_int64, C.c_int32, c_void_p, C.c_int32,
+                               C.c_int32, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64,
+                               c_void_p, c_void_p]),
     "sf_launch_count": (C.c_longlong, []),
     "sf_profile_begin": (c_int, [c_int]),
     "sf_profile_end": (c_int, []),

@@ -48,6 +48,13 @@ int cuda_status(cudaError_t e, const char* what) {
   return fail(SF_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+}  // namespace
+
+// the same for the entry points of other files
+int sf::report(int code, const char* msg) { return fail(code, "%s", msg); }
+
+namespace {
+
 size_t esize(int dtype) { return dtype == SF_DTYPE_BF16 ? 2 : 4; }
 
 bool dtype_ok(int dtype) { return dtype == SF_DTYPE_F32 || dtype == SF_DTYPE_BF16; }

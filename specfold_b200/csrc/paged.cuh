@@ -1,0 +1,173 @@
+// Paged prefix cache: what its kernels, the plan builder and the C entries share.
+//
+// A pool of pages [num_pages][Hkv][page_size][hd] holds the keys (and another the values, a
+// third the fp32 accumulated attention weight of every key) of many sequences; a table
+// [B][width] of page ids maps a sequence's positions to pages.  A step runs the q_b new tokens
+// of every sequence against its n_b cached ones (the new ones included).  Token i of a chunk
+// sits at position p = n - q + i and sees key j when
+//     j < hi(i)  and  (j > p - window  or  j < sinks)
+//     hi(i) = min(n, n - q + (i / block + 1) * block), or n when block = 0
+// (window = 0: no lower bound).  block = 1 is the causal mask, block = N the block-causal one.
+//
+// The lengths are known on the host, so the split of the work over the SMs is made there once
+// per step, for all layers (paged_plan.cu): an item is a run of key blocks of one (sequence,
+// kv head, tile of query rows), and every CTA gets a contiguous share of the items of equal
+// cost.  A tile whose run was cut writes fp32 partials (O, m, l) that a merge joins in the
+// order of the pieces, so results do not depend on timing.
+#pragma once
+
+#include "../../include/specfold_b200.h"
+#include "sf_kernels.cuh"
+
+namespace sf {
+
+constexpr int kPagedKB = 128;         // keys of one block: the unit the plan counts in
+constexpr int kPagedMaxGroup = 16;    // query heads per kv head
+
+// A run [i0, i1) of the key blocks that a tile of query rows sees.  The blocks a tile sees
+// are the sink blocks 0 .. sink_blks - 1, then lo_blk, lo_blk + 1, ...
+struct alignas(16) PagedItem {
+  int32_t seq, kvh, tok0, ntok;       // the tile: tokens [tok0, tok0 + ntok) of the chunk
+  int32_t i0, i1, slot, sink_blks;    // slot < 0: writes the output itself
+  int32_t lo_blk, q0, q_len, kv_len;  // q0: the chunk's first row in q / out
+  __host__ __device__ int block(int i) const { return i < sink_blks ? i : i - sink_blks + lo_blk; }
+};
+// A tile whose run was cut into n pieces, in slots [slot0, slot0 + n)
+struct alignas(16) PagedMerge {
+  int32_t kvh, tok0, ntok, slot0;
+  int32_t n, q0, pad0, pad1;
+};
+// Key blocks [kb0, kb1) of one (sequence, kv head), for the weight accumulation
+struct alignas(16) PagedMassItem {
+  int32_t seq, kvh, kb0, kb1;
+  int32_t q0, q_len, kv_len, pad;
+};
+
+// The keys that some token of a range sees: [lo, hi) and [0, sinks)
+struct PagedRange {
+  int lo, hi, sinks;
+  __host__ __device__ bool has(int key) const { return key < hi && (key >= lo || key < sinks); }
+  // any key of [a, b)
+  __host__ __device__ bool meets(int a, int b) const { return a < hi && (b > lo || a < sinks); }
+};
+
+struct PagedMask {
+  int block, window, sinks, q_len, kv_len;
+  __host__ __device__ int pos(int i) const { return kv_len - q_len + i; }
+  // keys [0, hi) at most
+  __host__ __device__ int hi(int i) const {
+    if (block == 0) return kv_len;
+    const int64_t h = static_cast<int64_t>(kv_len) - q_len + (static_cast<int64_t>(i / block) + 1) * block;
+    return h < kv_len ? static_cast<int>(h) : kv_len;
+  }
+  // keys [lo, hi) and [0, sinks)
+  __host__ __device__ int lo(int i) const {
+    if (window == 0) return 0;
+    const int l = pos(i) - window + 1;
+    return l > 0 ? l : 0;
+  }
+  __host__ __device__ PagedRange range(int t0, int t1) const { return {lo(t0), hi(t1 - 1), window > 0 ? sinks : 0}; }
+  // the tokens of the chunk that see any key of block kb: [first, last)
+  __host__ __device__ void tokens(int kb, int* first, int* last) const {
+    const int k0 = kb * kPagedKB;
+    const int k1 = k0 + kPagedKB < kv_len ? k0 + kPagedKB : kv_len;   // exclusive
+    int f = 0, l = q_len;
+    if (block > 0) {
+      // hi(i) > k0  <=>  i / block + 1 > (k0 - base) / block
+      const int base = kv_len - q_len;
+      if (k0 >= base) f = (k0 - base) / block * block;
+    }
+    if (window > 0 && k0 >= sinks) {
+      // lo(i) < k1  <=>  i < k1 + window - 1 - base
+      const int64_t e = static_cast<int64_t>(k1) + window - 1 - (kv_len - q_len);
+      if (e < l) l = e > 0 ? static_cast<int>(e) : 0;
+    }
+    *first = f < q_len ? f : q_len;
+    *last = l > *first ? l : *first;
+  }
+};
+
+struct PagedPool {
+  const void* k;
+  const void* v;
+  int64_t page_stride, head_stride, row_stride;   // elements, k and v alike
+  float* mass;                                     // [num_pages][Hkv][page_size], contiguous
+  int num_pages, page_shift;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width;
+};
+
+struct PagedAttnParams {
+  const void* q;
+  int64_t q_tok, q_head;            // strides, elements
+  PagedPool pool;
+  void* out;                        // [T, H, hd] contiguous
+  float* lse;                       // [T, H]
+  const PagedItem* items;
+  const int32_t* first;             // [workers + 1] first item of every CTA
+  int workers;
+  const PagedMerge* merges;
+  int n_merges;
+  float* part_O;                    // [slots][rows][hd]
+  float* part_ml;                   // [slots][rows][2]
+  int rows, tile_tokens;            // rows of a slot; tokens of 128 (64) rows
+  int H, Hkv, G, hd, T;
+  int block, window, sinks;
+  float scale;
+  int* err;
+};
+
+struct PagedMassParams {
+  const void* q;
+  int64_t q_tok, q_head;
+  PagedPool pool;
+  const float* lse;                 // [T, H]
+  const PagedMassItem* items;
+  const int32_t* first;
+  int workers;
+  int H, Hkv, G, hd, T;
+  int block, window, sinks;
+  float scale;
+  int* err;
+};
+
+// page id of position pos; an id outside the pool is flagged and read as page 0
+__device__ __forceinline__ int paged_page(const PagedPool& p, int seq, int idx, int* err) {
+  const int id = p.table[seq * p.table_stride + idx];
+  if (id < 0 || id >= p.num_pages) {
+    flag_error(err, SF_DEV_ERR_INDEX);
+    return 0;
+  }
+  return id;
+}
+
+cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cudaStream_t st);
+cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st);
+cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st);
+
+// {sequence, position} of every new token
+struct PagedAppendParams {
+  const void* k_new;
+  const void* v_new;
+  int64_t new_tok, new_head;
+  PagedPool pool;
+  const int32_t* tokens;            // [T][2]
+  int T, Hkv, hd;
+  int* err;
+};
+cudaError_t launch_paged_append(int dtype, const PagedAppendParams& p, cudaStream_t st);
+
+struct PagedEvictParams {
+  PagedPool pool;                   // table = the source table
+  const int32_t* dst;               // destination table
+  int64_t dst_stride;
+  const int32_t* lens;              // [B][2]: cached keys, keys that stay
+  int32_t* kept;                    // [B][Hkv][kept_stride]
+  int kept_stride;
+  int B, Hkv, hd, sinks, recent, max_len, max_keep;
+  int* err;
+};
+cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_t st);
+
+}  // namespace sf

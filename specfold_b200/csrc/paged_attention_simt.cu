@@ -1,0 +1,389 @@
+// Attention over the paged cache and its weight accumulation on the FP32 pipe: the fp32 path
+// (the tensor core's tf32 products would round the inputs to 11 bits).
+//
+// One CTA walks the items of its share.  A tile of R = 16 * RM query rows (row = token * G + g)
+// meets 64 keys at a time: S = Q K^T from shared memory with an RM x 4 register tile per
+// thread, the running maximum and sum of the softmax per row, P back through shared memory, and
+// O += P V with an RM x hd/16 register tile.  K and V share one buffer so that two CTAs fit an
+// SM and one's loads run under the other's products.
+#include "paged.cuh"
+
+namespace sf {
+
+constexpr int kSimtThreads = 256;
+constexpr int kSimtKeys = 64;
+
+template <typename T>
+__device__ __forceinline__ void simt_store_row(float* dst, const T* src, int e);
+template <>
+__device__ __forceinline__ void simt_store_row<float>(float* dst, const float* src, int e) {
+  *reinterpret_cast<float4*>(dst + e) = *reinterpret_cast<const float4*>(src + e);
+}
+template <>
+__device__ __forceinline__ void simt_store_row<__nv_bfloat16>(float* dst, const __nv_bfloat16* src,
+                                                              int e) {
+  float f[8];
+  load_vec(src + e, f);
+  *reinterpret_cast<float4*>(dst + e) = make_float4(f[0], f[1], f[2], f[3]);
+  *reinterpret_cast<float4*>(dst + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+// keys [k0, k0 + 64) of a sequence into shared memory [64][HD + 4]; keys outside `range`, which
+// no row of the tile sees, are zero: their slots may never have been written (0 * NaN is NaN),
+// their pages may be gone
+template <typename T, int HD>
+__device__ __forceinline__ void simt_load_keys(float* dst, const void* pages, const PagedPool& pool,
+                                               int seq, int kvh, int k0, PagedRange range, int* err) {
+  constexpr int VPR = HD / Elt<T>::kVec;
+  for (int i = threadIdx.x; i < kSimtKeys * VPR; i += kSimtThreads) {
+    const int r = i / VPR, e = (i % VPR) * Elt<T>::kVec;
+    const int key = k0 + r;
+    float* d = dst + r * (HD + 4);
+    if (range.has(key)) {
+      const int page = paged_page(pool, seq, key >> pool.page_shift, err);
+      const T* src = static_cast<const T*>(pages) + page * pool.page_stride + kvh * pool.head_stride +
+                     (key & ((1 << pool.page_shift) - 1)) * pool.row_stride;
+      simt_store_row<T>(d, src, e);
+    } else {
+#pragma unroll
+      for (int x = 0; x < Elt<T>::kVec; x += 4)
+        *reinterpret_cast<float4*>(d + e + x) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+}
+
+template <typename T, int HD, int RM>
+__device__ __forceinline__ void simt_load_q(float* sQ, const void* q, int64_t q_tok, int64_t q_head,
+                                            int row0, int kvh, int G, int rows) {
+  constexpr int VPR = HD / Elt<T>::kVec;
+  for (int i = threadIdx.x; i < 16 * RM * VPR; i += kSimtThreads) {
+    const int r = i / VPR, e = (i % VPR) * Elt<T>::kVec;
+    float* d = sQ + r * (HD + 4);
+    if (r < rows) {
+      simt_store_row<T>(d, static_cast<const T*>(q) + (row0 + r / G) * q_tok + (kvh * G + r % G) * q_head, e);
+    } else {
+#pragma unroll
+      for (int x = 0; x < Elt<T>::kVec; x += 4)
+        *reinterpret_cast<float4*>(d + e + x) = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+}
+
+// s[a][c] = q row (ty + 16 a) . key (tx + 16 c)
+template <int HD, int RM>
+__device__ __forceinline__ void simt_scores(const float* sQ, const float* sK, float (&s)[RM][4]) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int a = 0; a < RM; ++a)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[a][c] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < HD; d += 4) {
+    float4 kf[4], qf[RM];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const float4*>(sK + (tx + 16 * c) * (HD + 4) + d);
+#pragma unroll
+    for (int a = 0; a < RM; ++a) qf[a] = *reinterpret_cast<const float4*>(sQ + (ty + 16 * a) * (HD + 4) + d);
+#pragma unroll
+    for (int a = 0; a < RM; ++a)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[a][c] = fmaf(qf[a].x, kf[c].x, s[a][c]);
+        s[a][c] = fmaf(qf[a].y, kf[c].y, s[a][c]);
+        s[a][c] = fmaf(qf[a].z, kf[c].z, s[a][c]);
+        s[a][c] = fmaf(qf[a].w, kf[c].w, s[a][c]);
+      }
+  }
+}
+
+__device__ __forceinline__ float half_warp_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float half_warp_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int HD, int RM>
+__global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(PagedAttnParams p) {
+  constexpr int R = 16 * RM, LD = HD + 4, LP = kSimtKeys + 4;
+  constexpr int DV = HD / 64;                           // float4 groups of O per thread
+  extern __shared__ __align__(16) float sm[];
+  float* sQ = sm;                                       // [R][LD]
+  float* sKV = sQ + R * LD;                             // [64][LD]
+  float* sP = sKV + kSimtKeys * LD;                     // [R][LP]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const float sl2 = p.scale * 1.4426950408889634f;
+  const int last = p.first[blockIdx.x + 1];
+  for (int it = p.first[blockIdx.x]; it < last; ++it) {
+    const PagedItem w = p.items[it];
+    const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
+    const int rows = w.ntok * p.G;
+    float m[RM], l[RM], o[RM][DV][4];
+    int hi[RM], lo[RM];
+#pragma unroll
+    for (int a = 0; a < RM; ++a) {
+      m[a] = -INFINITY;
+      l[a] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DV; ++d) o[a][d][0] = o[a][d][1] = o[a][d][2] = o[a][d][3] = 0.f;
+      const int r = ty + 16 * a;
+      const int i = w.tok0 + r / p.G;
+      hi[a] = r < rows ? mask.hi(i) : 0;
+      lo[a] = r < rows ? mask.lo(i) : 0;
+    }
+    const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
+    __syncthreads();                                    // the previous item's reads are done
+    simt_load_q<T, HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + w.tok0, w.kvh, p.G, rows);
+    for (int i = w.i0; i < w.i1; ++i) {
+      for (int sub = 0; sub < kPagedKB / kSimtKeys; ++sub) {
+        const int k0 = w.block(i) * kPagedKB + sub * kSimtKeys;
+        if (k0 >= range.hi) break;
+        __syncthreads();
+        simt_load_keys<T, HD>(sKV, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
+        __syncthreads();
+        float s[RM][4];
+        simt_scores<HD, RM>(sQ, sKV, s);
+#pragma unroll
+        for (int a = 0; a < RM; ++a) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int j = k0 + tx + 16 * c;
+            const bool see = j < hi[a] && (j >= lo[a] || j < p.sinks);
+            s[a][c] = see ? s[a][c] * sl2 : -INFINITY;
+            mx = fmaxf(mx, s[a][c]);
+          }
+          const float mn = fmaxf(m[a], half_warp_max(mx));
+          const float ref = mn == -INFINITY ? 0.f : mn;
+          const float alpha = exp2f(m[a] - ref);
+          float sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float e = exp2f(s[a][c] - ref);
+            sum += e;
+            sP[(ty + 16 * a) * LP + tx + 16 * c] = e;
+          }
+          l[a] = l[a] * alpha + half_warp_sum(sum);
+          m[a] = mn;
+#pragma unroll
+          for (int d = 0; d < DV; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[a][d][x] *= alpha;
+        }
+        __syncthreads();                                // K read, P written
+        simt_load_keys<T, HD>(sKV, p.pool.v, p.pool, w.seq, w.kvh, k0, range, p.err);
+        __syncthreads();
+        // a row of P is written and read by the same half-warp's 16 threads
+#pragma unroll 2
+        for (int j = 0; j < kSimtKeys; j += 4) {
+          float4 pf[RM];
+#pragma unroll
+          for (int a = 0; a < RM; ++a) pf[a] = *reinterpret_cast<const float4*>(sP + (ty + 16 * a) * LP + j);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+            for (int d = 0; d < DV; ++d) {
+              const float4 v = *reinterpret_cast<const float4*>(sKV + (j + jj) * LD + d * 64 + tx * 4);
+#pragma unroll
+              for (int a = 0; a < RM; ++a) {
+                const float e = jj == 0 ? pf[a].x : jj == 1 ? pf[a].y : jj == 2 ? pf[a].z : pf[a].w;
+                o[a][d][0] = fmaf(e, v.x, o[a][d][0]);
+                o[a][d][1] = fmaf(e, v.y, o[a][d][1]);
+                o[a][d][2] = fmaf(e, v.z, o[a][d][2]);
+                o[a][d][3] = fmaf(e, v.w, o[a][d][3]);
+              }
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < RM; ++a) {
+      const int r = ty + 16 * a;
+      if (r >= rows) continue;
+      if (w.slot >= 0) {
+        const int64_t pr = static_cast<int64_t>(w.slot) * p.rows + r;
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+          *reinterpret_cast<float4*>(p.part_O + pr * HD + d * 64 + tx * 4) =
+              make_float4(o[a][d][0], o[a][d][1], o[a][d][2], o[a][d][3]);
+        if (tx == 0) {
+          p.part_ml[2 * pr] = m[a];
+          p.part_ml[2 * pr + 1] = l[a];
+        }
+      } else {
+        const int64_t t = w.q0 + w.tok0 + r / p.G;
+        const int h = w.kvh * p.G + r % p.G;
+        const float inv = l[a] == 0.f ? 0.f : 1.f / l[a];   // a NaN sum stays one
+        T* dst = static_cast<T*>(p.out) + (t * p.H + h) * HD;
+#pragma unroll
+        for (int d = 0; d < DV; ++d)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) dst[d * 64 + tx * 4 + x] = Elt<T>::from_f(o[a][d][x] * inv);
+        if (tx == 0) p.lse[t * p.H + h] = m[a] * 0.6931471805599453f + logf(l[a]);
+      }
+    }
+  }
+}
+
+// Joins the pieces of the tiles that were cut: one warp per row, pieces in order.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnParams p) {
+  constexpr int E = HD / 32;
+  pdl_wait();
+  const PagedMerge w = p.merges[blockIdx.y];
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= w.ntok * p.G) return;
+  const int t = r / p.G, g = r % p.G;
+  const int half = t / p.tile_tokens;
+  const int pr = half * 128 + (t - half * p.tile_tokens) * p.G + g;
+  float m = -INFINITY;
+  for (int i = 0; i < w.n; ++i)
+    m = fmaxf(m, p.part_ml[2 * (static_cast<int64_t>(w.slot0 + i) * p.rows + pr)]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < w.n; ++i) {
+    const int64_t at = static_cast<int64_t>(w.slot0 + i) * p.rows + pr;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+    const float f = exp2f(ml.x - ref);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p.part_O + at * HD + lane * E + e);
+      o[e] = fmaf(v.x, f, o[e]);
+      o[e + 1] = fmaf(v.y, f, o[e + 1]);
+    }
+  }
+  const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + t) * p.H + w.kvh * p.G + g;
+  const float inv = l == 0.f ? 0.f : 1.f / l;           // a NaN sum stays one
+  T* dst = static_cast<T*>(p.out) + row * HD + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = Elt<T>::from_f(o[e] * inv);
+  if (lane == 0) p.lse[row] = m * 0.6931471805599453f + logf(l);
+}
+
+cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st) {
+  if (p.n_merges == 0) return cudaSuccess;
+  const dim3 grid((p.rows + 7) / 8, p.n_merges);
+  auto go = [&](auto* kernel) {
+    kernel<<<grid, 256, 0, st>>>(p);
+    return launched();
+  };
+  if (dtype == BF16)
+    return p.hd == 128 ? go(paged_merge_kernel<__nv_bfloat16, 128>) : go(paged_merge_kernel<__nv_bfloat16, 64>);
+  return p.hd == 128 ? go(paged_merge_kernel<float, 128>) : go(paged_merge_kernel<float, 64>);
+}
+
+template <typename T, int HD, int RM>
+static cudaError_t attention_simt(const PagedAttnParams& p, cudaStream_t st) {
+  constexpr int R = 16 * RM;
+  constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + R * (kSimtKeys + 4)) * 4;
+  cudaError_t e = cudaFuncSetAttribute(paged_attention_simt_kernel<T, HD, RM>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  paged_attention_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
+  return launched();
+}
+
+cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cudaStream_t st) {
+  if (p.workers == 0) return cudaSuccess;
+  const bool wide = p.rows == 64;
+  if (dtype == BF16) {
+    if (p.hd == 128) return wide ? attention_simt<__nv_bfloat16, 128, 4>(p, st) : attention_simt<__nv_bfloat16, 128, 1>(p, st);
+    return wide ? attention_simt<__nv_bfloat16, 64, 4>(p, st) : attention_simt<__nv_bfloat16, 64, 1>(p, st);
+  }
+  if (p.hd == 128) return wide ? attention_simt<float, 128, 4>(p, st) : attention_simt<float, 128, 1>(p, st);
+  return wide ? attention_simt<float, 64, 4>(p, st) : attention_simt<float, 64, 1>(p, st);
+}
+
+// ------------------------------------------------------------------ weight accumulation
+// A key's weight over all rows that see it: sum of exp(s - lse).  A CTA owns a key block and
+// walks the query rows, so each weight is summed in one place, in one order, without atomics.
+template <typename T, int HD, int RM>
+__global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedMassParams p) {
+  constexpr int R = 16 * RM, LD = HD + 4;
+  extern __shared__ __align__(16) float sm[];
+  float* sQ = sm;                                       // [R][LD]
+  float* sK = sQ + R * LD;                              // [64][LD]
+  float* sR = sK + kSimtKeys * LD;                      // [16][64]
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const float sl2 = p.scale * 1.4426950408889634f;
+  const int last = p.first[blockIdx.x + 1];
+  const int tile = R / p.G;
+  for (int it = p.first[blockIdx.x]; it < last; ++it) {
+    const PagedMassItem w = p.items[it];
+    const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
+    for (int kb = w.kb0; kb < w.kb1; ++kb) {
+      int t0, t1;
+      mask.tokens(kb, &t0, &t1);
+      if (t0 >= t1) continue;
+      const PagedRange range = mask.range(t0, t1);
+      for (int sub = 0; sub < kPagedKB / kSimtKeys; ++sub) {
+        const int k0 = kb * kPagedKB + sub * kSimtKeys;
+        if (k0 >= range.hi) break;
+        __syncthreads();
+        simt_load_keys<T, HD>(sK, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int t = t0; t < t1; t += tile) {
+          const int rows = min(tile, t1 - t) * p.G;
+          __syncthreads();
+          simt_load_q<T, HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + t, w.kvh, p.G, rows);
+          __syncthreads();
+          float s[RM][4];
+          simt_scores<HD, RM>(sQ, sK, s);
+#pragma unroll
+          for (int a = 0; a < RM; ++a) {
+            const int r = ty + 16 * a;
+            if (r >= rows) continue;
+            const int i = t + r / p.G;
+            const float lse = p.lse[static_cast<int64_t>(w.q0 + i) * p.H + w.kvh * p.G + r % p.G] * 1.4426950408889634f;
+            const int hi = mask.hi(i), lo = mask.lo(i);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int j = k0 + tx + 16 * c;
+              if (j < hi && (j >= lo || j < p.sinks)) acc[c] += exp2f(fmaf(s[a][c], sl2, -lse));
+            }
+          }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sR[ty * kSimtKeys + tx + 16 * c] = acc[c];
+        __syncthreads();
+        if (threadIdx.x < kSimtKeys && range.has(k0 + threadIdx.x)) {
+          float sum = 0.f;
+          for (int y = 0; y < 16; ++y) sum += sR[y * kSimtKeys + threadIdx.x];
+          const int j = k0 + threadIdx.x;
+          const int page = paged_page(p.pool, w.seq, j >> p.pool.page_shift, p.err);
+          p.pool.mass[((static_cast<int64_t>(page) * p.Hkv + w.kvh) << p.pool.page_shift) +
+                      (j & ((1 << p.pool.page_shift) - 1))] += sum;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int HD, int RM>
+static cudaError_t mass_simt(const PagedMassParams& p, cudaStream_t st) {
+  constexpr int R = 16 * RM;
+  constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + 16 * kSimtKeys) * 4;
+  cudaError_t e = cudaFuncSetAttribute(paged_mass_simt_kernel<T, HD, RM>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  paged_mass_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
+  return launched();
+}
+
+cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st) {
+  if (p.workers == 0) return cudaSuccess;
+  if (dtype == BF16)
+    return p.hd == 128 ? mass_simt<__nv_bfloat16, 128, 4>(p, st) : mass_simt<__nv_bfloat16, 64, 4>(p, st);
+  return p.hd == 128 ? mass_simt<float, 128, 4>(p, st) : mass_simt<float, 64, 4>(p, st);
+}
+
+}  // namespace sf

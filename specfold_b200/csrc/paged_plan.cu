@@ -1,0 +1,532 @@
+// The paged cache's plan (how a step's work is split over the SMs) and its C entries.
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+#include <queue>
+#include <vector>
+
+#include "paged.cuh"
+
+using namespace sf;
+
+namespace {
+
+int bad(const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return report(SF_ERR_ARG, buf);
+}
+
+constexpr int kItemWords = sizeof(PagedItem) / 4;
+constexpr int kMergeWords = sizeof(PagedMerge) / 4;
+constexpr int kMassWords = sizeof(PagedMassItem) / 4;
+constexpr int64_t kMaxWords = int64_t{1} << 30;
+
+int64_t up4(int64_t x) { return (x + 3) & ~int64_t{3}; }
+
+// Rows of a tile and of the two kernels' tiles.  bf16: one MMA tile of 128 rows (short chunks:
+// single tokens, small blocks), two of them (long ones).  fp32: 16 and 64 rows.
+struct Tiling {
+  int rows[2], tokens[2], per_tile[2], workers[2], mass_workers, mass_rows;
+};
+Tiling tiling(const sf_paged_plan& p) {
+  const int G = p.H / p.Hkv;
+  Tiling t{};
+  t.rows[0] = 16;
+  t.rows[1] = 64;
+  t.tokens[0] = 16 / G;
+  t.tokens[1] = 64 / G;
+  t.per_tile[0] = t.tokens[0];
+  t.per_tile[1] = t.tokens[1];
+  t.workers[0] = t.workers[1] = 2 * p.sms;
+  t.mass_workers = 2 * p.sms;
+  t.mass_rows = 64;
+  return t;
+}
+
+int check_plan(const sf_paged_plan* p, const int32_t* q_lens, const int32_t* kv_lens) {
+  if (!p || p->B < 0 || (p->B > 0 && (!q_lens || !kv_lens))) return bad("paged plan: null argument");
+  if (p->dtype != SF_DTYPE_F32 && p->dtype != SF_DTYPE_BF16) return bad("paged plan: dtype %d not supported", p->dtype);
+  if (p->hd != 64 && p->hd != 128) return bad("paged plan: head_dim %d must be 64 or 128", p->hd);
+  if (p->H <= 0 || p->Hkv <= 0 || p->H % p->Hkv != 0 || p->H / p->Hkv > kPagedMaxGroup)
+    return bad("paged plan: heads %d / kv heads %d unsupported", p->H, p->Hkv);
+  if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+    return bad("paged plan: page size %d must be a power of two in [16, 256]", p->page_size);
+  if (p->block < 0 || p->window < 0 || p->sinks < 0) return bad("paged plan: block, window and sinks must not be negative");
+  int64_t T = 0;
+  for (int b = 0; b < p->B; ++b) {
+    if (q_lens[b] < 0 || kv_lens[b] < 0) return bad("paged plan: sequence %d has a negative length", b);
+    if (kv_lens[b] > (1 << 30) || q_lens[b] > (1 << 30)) return bad("paged plan: sequence %d is too long", b);
+    T += q_lens[b];
+  }
+  // rows of q and out are counted in 32 bits, as are a tensor map's coordinates
+  if (T * p->H >= (int64_t{1} << 31)) return bad("paged plan: %lld query rows are too many", static_cast<long long>(T * p->H));
+  return SF_OK;
+}
+
+int device_sms(int asked) {
+  if (asked > 0) return asked;
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess &&
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0)
+    return n;
+  (void)cudaGetLastError();
+  return 148;
+}
+
+int which(const Tiling& t, int q_len, int G) { return static_cast<int64_t>(q_len) * G <= t.rows[0] ? 0 : 1; }
+
+struct Tile {
+  PagedItem item;   // i0 = 0, i1 = its key blocks
+};
+
+// Deals the tiles out in order: each worker takes its share of (key blocks + 1 per tile), and a
+// tile that does not fit goes on with the next one.
+void deal(const std::vector<PagedItem>& tiles, int workers, std::vector<PagedItem>* items,
+          std::vector<int32_t>* first, std::vector<PagedMerge>* merges, int* slots) {
+  int64_t total = 0;
+  for (const PagedItem& t : tiles) total += t.i1 + 1;
+  const int64_t w = std::max<int64_t>(1, std::min<int64_t>(workers, total));
+  first->push_back(0);
+  *slots = 0;
+  int64_t done = 0, worker = 0;   // cost dealt out; end of this worker's share: (worker+1)*total/w
+  for (const PagedItem& t : tiles) {
+    int at = 0, pieces = 0;
+    const size_t from = items->size();
+    do {
+      // what is left of this worker's share; a full one, or one too small to be worth a piece,
+      // ends here
+      int64_t room = (worker + 1) * total / w - done;
+      while (room <= 1 && worker + 1 < w) {
+        first->push_back(static_cast<int32_t>(items->size()));
+        ++worker;
+        room = (worker + 1) * total / w - done;
+      }
+      const int need = t.i1 - at;
+      int take = need;
+      if (worker + 1 < w && need + 1 > room) take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(need, room - 1)));
+      PagedItem it = t;
+      it.i0 = at;
+      it.i1 = at + take;
+      items->push_back(it);
+      at += take;
+      done += take + (pieces == 0 ? 1 : 0);
+      ++pieces;
+    } while (at < t.i1);
+    if (pieces > 1) {
+      PagedMerge m{};
+      m.kvh = t.kvh;
+      m.tok0 = t.tok0;
+      m.ntok = t.ntok;
+      m.slot0 = *slots;
+      m.n = pieces;
+      m.q0 = t.q0;
+      merges->push_back(m);
+      for (size_t i = from; i < items->size(); ++i) (*items)[i].slot = (*slots)++;
+    }
+  }
+  while (static_cast<int64_t>(first->size()) <= w) first->push_back(static_cast<int32_t>(items->size()));
+  first->back() = static_cast<int32_t>(items->size());
+}
+
+size_t list_ws(const sf_paged_list& l, int hd) {
+  return (static_cast<size_t>(l.slots) * l.rows * (hd + 2) * 4 + 255) / 256 * 256;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+PagedPool pool_of(const sf_paged_pool& s, int page_size) {
+  PagedPool p{};
+  p.k = s.k_pages;
+  p.v = s.v_pages;
+  p.mass = s.mass_pages;
+  p.page_stride = s.page_stride;
+  p.head_stride = s.head_stride;
+  p.row_stride = s.row_stride;
+  p.num_pages = s.num_pages;
+  p.page_shift = __builtin_ctz(page_size);
+  p.table = s.table;
+  p.table_stride = s.table_stride;
+  p.table_width = s.table_width;
+  return p;
+}
+
+int check_pool(const char* who, const sf_paged_pool* s, int dtype, int hd, int page_size, int64_t max_kv,
+               bool values, bool mass) {
+  if (!s) return bad("%s: null pool", who);
+  const int vec = dtype == SF_DTYPE_BF16 ? 8 : 4;
+  if (static_cast<int64_t>(s->table_width) * page_size < max_kv || s->table_stride < s->table_width)
+    return bad("%s: a table of %d pages does not hold %lld keys", who, s->table_width,
+               static_cast<long long>(max_kv));
+  if (!s->k_pages || (values && !s->v_pages) || (mass && !s->mass_pages) || (max_kv > 0 && !s->table) || s->num_pages < 1)
+    return bad("%s: null pool pointer or empty pool", who);
+  if (!aligned16(s->k_pages) || !aligned16(s->v_pages) || s->page_stride % vec || s->head_stride % vec ||
+      s->row_stride % vec)
+    return bad("%s: the pools need 16-byte aligned rows", who);
+  if (s->row_stride < hd || s->head_stride < hd || s->page_stride < hd)
+    return bad("%s: pool strides must be positive and at least head_dim", who);
+  return SF_OK;
+}
+
+int check_ready(const char* who, const sf_paged_plan* p) {
+  if (!p) return bad("%s: null plan", who);
+  if (p->words <= 0 || (p->dtype != SF_DTYPE_F32 && p->dtype != SF_DTYPE_BF16) || (p->hd != 64 && p->hd != 128) ||
+      p->page_size < 16)
+    return bad("%s: the plan was not built", who);
+  if (!p->dev || !p->err || (p->ws_bytes > 0 && !p->ws)) return bad("%s: the plan has no device memory", who);
+  return SF_OK;
+}
+
+int check_rows(const char* who, const sf_paged_plan* p, const void* q, int64_t tok, int64_t head) {
+  const int vec = p->dtype == SF_DTYPE_BF16 ? 8 : 4;
+  if (!q || !aligned16(q) || tok % vec || head % vec || tok < 0 || head < p->hd)
+    return bad("%s: rows must be 16-byte aligned, head stride at least head_dim", who);
+  return SF_OK;
+}
+
+int status(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return SF_OK;
+  char buf[256];
+  snprintf(buf, sizeof(buf), "%s: %s", what, cudaGetErrorString(e));
+  return report(SF_ERR_CUDA, buf);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t sf_paged_plan_words(const sf_paged_plan* plan, const int32_t* q_lens, const int32_t* kv_lens) {
+  if (check_plan(plan, q_lens, kv_lens) != SF_OK) return 0;
+  sf_paged_plan p = *plan;
+  p.sms = device_sms(p.sms);
+  const Tiling t = tiling(p);
+  int64_t items = 0, mass = 0, tokens = 0;
+  for (int b = 0; b < p.B; ++b) {
+    const int k = which(t, q_lens[b], p.H / p.Hkv);
+    items += static_cast<int64_t>((q_lens[b] + t.per_tile[k] - 1) / t.per_tile[k]) * p.Hkv;
+    if (q_lens[b] > 0) mass += static_cast<int64_t>((kv_lens[b] + kPagedKB - 1) / kPagedKB) * p.Hkv;
+    tokens += q_lens[b];
+  }
+  const int64_t w = t.workers[0] + t.workers[1];
+  const int64_t words = (items + w) * kItemWords + w * kMergeWords + 2 * (w + 16) + mass * kMassWords +
+                        (t.mass_workers + p.B * static_cast<int64_t>(p.Hkv)) * kMassWords + t.mass_workers + 16 + 2 * tokens + 64;
+  if (words > kMaxWords) {
+    bad("paged plan: the step is too large");
+    return 0;
+  }
+  return words;
+}
+
+int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_t* kv_lens, int32_t* words,
+                        int64_t cap) {
+  const int64_t need = sf_paged_plan_words(plan, q_lens, kv_lens);
+  if (need == 0) return SF_ERR_ARG;
+  if (!words || cap < need)
+    return bad("paged plan: %lld words given, %lld needed", static_cast<long long>(cap), static_cast<long long>(need));
+  try {
+    sf_paged_plan& p = *plan;
+    p.sms = device_sms(p.sms);
+    const int G = p.H / p.Hkv;
+    const Tiling t = tiling(p);
+    p.T = 0;
+    p.max_kv = 0;
+    p.short_chunk = 0;
+    int64_t at = 0;
+    // {sequence, position} of every new token
+    p.tokens = 0;
+    for (int b = 0; b < p.B; ++b) {
+      for (int i = 0; i < q_lens[b]; ++i) {
+        words[at++] = b;
+        words[at++] = kv_lens[b] - q_lens[b] + i;
+      }
+      p.T += q_lens[b];
+      if (q_lens[b] > 0) p.max_kv = std::max(p.max_kv, kv_lens[b]);
+      if (q_lens[b] > kv_lens[b]) p.short_chunk = 1;
+    }
+    at = up4(at);
+    p.ws_bytes = 0;
+    for (int k = 0; k < 2; ++k) {
+      std::vector<PagedItem> tiles, items;
+      std::vector<PagedMerge> merges;
+      std::vector<int32_t> first;
+      int q0 = 0;
+      for (int b = 0; b < p.B; q0 += q_lens[b], ++b) {
+        if (q_lens[b] == 0 || which(t, q_lens[b], G) != k) continue;
+        const PagedMask mask{p.block, p.window, p.sinks, q_lens[b], kv_lens[b]};
+        for (int h = 0; h < p.Hkv; ++h)
+          for (int t0 = 0; t0 < q_lens[b]; t0 += t.per_tile[k]) {
+            PagedItem it{};
+            it.seq = b;
+            it.kvh = h;
+            it.tok0 = t0;
+            it.ntok = std::min(t.per_tile[k], q_lens[b] - t0);
+            it.slot = -1;
+            const int hi = std::max(0, mask.hi(t0 + it.ntok - 1));
+            const int end = (hi + kPagedKB - 1) / kPagedKB;
+            it.lo_blk = std::min(mask.lo(t0) / kPagedKB, end);
+            it.sink_blks = std::min((std::min(p.sinks, hi) + kPagedKB - 1) / kPagedKB, it.lo_blk);
+            it.i1 = it.sink_blks + end - it.lo_blk;
+            it.q0 = q0;
+            it.q_len = q_lens[b];
+            it.kv_len = kv_lens[b];
+            tiles.push_back(it);
+          }
+      }
+      sf_paged_list& l = p.attn[k];
+      l = sf_paged_list{};
+      l.rows = t.rows[k];
+      l.tile_tokens = t.tokens[k];
+      if (!tiles.empty()) {
+        int slots = 0;
+        deal(tiles, t.workers[k], &items, &first, &merges, &slots);
+        l.slots = slots;
+        l.n_items = static_cast<int32_t>(items.size());
+        l.workers = static_cast<int32_t>(first.size()) - 1;
+        l.n_merges = static_cast<int32_t>(merges.size());
+      }
+      l.items = static_cast<int32_t>(at);
+      memcpy(words + at, items.data(), items.size() * sizeof(PagedItem));
+      at += static_cast<int64_t>(items.size()) * kItemWords;
+      l.merges = static_cast<int32_t>(at);
+      memcpy(words + at, merges.data(), merges.size() * sizeof(PagedMerge));
+      at += static_cast<int64_t>(merges.size()) * kMergeWords;
+      l.first = static_cast<int32_t>(at);
+      memcpy(words + at, first.data(), first.size() * 4);
+      at = up4(at + static_cast<int64_t>(first.size()));
+      p.ws_bytes += list_ws(l, p.hd);
+    }
+    // weight accumulation: runs of key blocks of equal cost (query tiles + 1 per block)
+    {
+      std::vector<PagedMassItem> items;
+      std::vector<int32_t> first;
+      const int tile = std::max(1, t.mass_rows / G);
+      struct Unit {
+        int64_t cost;
+        PagedMassItem item;
+      };
+      std::vector<Unit> units;
+      int64_t total = 0, top = 0;
+      int q0 = 0;
+      for (int b = 0; b < p.B; q0 += q_lens[b], ++b) {
+        if (q_lens[b] == 0) continue;
+        const PagedMask mask{p.block, p.window, p.sinks, q_lens[b], kv_lens[b]};
+        const int nb = (kv_lens[b] + kPagedKB - 1) / kPagedKB;
+        for (int h = 0; h < p.Hkv; ++h)
+          for (int kb = 0; kb < nb; ++kb) {
+            int f, e;
+            mask.tokens(kb, &f, &e);
+            if (f >= e) continue;
+            Unit u{(e - f + tile - 1) / tile + 1, {b, h, kb, kb + 1, q0, q_lens[b], kv_lens[b], 0}};
+            total += u.cost;
+            top = std::max(top, u.cost);
+            units.push_back(u);
+          }
+      }
+      sf_paged_list& l = p.mass;
+      l = sf_paged_list{};
+      if (!units.empty()) {
+        const int w = static_cast<int>(std::min<int64_t>(t.mass_workers, static_cast<int64_t>(units.size())));
+        if (top * 4 * w > total) {
+          // blocks that are a good part of a worker's share: the dearest first, each to the
+          // worker with the least so far
+          std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.cost > b.cost; });
+          std::vector<std::vector<PagedMassItem>> of(w);
+          typedef std::pair<int64_t, int> Load;
+          std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
+          for (int i = 0; i < w; ++i) least.push({0, i});
+          for (const Unit& u : units) {
+            Load x = least.top();
+            least.pop();
+            of[x.second].push_back(u.item);
+            x.first += u.cost;
+            least.push(x);
+          }
+          for (int i = 0; i < w; ++i) {
+            first.push_back(static_cast<int32_t>(items.size()));
+            items.insert(items.end(), of[i].begin(), of[i].end());
+          }
+        } else {
+          int64_t done = 0;
+          int worker = -1;
+          for (const Unit& u : units) {
+            const int mine = static_cast<int>(std::min<int64_t>(w - 1, done * w / total));
+            const bool fresh = mine != worker;
+            while (worker < mine) {
+              first.push_back(static_cast<int32_t>(items.size()));
+              ++worker;
+            }
+            if (!fresh && !items.empty() && items.back().seq == u.item.seq && items.back().kvh == u.item.kvh &&
+                items.back().kb1 == u.item.kb0)
+              items.back().kb1 = u.item.kb1;
+            else
+              items.push_back(u.item);
+            done += u.cost;
+          }
+          while (static_cast<int>(first.size()) < w) first.push_back(static_cast<int32_t>(items.size()));
+        }
+        first.push_back(static_cast<int32_t>(items.size()));
+        l.workers = w;
+        l.n_items = static_cast<int32_t>(items.size());
+      }
+      l.items = static_cast<int32_t>(at);
+      memcpy(words + at, items.data(), items.size() * sizeof(PagedMassItem));
+      at += static_cast<int64_t>(items.size()) * kMassWords;
+      l.first = static_cast<int32_t>(at);
+      memcpy(words + at, first.data(), first.size() * 4);
+      at = up4(at + static_cast<int64_t>(first.size()));
+    }
+    p.words = std::max<int64_t>(at, 4);
+    p.dev = nullptr;
+    p.ws = nullptr;
+    p.err = nullptr;
+    return SF_OK;
+  } catch (const std::exception& e) {
+    return bad("paged plan: %s", e.what());
+  }
+}
+
+int sf_paged_kv_append(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* k_new, const void* v_new,
+                       int64_t new_tok_stride, int64_t new_head_stride, void* stream) {
+  int rc = check_ready("paged_kv_append", plan);
+  if (rc == SF_OK && plan->short_chunk) rc = bad("paged_kv_append: a sequence has more new tokens than cached keys");
+  if (rc != SF_OK || plan->T == 0) return rc;
+  if ((rc = check_pool("paged_kv_append", pool, plan->dtype, plan->hd, plan->page_size, plan->max_kv, true, false)) != SF_OK ||
+      (rc = check_rows("paged_kv_append", plan, k_new, new_tok_stride, new_head_stride)) != SF_OK ||
+      (rc = check_rows("paged_kv_append", plan, v_new, new_tok_stride, new_head_stride)) != SF_OK)
+    return rc;
+  PagedAppendParams p{};
+  p.k_new = k_new;
+  p.v_new = v_new;
+  p.new_tok = new_tok_stride;
+  p.new_head = new_head_stride;
+  p.pool = pool_of(*pool, plan->page_size);
+  p.tokens = plan->dev + plan->tokens;
+  p.T = plan->T;
+  p.Hkv = plan->Hkv;
+  p.hd = plan->hd;
+  p.err = plan->err;
+  return status(launch_paged_append(plan->dtype, p, static_cast<cudaStream_t>(stream)), "paged_kv_append");
+}
+
+int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* q, int64_t q_tok_stride,
+                       int64_t q_head_stride, void* out, float* lse, float scale, void* stream) {
+  int rc = check_ready("paged_attention", plan);
+  if (rc != SF_OK || plan->T == 0) return rc;
+  if ((rc = check_pool("paged_attention", pool, plan->dtype, plan->hd, plan->page_size, plan->max_kv, true, false)) != SF_OK ||
+      (rc = check_rows("paged_attention", plan, q, q_tok_stride, q_head_stride)) != SF_OK)
+    return rc;
+  if (!out || !lse || !aligned16(out)) return bad("paged_attention: out and lse must be given, out 16-byte aligned");
+  if (!(scale > 0.f) || scale > 3.0e38f) return bad("paged_attention: scale must be positive");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  size_t off = 0;
+  for (int k = 0; k < 2; ++k) {
+    const sf_paged_list& l = plan->attn[k];
+    if (l.n_items == 0) continue;
+    PagedAttnParams p{};
+    p.q = q;
+    p.q_tok = q_tok_stride;
+    p.q_head = q_head_stride;
+    p.pool = pool_of(*pool, plan->page_size);
+    p.out = out;
+    p.lse = lse;
+    p.items = reinterpret_cast<const PagedItem*>(plan->dev + l.items);
+    p.first = plan->dev + l.first;
+    p.workers = l.workers;
+    p.merges = reinterpret_cast<const PagedMerge*>(plan->dev + l.merges);
+    p.n_merges = l.n_merges;
+    p.part_O = reinterpret_cast<float*>(static_cast<char*>(plan->ws) + off);
+    p.part_ml = p.part_O + static_cast<size_t>(l.slots) * l.rows * plan->hd;
+    off += list_ws(l, plan->hd);
+    p.rows = l.rows;
+    p.tile_tokens = l.tile_tokens;
+    p.H = plan->H;
+    p.Hkv = plan->Hkv;
+    p.G = plan->H / plan->Hkv;
+    p.hd = plan->hd;
+    p.T = plan->T;
+    p.block = plan->block;
+    p.window = plan->window;
+    p.sinks = plan->sinks;
+    p.scale = scale;
+    p.err = plan->err;
+    cudaError_t e = launch_paged_attention_simt(plan->dtype, p, st);
+    if (e == cudaSuccess) e = launch_paged_merge(plan->dtype, p, st);
+    if (e != cudaSuccess) return status(e, "paged_attention");
+  }
+  return SF_OK;
+}
+
+int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* q, int64_t q_tok_stride,
+                            int64_t q_head_stride, const float* lse, float scale, void* stream) {
+  int rc = check_ready("paged_attention_mass", plan);
+  if (rc != SF_OK || plan->mass.n_items == 0) return rc;
+  if ((rc = check_pool("paged_attention_mass", pool, plan->dtype, plan->hd, plan->page_size, plan->max_kv, false, true)) != SF_OK ||
+      (rc = check_rows("paged_attention_mass", plan, q, q_tok_stride, q_head_stride)) != SF_OK)
+    return rc;
+  if (!lse) return bad("paged_attention_mass: null lse");
+  if (!(scale > 0.f) || scale > 3.0e38f) return bad("paged_attention_mass: scale must be positive");
+  PagedMassParams p{};
+  p.q = q;
+  p.q_tok = q_tok_stride;
+  p.q_head = q_head_stride;
+  p.pool = pool_of(*pool, plan->page_size);
+  p.lse = lse;
+  p.items = reinterpret_cast<const PagedMassItem*>(plan->dev + plan->mass.items);
+  p.first = plan->dev + plan->mass.first;
+  p.workers = plan->mass.workers;
+  p.H = plan->H;
+  p.Hkv = plan->Hkv;
+  p.G = plan->H / plan->Hkv;
+  p.hd = plan->hd;
+  p.T = plan->T;
+  p.block = plan->block;
+  p.window = plan->window;
+  p.sinks = plan->sinks;
+  p.scale = scale;
+  p.err = plan->err;
+  return status(launch_paged_mass_simt(plan->dtype, p, static_cast<cudaStream_t>(stream)), "paged_attention_mass");
+}
+
+int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_table, int64_t dst_stride,
+                   int32_t dst_width, const int32_t* lens, int32_t max_len, int32_t max_keep, int B, int Hkv, int hd,
+                   int page_size, int sinks, int recent, int32_t* kept, int64_t kept_stride, int* err, void* stream) {
+  if (dtype != SF_DTYPE_F32 && dtype != SF_DTYPE_BF16) return bad("paged_evict: dtype %d not supported", dtype);
+  if (hd != 64 && hd != 128) return bad("paged_evict: head_dim %d must be 64 or 128", hd);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return bad("paged_evict: page size %d must be a power of two in [16, 256]", page_size);
+  if (B < 0 || Hkv < 1 || static_cast<int64_t>(B) * Hkv > 65535) return bad("paged_evict: %d sequences of %d heads", B, Hkv);
+  if (sinks < 0 || recent < 0 || max_len < 0 || max_keep < 0 || static_cast<int64_t>(sinks) + recent > max_keep)
+    return bad("paged_evict: sinks %d + recent %d do not fit the %d keys that stay", sinks, recent, max_keep);
+  if (B == 0) return SF_OK;
+  const int stay = std::min(max_len, max_keep);
+  if (stay == 0) return SF_OK;
+  if (!lens || !kept || !err || kept_stride < stay || kept_stride > INT32_MAX)
+    return bad("paged_evict: null argument or kept rows shorter than %d", stay);
+  int rc = check_pool("paged_evict", pool, dtype, hd, page_size, max_len, true, true);
+  if (rc != SF_OK) return rc;
+  if (static_cast<int64_t>(dst_width) * page_size < stay || dst_stride < dst_width)
+    return bad("paged_evict: a destination table of %d pages does not hold %d keys", dst_width, stay);
+  if (!dst_table) return bad("paged_evict: null destination table");
+  PagedEvictParams p{};
+  p.pool = pool_of(*pool, page_size);
+  p.dst = dst_table;
+  p.dst_stride = dst_stride;
+  p.lens = lens;
+  p.kept = kept;
+  p.kept_stride = static_cast<int>(kept_stride);
+  p.B = B;
+  p.Hkv = Hkv;
+  p.hd = hd;
+  p.sinks = sinks;
+  p.recent = recent;
+  p.max_len = max_len;
+  p.max_keep = max_keep;
+  p.err = err;
+  return status(launch_paged_evict(dtype, p, static_cast<cudaStream_t>(stream)), "paged_evict");
+}
+
+}  // extern "C"

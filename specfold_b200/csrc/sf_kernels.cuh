@@ -48,6 +48,9 @@ inline cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
   return e;
 }
 
+// records msg for sf_last_error() and returns code
+int report(int code, const char* msg);
+
 // number of kernels this library has launched (all threads, all devices)
 void count_launch(int n = 1);
 // launch status of the kernel just launched; counts it when it launched

@@ -7,7 +7,8 @@ generator calls the whole-forward entry point instead.
 
 from __future__ import annotations
 
-from typing import Dict, Optional
+import ctypes
+from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -295,3 +296,236 @@ def kv_append(cache_k, cache_v, new_k, new_v, P):
         dtype_code(cache_k), cache_k.data_ptr(), cache_v.data_ptr(), cache_k.stride(0),
         new_k.data_ptr(), new_v.data_ptr(), new_k.stride(0), Hkv, hd, P, n, _stream()),
         "kv_append")
+
+
+# ---------------------------------------------------------------------------- paged cache
+def _int32(lens) -> torch.Tensor:
+    t = torch.as_tensor(lens, dtype=torch.int64).reshape(-1)
+    if t.is_cuda:
+        raise ValueError("lengths are host integers (the split of the work is made on the host)")
+    if t.numel() and (int(t.min()) < 0 or int(t.max()) > 1 << 30):
+        raise ValueError("lengths must lie in [0, 2^30]")
+    return t.to(torch.int32)
+
+
+def _cuda_device(device) -> torch.device:
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError("specfold_b200 kernels run on a CUDA device")
+    return torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+
+
+class _OnStream:
+    """Device buffers made on one stream and used on others: a use on another stream waits for
+    their making and keeps them from being handed out again while it runs."""
+
+    def _made(self, device: torch.device, *tensors: torch.Tensor) -> None:
+        self.device = device
+        self._tensors = tensors
+        self._home = torch.cuda.current_stream(device)
+        self._ready = self._home.record_event()
+
+    def _stream(self) -> int:
+        st = torch.cuda.current_stream(self.device)
+        # (a capture begins after a synchronisation and may not wait for what it did not record)
+        if st != self._home and not torch.cuda.is_current_stream_capturing():
+            st.wait_event(self._ready)
+            for t in self._tensors:
+                t.record_stream(st)
+        return st.cuda_stream
+
+    def check(self) -> None:
+        """Raises what the kernels reported (a page id outside the pool, a wait that ran out).
+        Synchronises with the device."""
+        raise_device_error(self.err)
+
+
+class PagedPlan(_OnStream):
+    """One step of a batch over a paged cache: how its work is split over the SMs, the scratch
+    and the error word of its calls.  Made once per step from the lengths on the host and used
+    by every layer; calls that share a plan must not overlap on the GPU.
+
+    ``q_lens[b]`` new tokens of sequence b see its ``kv_lens[b]`` cached keys (the new ones
+    included): all up to the end of their own block of ``block`` tokens (1: causal, N:
+    block-causal, 0: all), and with ``window`` > 0 only those less than ``window`` positions
+    back and the first ``sinks``."""
+
+    def __init__(self, q_lens: Sequence[int], kv_lens: Sequence[int], *, heads: int, kv_heads: int,
+                 head_dim: int, page_size: int, dtype: torch.dtype = torch.bfloat16, block: int = 1,
+                 window: int = 0, sinks: int = 0, device="cuda"):
+        q, n = _int32(q_lens), _int32(kv_lens)
+        if q.numel() != n.numel():
+            raise ValueError(f"{q.numel()} chunk lengths for {n.numel()} cache lengths")
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"unsupported dtype {dtype}; the kernels take float32 or bfloat16")
+        lib = _lib.load()
+        c = _lib.SfPagedPlan(dtype=_lib.SF_DTYPE_BF16 if dtype == torch.bfloat16 else _lib.SF_DTYPE_F32,
+                             B=q.numel(), H=heads, Hkv=kv_heads, hd=head_dim, page_size=page_size,
+                             block=block, window=window, sinks=sinks)
+        device = _cuda_device(device)
+        c.sms = torch.cuda.get_device_properties(device).multi_processor_count
+        cap = lib.sf_paged_plan_words(ctypes.byref(c), q.data_ptr(), n.data_ptr())
+        if cap <= 0:
+            _lib.check(_lib.SF_ERR_ARG, "paged plan")
+        words = torch.empty(cap, dtype=torch.int32)
+        _lib.check(lib.sf_paged_plan_build(ctypes.byref(c), q.data_ptr(), n.data_ptr(),
+                                           words.data_ptr(), cap), "paged plan")
+        self.dtype, self.tokens, self.sequences = dtype, c.T, c.B
+        self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
+        self._dev = words[:c.words].to(device)
+        self._ws = torch.empty(max(c.ws_bytes, 256), dtype=torch.uint8, device=device)
+        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        c.dev, c.ws, c.err = self._dev.data_ptr(), self._ws.data_ptr(), self.err.data_ptr()
+        self._c = c
+        self._ref = ctypes.byref(c)
+        self._made(device, self._dev, self._ws, self.err)
+
+
+class EvictPlan(_OnStream):
+    """What an eviction needs on the device: of ``kv_lens[b]`` cached keys ``keep`` (or
+    ``keep[b]``) stay, the first ``sinks`` and the last ``recent`` among them."""
+
+    def __init__(self, kv_lens: Sequence[int], keep: Union[int, Sequence[int]], *, kv_heads: int,
+                 page_size: int, sinks: int = 0, recent: int = 0, device="cuda"):
+        n = _int32(kv_lens)
+        k = _int32([keep] * n.numel() if isinstance(keep, int) else keep)
+        if k.numel() != n.numel():
+            raise ValueError(f"{k.numel()} budgets for {n.numel()} cache lengths")
+        if sinks < 0 or recent < 0:
+            raise ValueError("sinks and recent must not be negative")
+        if bool(((n > k) & (k < sinks + recent)).any()):
+            raise ValueError(f"sinks {sinks} + recent {recent} do not fit a budget that evicts")
+        device = _cuda_device(device)
+        self.sequences, self.kv_heads, self.page_size = n.numel(), kv_heads, page_size
+        self.sinks, self.recent = sinks, recent
+        self.stay = torch.minimum(n, k).tolist()
+        self.max_len = int(n.max()) if n.numel() else 0
+        # budgets above every length evict nothing: sinks + recent then bounds nothing
+        self.max_keep = max(int(k.max()) if n.numel() else 0, sinks + recent)
+        self.kept = max(self.stay, default=0)
+        self._lens = torch.stack((n, k), 1).contiguous().to(device)
+        self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self._made(device, self._lens, self.err)
+
+
+def _aligned_rows(t: torch.Tensor, what: str) -> Tuple[int, int]:
+    """(outer, head) strides of [N, H, hd] rows; those of an axis of one element are not used"""
+    if t.stride(2) != 1:
+        raise ValueError(f"{what}: head_dim must be contiguous")
+    H, hd = t.shape[1], t.shape[2]
+    head = t.stride(1) if H > 1 else hd
+    return (t.stride(0) if t.shape[0] > 1 else H * head), head
+
+
+def _paged_pool(k_pages, v_pages, table, mass_pages, plan, dtype):
+    if k_pages.dim() != 4:
+        raise ValueError("pools are [pages, kv heads, page size, head_dim]")
+    N, Hkv, ps, hd = k_pages.shape
+    if Hkv != plan.kv_heads or ps != plan.page_size or k_pages.dtype != dtype or k_pages.stride(3) != 1:
+        raise ValueError(f"the plan is for {dtype} pools of {plan.kv_heads} kv heads and pages of "
+                         f"{plan.page_size}, got {k_pages.dtype} {tuple(k_pages.shape)}")
+    if v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != dtype
+                                or v_pages.stride() != k_pages.stride()):
+        raise ValueError("k_pages and v_pages must share shape, dtype and strides")
+    if mass_pages is not None and (mass_pages.shape != (N, Hkv, ps) or mass_pages.dtype != torch.float32
+                                   or not mass_pages.is_contiguous()):
+        raise ValueError(f"mass_pages must be contiguous float32 {(N, Hkv, ps)}")
+    if (table.dim() != 2 or table.shape[0] != plan.sequences or table.dtype != torch.int32
+            or (table.shape[1] > 1 and table.stride(1) != 1)):
+        raise ValueError(f"the table must be int32 [{plan.sequences}, pages], rows contiguous")
+    dev = plan.device
+    for t in (k_pages, v_pages, mass_pages, table):
+        if t is not None and t.device != dev:
+            raise ValueError(f"the plan lives on {dev}, got a tensor on {t.device}")
+    return _lib.SfPagedPool(
+        k_pages.data_ptr(), _ptr(v_pages), _ptr(mass_pages),
+        k_pages.stride(0) if N > 1 else Hkv * ps * hd, k_pages.stride(1) if Hkv > 1 else ps * hd,
+        k_pages.stride(2), table.data_ptr(),
+        table.stride(0) if table.shape[0] > 1 else table.shape[1], N, table.shape[1])
+
+
+def _paged_rows(t: torch.Tensor, heads: int, plan: PagedPlan, what: str) -> Tuple[int, int]:
+    if t.shape != (plan.tokens, heads, plan.head_dim) or t.dtype != plan.dtype or t.device != plan.device:
+        raise ValueError(f"{what} must be {plan.dtype} {(plan.tokens, heads, plan.head_dim)} on "
+                         f"{plan.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return _aligned_rows(t, what)
+
+
+def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k_new: torch.Tensor,
+                    v_new: torch.Tensor, table: torch.Tensor, plan: PagedPlan,
+                    mass_pages: Optional[torch.Tensor] = None) -> None:
+    """The new tokens' keys and values [T, Hkv, hd] (strided rows, e.g. slices of a fused
+    projection's output) into their sequences' pages (sf_paged_kv_append); their accumulated
+    weights start at zero."""
+    pool = _paged_pool(k_pages, v_pages, table, mass_pages, plan, plan.dtype)
+    tok, head = _paged_rows(k_new, plan.kv_heads, plan, "k_new")
+    if _paged_rows(v_new, plan.kv_heads, plan, "v_new") != (tok, head):
+        raise ValueError("k_new and v_new must share their strides")
+    with torch.cuda.device(plan.device):
+        _lib.check(_lib.load().sf_paged_kv_append(plan._ref, ctypes.byref(pool), k_new.data_ptr(),
+                                                  v_new.data_ptr(), tok, head, plan._stream()),
+                   "paged_kv_append")
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    table: torch.Tensor, plan: PagedPlan, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of every sequence's new tokens q [T, H, hd] over its pages, under the plan's
+    mask (sf_paged_attention).  Returns (out [T, H, hd], lse [T, H] float32); a token that sees
+    no key gets zeros and -inf.  ``scale`` defaults to head_dim ** -0.5."""
+    pool = _paged_pool(k_pages, v_pages, table, None, plan, plan.dtype)
+    tok, head = _paged_rows(q, plan.heads, plan, "q")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
+        raise ValueError("out must be contiguous, of q's shape, dtype and device")
+    if lse is None:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+        raise ValueError("lse must be contiguous float32 [T, H] on q's device")
+    with torch.cuda.device(plan.device):
+        _lib.check(_lib.load().sf_paged_attention(
+            plan._ref, ctypes.byref(pool), q.data_ptr(), tok, head, out.data_ptr(), lse.data_ptr(),
+            plan.head_dim ** -0.5 if scale is None else scale, plan._stream()), "paged_attention")
+    return out, lse
+
+
+def paged_attention_mass(q: torch.Tensor, k_pages: torch.Tensor, table: torch.Tensor,
+                         lse: torch.Tensor, mass_pages: torch.Tensor, plan: PagedPlan,
+                         scale: Optional[float] = None) -> None:
+    """Adds to every cached key's accumulated weight what the new tokens' softmax gave it,
+    summed over tokens and the query heads of its kv head (sf_paged_attention_mass); ``lse`` is
+    paged_attention's."""
+    pool = _paged_pool(k_pages, None, table, mass_pages, plan, plan.dtype)
+    tok, head = _paged_rows(q, plan.heads, plan, "q")
+    if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+        raise ValueError("lse must be contiguous float32 [T, H] on q's device")
+    with torch.cuda.device(plan.device):
+        _lib.check(_lib.load().sf_paged_attention_mass(
+            plan._ref, ctypes.byref(pool), q.data_ptr(), tok, head, lse.data_ptr(),
+            plan.head_dim ** -0.5 if scale is None else scale, plan._stream()),
+            "paged_attention_mass")
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass_pages: torch.Tensor,
+                table: torch.Tensor, dst_table: torch.Tensor, plan: EvictPlan) -> torch.Tensor:
+    """Cuts every sequence to its budget, per kv head by accumulated weight, and moves what
+    stays, in order, to the pages of ``dst_table``, which no source table may hold
+    (sf_paged_evict).  Returns the old positions of what stayed, int32 [B, Hkv, most kept],
+    -1 after the last."""
+    dtype = k_pages.dtype
+    code = dtype_code(k_pages)
+    pool = _paged_pool(k_pages, v_pages, table, mass_pages, plan, dtype)
+    if (dst_table.dim() != 2 or dst_table.shape[0] != plan.sequences or dst_table.dtype != torch.int32
+            or (dst_table.shape[1] > 1 and dst_table.stride(1) != 1) or dst_table.device != plan.device):
+        raise ValueError(f"dst_table must be int32 [{plan.sequences}, pages] on {plan.device}")
+    kept = torch.empty(plan.sequences, plan.kv_heads, plan.kept, dtype=torch.int32, device=plan.device)
+    with torch.cuda.device(plan.device):
+        _lib.check(_lib.load().sf_paged_evict(
+            code, ctypes.byref(pool), dst_table.data_ptr(),
+            dst_table.stride(0) if plan.sequences > 1 else dst_table.shape[1], dst_table.shape[1],
+            plan._lens.data_ptr(), plan.max_len, plan.max_keep, plan.sequences, plan.kv_heads,
+            k_pages.shape[3], plan.page_size, plan.sinks, plan.recent, kept.data_ptr(), plan.kept,
+            plan.err.data_ptr(), plan._stream()), "paged_evict")
+    return kept
