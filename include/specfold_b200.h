@@ -356,7 +356,7 @@ int sf_parent_map(const int64_t* ids, int B1, int N, int64_t* par_idx, void* str
  *
  * head_dim 64 or 128, H / Hkv <= 16, page_size a power of two in [16, 256].               */
 typedef struct sf_paged_list {       /* one kernel's share of a plan (offsets in words) */
-  int32_t items, n_items, first, workers, merges, n_merges, slots, rows, tile_tokens, pad;
+  int32_t items, n_items, first, workers, merges, n_merges, slots, rows, tile_tokens, max_rows;
 } sf_paged_list;
 
 typedef struct sf_paged_plan {

@@ -48,7 +48,7 @@ class SfVerifyArgs(C.Structure):
 
 class SfPagedList(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("items", "n_items", "first", "workers", "merges", "n_merges",
-                                         "slots", "rows", "tile_tokens", "pad")]
+                                         "slots", "rows", "tile_tokens", "max_rows")]
 
 
 class SfPagedPlan(C.Structure):

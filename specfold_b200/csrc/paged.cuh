@@ -143,6 +143,8 @@ __device__ __forceinline__ int paged_page(const PagedPool& p, int seq, int idx, 
 }
 
 cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cudaStream_t st);
+cudaError_t launch_paged_attention_tokens(const PagedAttnParams& p, int copies, cudaStream_t st);
+cudaError_t launch_paged_attention_chunk(const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st);
 

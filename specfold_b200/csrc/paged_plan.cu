@@ -36,6 +36,17 @@ struct Tiling {
 Tiling tiling(const sf_paged_plan& p) {
   const int G = p.H / p.Hkv;
   Tiling t{};
+  if (p.dtype == SF_DTYPE_BF16) {
+    t.rows[0] = 128;
+    t.rows[1] = 256;
+    t.tokens[0] = t.tokens[1] = 128 / G;
+    t.per_tile[0] = t.tokens[0];
+    t.per_tile[1] = 2 * t.tokens[1];
+    t.workers[0] = t.workers[1] = p.sms;
+    t.mass_workers = 2 * p.sms;
+    t.mass_rows = 64;
+    return t;
+  }
   t.rows[0] = 16;
   t.rows[1] = 64;
   t.tokens[0] = 16 / G;
@@ -280,6 +291,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       l = sf_paged_list{};
       l.rows = t.rows[k];
       l.tile_tokens = t.tokens[k];
+      for (const PagedItem& it : tiles) l.max_rows = std::max(l.max_rows, it.ntok * G);
       if (!tiles.empty()) {
         int slots = 0;
         deal(tiles, t.workers[k], &items, &first, &merges, &slots);
@@ -453,7 +465,13 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
     p.sinks = plan->sinks;
     p.scale = scale;
     p.err = plan->err;
-    cudaError_t e = launch_paged_attention_simt(plan->dtype, p, st);
+    cudaError_t e;
+    if (plan->dtype == SF_DTYPE_BF16 && k == 0)
+      e = launch_paged_attention_tokens(p, l.max_rows <= 32 ? 4 : l.max_rows <= 64 ? 2 : 1, st);
+    else if (plan->dtype == SF_DTYPE_BF16)
+      e = launch_paged_attention_chunk(p, st);
+    else
+      e = launch_paged_attention_simt(plan->dtype, p, st);
     if (e == cudaSuccess) e = launch_paged_merge(plan->dtype, p, st);
     if (e != cudaSuccess) return status(e, "paged_attention");
   }

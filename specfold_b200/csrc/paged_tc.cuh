@@ -1,0 +1,126 @@
+// What the tensor-core kernels of the paged cache share: tensor maps of the pools and the
+// queries, the load of a key block by pages, and the device side of a bounded unwind.
+#pragma once
+
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "paged.cuh"
+
+namespace sf {
+
+// TMA load of one box of a 3-D / 4-D tensor map (coordinates in elements of each dimension)
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, uint64_t* bar, int c0, int c1,
+                                            int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* map, uint64_t* bar, int c0, int c1,
+                                            int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+// 32 lanes x 32 bits, 32 consecutive columns per thread
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+// 2^x by the hardware's approximation (2 units in the last place, below what any use here rounds
+// to); -inf gives 0
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr int kPagedBox = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzled
+
+// One warp loads the 128 rows of key block kb: [hd / 64][128 rows][64], 128-byte swizzle, a box
+// per page (or half page) and 64 columns.  Pages that no row of the tile sees are not read.
+// Completes on `bar` (one arrival with the bytes).
+template <int HD>
+__device__ __forceinline__ void load_key_block(unsigned char* dst, const void* map, uint64_t* bar,
+                                               const PagedPool& pool, const PagedItem& w,
+                                               const PagedRange& range, int kb, int lane, int* err) {
+  constexpr int KCH = HD / 64;
+  const int ps = 1 << pool.page_shift;
+  const int br = ps < 128 ? ps : 128;                   // rows of a box
+  const int boxes = 128 / br;
+  // lane l fetches box l / KCH, column chunk l % KCH
+  const int x = lane / KCH, c = lane % KCH;
+  const int k0 = kb * kPagedKB + x * br;
+  const bool mine = x < boxes && range.meets(k0, k0 + br);
+  int page = 0;
+  if (mine) page = paged_page(pool, w.seq, k0 >> pool.page_shift, err);
+  const unsigned n = __popc(__ballot_sync(0xffffffffu, mine));
+  if (lane == 0) mbar_arrive_expect_tx(bar, n * br * 128);
+  __syncwarp();
+  if (mine) tma_load_4d(dst + c * kPagedBox + x * br * 128, map, bar, c * 64, k0 & (ps - 1), w.kvh, page);
+}
+
+// ------------------------------------------------------------------ host side
+inline PFN_cuTensorMapEncodeTiled_v12000 paged_encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* ptr = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+inline bool paged_tmap(CUtensorMap* m, const void* ptr, int rank, const cuuint64_t* dims,
+                       const cuuint64_t* strides, const cuuint32_t* box) {
+  auto fn = paged_encode_fn();
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(ptr), dims, strides, box, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// a pool [num_pages][Hkv][page_size][hd]: boxes of 64 columns and a page (at most 128 rows of it)
+inline bool pool_tmap(CUtensorMap* m, const void* pages, const PagedPool& p, int Hkv, int hd) {
+  const cuuint64_t ps = 1ull << p.page_shift;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), ps, static_cast<cuuint64_t>(Hkv),
+                              static_cast<cuuint64_t>(p.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.row_stride) * 2, static_cast<cuuint64_t>(p.head_stride) * 2,
+                                 static_cast<cuuint64_t>(p.page_stride) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(ps < 128 ? ps : 128), 1, 1};
+  return paged_tmap(m, pages, 4, dims, strides, box);
+}
+// query rows [T][H][hd]: boxes of 64 columns, the G heads of a group and `tokens` tokens, which
+// land as rows token * G + g
+inline bool query_tmap(CUtensorMap* m, const void* q, int64_t tok, int64_t head, int T, int H, int hd, int G,
+                       int tokens) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(T)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head) * 2, static_cast<cuuint64_t>(tok) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(tokens)};
+  return paged_tmap(m, q, 3, dims, strides, box);
+}
+
+}  // namespace sf

@@ -6,8 +6,9 @@ from typing import List
 import torch
 
 # Rounding units.  U32: one fp32 rounding.  UW: what a bf16 kernel may lose in a softmax weight
-# before it is rounded to bf16 (an exponential good to 14 bits).  UB: one bf16 rounding.
-U32, UW, UB = 2.0 ** -24, 2.0 ** -14, 2.0 ** -9
+# before it is rounded to bf16 (an exponential good to 14 bits).  UB: one bf16 rounding (8
+# significant bits: half a unit of the last one is 2^-8 of the value at most).
+U32, UW, UB = 2.0 ** -24, 2.0 ** -14, 2.0 ** -8
 
 
 @dataclasses.dataclass
