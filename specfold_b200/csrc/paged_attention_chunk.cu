@@ -6,19 +6,98 @@
 //   warps 0-3, 4-7   softmax of tile 0 and of tile 1, a query row per thread
 //   warps 8-11       output: O out of TMEM, normalised, written
 //   warp 12          TMA: queries, and K and V blocks through a ring of 32 KB stages
-//   warp 13          issues tcgen05.mma
+//   warps 13, 14     issue tcgen05.mma, one warp per tile
 // While one tile's softmax runs, the tensor core works on the other tile: P V of the last block,
 // then S = Q K^T of the next.  S [128 x 128] fp32 and P (bf16, over S's first 64 columns) of
 // both tiles and both O fill the 512 columns of TMEM.  A tile's S of block j + 1 is issued after
 // its P V of block j, and its commit covers both: a softmax thread that sees S may change O, so
 // the (rare) rescaling needs no wait of its own.
 //
-// The rescaling waits until a row's maximum has grown by 2^8 (see paged_attention_tokens.cu).
+// The softmax's reference need not be the running maximum: any value that no weight outgrows by
+// more than 2^60, and that is no larger than the true maximum, gives the same quotient O / l with
+// the same relative rounding.  So a row takes the exact maximum of an item's first block, and
+// later blocks are only checked: the first 64 weights by their sum, the other 64 by their largest
+// score, found while the special-function unit works on the first.  A row that fails (or has
+// seen no key yet) sends its warp through the block again with the exact maximum.
 #include "paged_tc.cuh"
 
 namespace sf {
 
 constexpr int kChunkThreads = 512;
+
+// Of every 8 pairs of a block's second 64 weights, this many take the polynomial instead of the
+// special-function unit.
+constexpr int kPolyPairs = 4;
+
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the larger of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// the largest of 64, NaN if one is
+__device__ __forceinline__ float max64(const float* v) {
+  float m[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    m[c] = max3(v[c * 16], v[c * 16 + 1], v[c * 16 + 2]);
+#pragma unroll
+    for (int j = 3; j < 15; j += 2) m[c] = max3(m[c], v[c * 16 + j], v[c * 16 + j + 1]);
+  }
+  return max3(max3(m[0], m[1], v[15]), max3(m[2], m[3], v[31]), max3(v[47], v[63], v[63]));
+}
+// How far a row may outgrow its reference (see the head of the file): weights up to 2^60, which
+// bf16 and the fp32 sums hold.
+constexpr float kGrowth = 1152921504606846976.f, kGrowthLog2 = 60.f;
+
+// 2^x of a pair on the FMA and integer pipes: x = i + r with |r| <= 1/2, 2^r by the polynomial of
+// degree 4 with p(0) = 1 that is minimax in relative error on that interval (2.8e-6, found by
+// linear programming), i added to the exponent.  x <= -127 gives 0.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  const uint64_t t = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f);   // 1.5 * 2^23: the sum's low bits are i
+  const uint64_t z = add2(t, magic);
+  const uint64_t i = add2(z, pair(-12582912.f, -12582912.f));
+  const uint64_t r = fma2(i, pair(-1.f, -1.f), t);
+  uint64_t y = pair(0.009582576341927052f, 0.009582576341927052f);
+  y = fma2(y, r, pair(0.05590682849287987f, 0.05590682849287987f));
+  y = fma2(y, r, pair(0.24024106562137604f, 0.24024106562137604f));
+  y = fma2(y, r, pair(0.6931241154670715f, 0.6931241154670715f));
+  y = fma2(y, r, pair(1.f, 1.f));
+  float za, zb, ya, yb;
+  unpair(z, za, zb);
+  unpair(y, ya, yb);
+  return pair(__int_as_float(__float_as_int(ya) + (__float_as_int(za) << 23)),
+              __int_as_float(__float_as_int(yb) + (__float_as_int(zb) << 23)));
+}
+
+// shared-memory matrix descriptors of sf_common.cuh, in the two words an issue loop steps
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint64_t desc(uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(kDescHi));
+  return d;
+}
 
 template <int HD>
 struct ChunkSmem {
@@ -28,7 +107,7 @@ struct ChunkSmem {
   static constexpr int ring = q + 2 * kTile;             // [kStages][kTile]
   static constexpr int ml = ring + kStages * kTile;      // [2 tiles][m (log2 units), l][128]
   static constexpr int bars = ml + 2 * 2 * 128 * 4;
-  static constexpr int bytes = bars + (2 * kStages + 17) * 8 + 8;
+  static constexpr int bytes = bars + (2 * kStages + 20) * 8 + 8;
 };
 
 template <int HD>
@@ -39,7 +118,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int KCH = HD / 64, NS = L::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bars);
-  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 17);
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 20);
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
   if (smem_u32(sm) & 1023) {                             // the swizzled tiles need it; all threads see it
     flag_error(p.err, SF_DEV_ERR_TMEM);
@@ -55,28 +134,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* o_free = q_full + 10;
   uint64_t* ml_full = q_full + 12;
   uint64_t* ml_free = q_full + 14;
-  uint64_t* drain = q_full + 16;
+  uint64_t* p_half = q_full + 16;
+  uint64_t* drain = q_full + 18;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);                           // both tiles
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
+      mbar_init(&drain[t], 1);
       mbar_init(&o_free[t], 4);
       mbar_init(&ml_full[t], 4);
       mbar_init(&ml_free[t], 4);
     }
-    mbar_init(drain, 1);
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -93,7 +174,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int first = p.first[blockIdx.x], last = p.first[blockIdx.x + 1];
   const int tq = p.tile_tokens;                          // tokens of one tile
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 12) {
       // -------------------------------------------------------------- TMA
       uint32_t u = 0;                                    // ring units issued (K and V blocks)
@@ -106,7 +187,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
         const int tiles = w.ntok > tq ? 2 : 1;
         auto load_q = [&](int t) {
-          ok = __all_sync(0xffffffffu, !abort_flag && mbar_wait(&q_empty[t], (qn[t] & 1) ^ 1, p.err));
+          ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[t], (qn[t] & 1) ^ 1, p.err, &abort_flag));
           if (!ok) return;
           if (lane == 0) mbar_arrive_expect_tx(&q_full[t], KCH * tq * p.G * 128);
           __syncwarp();
@@ -121,7 +202,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (i == w.i0 && kv < tiles) load_q(kv);
             if (!ok) break;
             const int s = u % NS;
-            ok = __all_sync(0xffffffffu, !abort_flag && mbar_wait(&empty[s], ((u / NS) & 1) ^ 1, p.err));
+            ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((u / NS) & 1) ^ 1, p.err, &abort_flag));
             if (!ok) break;
             load_key_block<HD>(sm + L::ring + s * L::kTile, kv ? &tmV : &tmK, &full[s], p.pool, w, range, w.block(i),
                                lane, p.err);
@@ -133,84 +214,80 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int t = 0; t < 2; ++t)
           if (qn[t] > 0) mbar_wait(&q_full[t], (qn[t] - 1) & 1, p.err);
       }
-    } else if (warp == 13 && lane == 0) {
+    } else if (warp <= 14 && elect_one()) {
       // -------------------------------------------------------------- MMA
+      // One warp per tile: a commit holds its thread until the tensor core has run what was
+      // issued before it, and the other tile's products must be in the queue by then.
+      const int t = warp - 13;
       const uint32_t id_s = idesc_bf16(128, kPagedKB);
       const uint32_t id_pv = idesc_bf16(128, HD, 0, 1);
-      uint32_t n = 0;                                    // block of the stream whose P V comes next
-      uint32_t sn[2] = {0, 0}, on[2] = {0, 0};           // blocks, items of each tile
-      uint32_t qn[2] = {0, 0};
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return !abort_flag && mbar_wait(bar, parity, p.err); };
-      // S of tile t for block x of the stream (the i-th of an item's [i0, i1))
-      auto issue_s = [&](int t, uint32_t x, bool begin, bool end) -> bool {
-        const uint32_t u = 2 * x;
-        if (begin && !wait(&q_full[t], qn[t]++ & 1)) return false;
-        if (!wait(&full[u % NS], (u / NS) & 1)) return false;
+      const uint32_t ring_lo = smem_u32(sm + L::ring) >> 4;
+      const uint32_t q_lo = ((smem_u32(sm + L::q) + t * L::kTile) >> 4) | (1u << 16);
+      const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
+      uint32_t x = 0, sn = 0, on = 0, qn = 0;            // blocks of the stream; this tile's blocks, items
+      uint32_t due_u = 0;                                // the ring unit of V of the block whose P V is due
+      bool ok = true, due = false, due_begin = false, due_end = false;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, p.err, &abort_flag); };
+      auto issue_pv = [&]() -> bool {
+        const uint32_t s = due_u % NS;
+        const uint32_t v_lo = (ring_lo + s * (L::kTile >> 4)) | ((kPagedBox >> 4) << 16);
+        if (due_begin && !wait(&o_free[t], (on++ & 1) ^ 1)) return false;
+        if (!wait(&full[s], (due_u / NS) & 1) || !wait(&p_half[t], sn & 1)) return false;
         tc_fence_after();
-        const uint32_t q_s = smem_u32(sm + L::q + t * L::kTile);
-        const uint32_t k_s = smem_u32(sm + L::ring + (u % NS) * L::kTile);
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          umma_f16(tmem + t * 128, sdesc_kmajor_sw128(q_s + (kk >> 2) * kPagedBox + (kk & 3) * 32),
-                   sdesc_kmajor_sw128(k_s + (kk >> 2) * kPagedBox + (kk & 3) * 32), id_s, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[t]);
-        if (end) umma_commit(&q_empty[t]);
+        for (int kk = 0; kk < 4; ++kk)
+          umma_f16_ts(tO, tS + kk * 8, desc(v_lo + kk * 128), id_pv, (!due_begin || kk > 0) ? 1u : 0u);
+        if (!wait(&p_full[t], sn++ & 1)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 4; kk < 8; ++kk) umma_f16_ts(tO, tS + kk * 8, desc(v_lo + kk * 128), id_pv, 1u);
         return true;
       };
-      int it = first;
-      while (it < last && p.items[it].i0 == p.items[it].i1) ++it;
-      if (it < last) {
-        int i0 = p.items[it].i0, i1 = p.items[it].i1, tiles = p.items[it].ntok > tq ? 2 : 1, i = i0;
-        for (int t = 0; ok && t < tiles; ++t) ok = issue_s(t, 0, true, i0 + 1 == i1);
-        if (ok) umma_commit(&empty[0]);
-        while (ok) {
-          // what follows block i: the next one of the item, or the first of the next item
-          const bool begin = i == i0, end = i + 1 == i1;
-          int nit = it, ni0 = i0, ni1 = i1, ntiles = tiles;
-          if (end) {
-            ++nit;
-            while (nit < last && p.items[nit].i0 == p.items[nit].i1) ++nit;
-            if (nit < last) {
-              ni0 = p.items[nit].i0;
-              ni1 = p.items[nit].i1;
-              ntiles = p.items[nit].ntok > tq ? 2 : 1;
-            }
-          }
-          const bool more = nit < last;
-          const int ni = end ? ni0 : i + 1;
-          const uint32_t u = 2 * n + 1;
-          for (int t = 0; ok && t < 2; ++t) {
-            if (t < tiles) {
-              if (begin) ok = wait(&o_free[t], (on[t]++ & 1) ^ 1);
-              ok = ok && wait(&p_full[t], sn[t]++ & 1) && wait(&full[u % NS], (u / NS) & 1);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t v_s = smem_u32(sm + L::ring + (u % NS) * L::kTile);
+      // the stage of V is free and, after an item's last block, O is done, with what was issued
+      auto commit_pv = [&]() {
+        umma_commit(&empty[due_u % NS]);
+        if (due_end) umma_commit(&o_done[t]);
+      };
+      for (int it = first; ok && it < last; ++it) {
+        const int i0 = p.items[it].i0, i1 = p.items[it].i1;
+        if (i0 == i1) continue;
+        const bool active = t == 0 || p.items[it].ntok > tq;
+        if (active) ok = wait(&q_full[t], qn++ & 1);
+        for (int i = i0; ok && i < i1; ++i, ++x) {
+          const uint32_t u = 2 * x, s = u % NS;
+          ok = wait(&full[s], (u / NS) & 1) && (!due || issue_pv());
+          if (!ok) break;
+          if (active) {
+            tc_fence_after();
+            const uint32_t k_lo = (ring_lo + s * (L::kTile >> 4)) | (1u << 16);
 #pragma unroll
-              for (int kk = 0; kk < kPagedKB / 16; ++kk)
-                umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
-                            sdesc_mnmajor_sw128(v_s + kk * 2048, kPagedBox), id_pv, (!begin || kk > 0) ? 1u : 0u);
-              if (end) umma_commit(&o_done[t]);
-              if (t + 1 == tiles) umma_commit(&empty[u % NS]);
-            }
-            if (more && t < ntiles) {
-              ok = issue_s(t, n + 1, end, ni + 1 == ni1);
-              if (ok && t + 1 == ntiles) umma_commit(&empty[(2 * n + 2) % NS]);
-            }
+            for (int kk = 0; kk < HD / 16; ++kk)
+              umma_f16(tS, desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
+                       desc(k_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id_s, kk > 0 ? 1u : 0u);
+            umma_commit(&s_full[t]);
+            umma_commit(&empty[s]);
+            if (i + 1 == i1) umma_commit(&q_empty[t]);
+          } else {
+            mbar_arrive(&empty[s]);
           }
-          if (!more) break;
-          ++n;
-          it = nit;
-          i0 = ni0;
-          i1 = ni1;
-          i = ni;
-          tiles = ntiles;
+          if (due) commit_pv();
+          due = active;
+          due_u = u + 1;
+          due_begin = i == i0;
+          due_end = i + 1 == i1;
+          if (!active) {
+            ok = wait(&full[(u + 1) % NS], ((u + 1) / NS) & 1);
+            mbar_arrive(&empty[(u + 1) % NS]);
+          }
         }
       }
+      if (ok && due) {
+        ok = issue_pv();
+        if (ok) commit_pv();
+      }
       if (!ok) abort_flag = 1;
-      umma_commit(drain);
-      mbar_wait(drain, 0, p.err);
+      umma_commit(&drain[t]);
+      mbar_wait(&drain[t], 0, p.err);
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- output
@@ -226,8 +303,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int rows = (min(w.ntok, (t + 1) * tq) - t * tq) * p.G;
         float m = -INFINITY, l = 0.f;
         if (any) {
-          ok = __all_sync(0xffffffffu, !abort_flag && mbar_wait(&ml_full[t], on[t] & 1, p.err) &&
-                                           mbar_wait(&o_done[t], on[t] & 1, p.err));
+          ok = __all_sync(0xffffffffu, wait_or_abort(&ml_full[t], on[t] & 1, p.err, &abort_flag) &&
+                                           wait_or_abort(&o_done[t], on[t] & 1, p.err, &abort_flag));
           if (!ok) break;
           ++on[t];
           tc_fence_after();
@@ -241,14 +318,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int64_t prow = static_cast<int64_t>(w.slot) * p.rows + t * 128 + r;
         const float f = w.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          float o[32];
+        for (int c = 0; c < HD; c += 16) {
+          float o[16];
           __syncwarp();
           if (any) {
-            tmem_ld32(tmem + 256 + t * 128 + lane_off + c, o);
+            tmem_ld16(tmem + 256 + t * 128 + lane_off + c, o);
             tmem_ld_wait();
           }
-          if (any && c + 32 == HD) {                     // O is read: the next item may begin
+          if (any && c + 16 == HD) {                     // O is read: the next item may begin
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_free[t]);
@@ -256,16 +333,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (r < rows) {
             if (!any || f == 0.f) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = 0.f;
+              for (int j = 0; j < 16; ++j) o[j] = 0.f;
             }
             if (w.slot >= 0) {
               float4* dst = reinterpret_cast<float4*>(p.part_O + prow * HD + c);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
             } else {
               uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * HD + c);
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
+              for (int j = 0; j < 2; ++j)
                 dst[j] = make_uint4(pack_bf16(o[8 * j] * f, o[8 * j + 1] * f), pack_bf16(o[8 * j + 2] * f, o[8 * j + 3] * f),
                                     pack_bf16(o[8 * j + 4] * f, o[8 * j + 5] * f), pack_bf16(o[8 * j + 6] * f, o[8 * j + 7] * f));
             }
@@ -284,15 +361,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (!ok) abort_flag = 1;
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
     const float sl2 = p.scale * 1.4426950408889634f;     // scores in log2 units
-    uint32_t n = 0, items = 0;                           // this tile's blocks and items
+    uint32_t n = 0, items = 0, x = 0;                    // this tile's blocks, items; blocks of the stream
     bool ok = true;
     for (int it = first; ok && it < last; ++it) {
       const PagedItem w = p.items[it];
+      if (t == 1 && w.ntok <= tq) x += w.i1 - w.i0;
       if (w.i0 == w.i1 || (t == 1 && w.ntok <= tq)) continue;
       const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
       const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
@@ -302,30 +380,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int hi = mask.hi(tok), lo = mask.lo(tok);
       const int hi_min = mask.hi(t0), lo_max = mask.lo(t1 - 1);
       float m = -INFINITY, l = 0.f;
-      for (int i = w.i0; i < w.i1; ++i, ++n) {
+      for (int i = w.i0; i < w.i1; ++i, ++n, ++x) {
         const int k0 = w.block(i) * kPagedKB;
-        ok = __all_sync(0xffffffffu, !abort_flag && mbar_wait(&s_full[t], n & 1, p.err));
+        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[t], n & 1, p.err, &abort_flag));
         if (!ok) break;
         tc_fence_after();
-        float v[128];
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld32(tS + c, v + c);
-        tmem_ld_wait();
-        if (k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks)) {
-          const int h = hi - k0, b = lo - k0, f = range.sinks - k0;
-#pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (!(j < h && (j >= b || j < f))) v[j] = -INFINITY;
-        }
-        float mx = fmaxf(v[0], v[1]);
-#pragma unroll
-        for (int j = 2; j < 128; j += 2) mx = fmaxf(mx, fmaxf(v[j], v[j + 1]));
-        mx *= sl2;
         // the keys of this block that no row sees hold whatever their pages do: weight 0 times
-        // that must be 0 (thread r of tile 0, whose blocks are all of the stream's, clears row r
-        // of V; tile 1's P V comes later)
-        if (t == 0 && (k0 < range.lo || k0 + kPagedKB > range.hi) && !range.has(k0 + r)) {
-          const uint32_t u = 2 * n + 1;
+        // that must be 0 (thread r clears row r of V; the other tile clears the same rows)
+        if ((k0 < range.lo || k0 + kPagedKB > range.hi) && !range.has(k0 + r)) {
+          const uint32_t u = 2 * x + 1;
           ok = mbar_wait(&full[u % NS], (u / NS) & 1, p.err);
           unsigned char* row = sm + L::ring + (u % NS) * L::kTile + r * 128;
 #pragma unroll
@@ -334,45 +397,102 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int y = 0; y < 8; ++y) *reinterpret_cast<uint4*>(row + c * kPagedBox + y * 16) = make_uint4(0, 0, 0, 0);
           fence_async_shared();
         }
-        const bool grew = valid && mx > m + 8.f;                  // also the first finite maximum of a row
-        if (__any_sync(0xffffffffu, grew)) {
-          const float alpha = grew ? ex2(m - mx) : 1.f;
-          if (grew) m = mx;
-          l *= alpha;
-          if (i > w.i0) {
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-              float o[16];
-              tmem_ld16(tO + c, o);
-              tmem_ld_wait();
-              uint32_t b[16];
+        const bool edge = k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks);
+        const int h = hi - k0, b = lo - k0, f = range.sinks - k0;
+        float v2[64];                                    // scores of the second half of the keys
+        tmem_ld32(tS + 64, v2);
+        tmem_ld32(tS + 96, v2 + 32);
+        uint32_t w1[32];                                 // weights of the first half
+        uint64_t sum;
+        const uint64_t scale2 = pair(sl2, sl2);
+        bool exact = i == w.i0;
+        while (true) {
+          float v1[64];
+          tmem_ld32(tS, v1);
+          tmem_ld32(tS + 32, v1 + 32);
+          tmem_ld_wait();
+          if (edge) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) b[j] = __float_as_uint(o[j] * alpha);
-              tmem_st16(tO + c, b);
+            for (int j = 0; j < 64; ++j) {
+              if (!(j < h && (j >= b || j < f))) v1[j] = -INFINITY;
+              if (!(j + 64 < h && (j + 64 >= b || j + 64 < f))) v2[j] = -INFINITY;
             }
           }
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l0 = 0.f, l1 = 0.f;
+          const float mx2 = max64(v2) * sl2;
+          if (exact) {
+            const float mx = max3(max64(v1) * sl2, mx2, mx2);
+            const bool grew = valid && !(mx <= m + 8.f);
+            const float alpha = grew ? ex2(m - mx) : 1.f;
+            if (grew) m = mx;
+            l *= alpha;
+            if (i > w.i0) {
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 16) {
+                float o[16];
+                tmem_ld16(tO + c, o);
+                tmem_ld_wait();
+                uint32_t e[16];
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t b[16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float e0 = ex2(fmaf(v[c + j], sl2, -ref)), e1 = ex2(fmaf(v[c + j + 1], sl2, -ref));
-            l0 += e0;
-            l1 += e1;
-            b[j / 2] = pack_bf16(e0, e1);
+                for (int j = 0; j < 16; ++j) e[j] = __float_as_uint(o[j] * alpha);
+                tmem_st16(tO + c, e);
+              }
+            }
           }
-          tmem_st16(tS + c / 2, b);
+          const float ref = m == -INFINITY ? 0.f : m;
+          const uint64_t ref2 = pair(-ref, -ref);
+          sum = pair(0.f, 0.f);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            float e0, e1;
+            unpair(fma2(pair(v1[2 * j], v1[2 * j + 1]), scale2, ref2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            sum = add2(sum, pair(e0, e1));
+            w1[j] = pack_bf16(e0, e1);
+          }
+          if (exact) break;
+          float s0, s1;
+          unpair(sum, s0, s1);
+          const bool fine = !valid || (m > -INFINITY && s0 + s1 <= kGrowth && mx2 <= m + kGrowthLog2);
+          if (__all_sync(0xffffffffu, fine)) break;
+          exact = true;
         }
-        l += l0 + l1;
+        tmem_st16(tS, w1);
+        tmem_st16(tS + 16, w1 + 16);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_half[t]);          // half of the keys: P V may begin
+        const float ref = m == -INFINITY ? 0.f : m;
+        const uint64_t ref2 = pair(-ref, -ref);
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t e[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const uint64_t y = fma2(pair(v2[c + 2 * j], v2[c + 2 * j + 1]), scale2, ref2);
+            float e0, e1;
+            if ((j & 7) < kPolyPairs) {
+              unpair(exp2_pair(y), e0, e1);
+            } else {
+              unpair(y, e0, e1);
+              e0 = ex2(e0);
+              e1 = ex2(e1);
+            }
+            sum = add2(sum, pair(e0, e1));
+            e[j] = pack_bf16(e0, e1);
+          }
+          tmem_st16(tS + 32 + c / 2, e);
+        }
+        float s0, s1;
+        unpair(sum, s0, s1);
+        l += s0 + s1;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      ok = __all_sync(0xffffffffu, ok && !abort_flag && mbar_wait(&ml_free[t], (items & 1) ^ 1, p.err));
+      ok = __all_sync(0xffffffffu, ok && wait_or_abort(&ml_free[t], (items & 1) ^ 1, p.err, &abort_flag));
       if (!ok) break;
       ++items;
       ml[t * 256 + r] = m;

@@ -57,6 +57,24 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Bounded wait that also ends when another role of the CTA gave up (sets *abort itself when the
+// time is up).  A phase that is complete costs one try.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, int* err, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (globaltimer() - t0 > kWaitNs) {
+      flag_error(err, SF_DEV_ERR_TIMEOUT);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
 constexpr int kPagedBox = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzled
 
 // One warp loads the 128 rows of key block kb: [hd / 64][128 rows][64], 128-byte swizzle, a box
