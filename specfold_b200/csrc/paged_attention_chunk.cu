@@ -7,27 +7,25 @@
 //   warps 8-11       output: O out of TMEM, normalised, written
 //   warp 12          TMA: queries, and K and V blocks through a ring of 32 KB stages
 //   warps 13, 14     issue tcgen05.mma, one warp per tile
-// While one tile's softmax runs, the tensor core works on the other tile: P V of the last block,
-// then S = Q K^T of the next.  S [128 x 128] fp32 and P (bf16, over S's first 64 columns) of
-// both tiles and both O fill the 512 columns of TMEM.  A tile's S of block j + 1 is issued after
-// its P V of block j, and its commit covers both: a softmax thread that sees S may change O, so
-// the (rare) rescaling needs no wait of its own.
+// A key block is worked on in two halves of 64 keys, each with its own S [128 x 64] in TMEM (its
+// weights P, in bf16, take the place of its first 32 columns).  While the softmax is on one half,
+// the tensor core adds P V of the other and writes the other's next S = Q K^T, so that the softmax
+// warps, which set the pace, find their next scores ready.  S of both tiles' halves and both O
+// fill the 512 columns of TMEM.
 //
 // The softmax's reference need not be the running maximum: any value that no weight outgrows by
 // more than 2^60, and that is no larger than the true maximum, gives the same quotient O / l with
-// the same relative rounding.  So a row takes the exact maximum of an item's first block, and
-// later blocks are only checked: the first 64 weights by their sum, the other 64 by their largest
-// score, found while the special-function unit works on the first.  A row that fails (or has
-// seen no key yet) sends its warp through the block again with the exact maximum.
+// the same relative rounding.  So a row takes the maximum of the first half block that it sees a
+// key of, and later halves only check their largest score against it; where a row outgrows it, the
+// reference moves and O is rescaled.
 #include "paged_tc.cuh"
 
 namespace sf {
 
 constexpr int kChunkThreads = 512;
 
-// Of every 8 pairs of a block's second 64 weights, this many take the polynomial instead of the
-// special-function unit.
-constexpr int kPolyPairs = 4;
+// Of every 8 pairs of weights, this many take the polynomial instead of the special-function unit.
+constexpr int kPolyPairs = 1;
 
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t d;
@@ -66,7 +64,7 @@ __device__ __forceinline__ float max64(const float* v) {
 }
 // How far a row may outgrow its reference (see the head of the file): weights up to 2^60, which
 // bf16 and the fp32 sums hold.
-constexpr float kGrowth = 1152921504606846976.f, kGrowthLog2 = 60.f;
+constexpr float kGrowthLog2 = 60.f;
 
 // 2^x of a pair on the FMA and integer pipes: x = i + r with |r| <= 1/2, 2^r by the polynomial of
 // degree 4 with p(0) = 1 that is minimax in relative error on that interval (2.8e-6, found by
@@ -107,7 +105,7 @@ struct ChunkSmem {
   static constexpr int ring = q + 2 * kTile;             // [kStages][kTile]
   static constexpr int ml = ring + kStages * kTile;      // [2 tiles][m (log2 units), l][128]
   static constexpr int bars = ml + 2 * 2 * 128 * 4;
-  static constexpr int bytes = bars + (2 * kStages + 20) * 8 + 8;
+  static constexpr int bytes = bars + (2 * kStages + 24) * 8 + 8;
 };
 
 template <int HD>
@@ -118,7 +116,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int KCH = HD / 64, NS = L::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bars);
-  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 20);
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 24);
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
   if (smem_u32(sm) & 1023) {                             // the swizzled tiles need it; all threads see it
     flag_error(p.err, SF_DEV_ERR_TMEM);
@@ -128,14 +126,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* empty = bars + NS;                           // [NS]
   uint64_t* q_full = bars + 2 * NS;                      // [2] and so on: one per tile
   uint64_t* q_empty = q_full + 2;
-  uint64_t* s_full = q_full + 4;
-  uint64_t* p_full = q_full + 6;
-  uint64_t* o_done = q_full + 8;
-  uint64_t* o_free = q_full + 10;
-  uint64_t* ml_full = q_full + 12;
-  uint64_t* ml_free = q_full + 14;
-  uint64_t* p_half = q_full + 16;
-  uint64_t* drain = q_full + 18;
+  uint64_t* o_done = q_full + 4;
+  uint64_t* o_free = q_full + 6;
+  uint64_t* ml_full = q_full + 8;
+  uint64_t* ml_free = q_full + 10;
+  uint64_t* pv_done = q_full + 12;
+  uint64_t* drain = q_full + 14;
+  uint64_t* s_full = q_full + 16;                        // [2 tiles][2 halves]
+  uint64_t* p_full = q_full + 20;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -149,9 +147,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 4);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s_full[2 * t + h], 1);
+        mbar_init(&p_full[2 * t + h], 4);
+      }
       mbar_init(&o_done[t], 1);
       mbar_init(&drain[t], 1);
       mbar_init(&o_free[t], 4);
@@ -174,7 +174,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int first = p.first[blockIdx.x], last = p.first[blockIdx.x + 1];
   const int tq = p.tile_tokens;                          // tokens of one tile
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 12) {
       // -------------------------------------------------------------- TMA
       uint32_t u = 0;                                    // ring units issued (K and V blocks)
@@ -219,71 +218,99 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // One warp per tile: a commit holds its thread until the tensor core has run what was
       // issued before it, and the other tile's products must be in the queue by then.
       const int t = warp - 13;
-      const uint32_t id_s = idesc_bf16(128, kPagedKB);
+      const uint32_t id_s = idesc_bf16(128, kPagedKB / 2);
       const uint32_t id_pv = idesc_bf16(128, HD, 0, 1);
       const uint32_t ring_lo = smem_u32(sm + L::ring) >> 4;
       const uint32_t q_lo = ((smem_u32(sm + L::q) + t * L::kTile) >> 4) | (1u << 16);
       const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * 128;
-      uint32_t x = 0, sn = 0, on = 0, qn = 0;            // blocks of the stream; this tile's blocks, items
-      uint32_t due_u = 0;                                // the ring unit of V of the block whose P V is due
-      bool ok = true, due = false, due_begin = false, due_end = false;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, p.err, &abort_flag); };
-      auto issue_pv = [&]() -> bool {
-        const uint32_t s = due_u % NS;
-        const uint32_t v_lo = (ring_lo + s * (L::kTile >> 4)) | ((kPagedBox >> 4) << 16);
-        if (due_begin && !wait(&o_free[t], (on++ & 1) ^ 1)) return false;
-        if (!wait(&full[s], (due_u / NS) & 1) || !wait(&p_half[t], sn & 1)) return false;
+      // parities of this tile's next block (bit 0), item (bit 1) and query tile (bit 2)
+      uint32_t par = 0;
+      // ring stage and parity of the stream's next K block; of the V block whose P V is due, with
+      // whether it begins and ends its item
+      uint32_t stage = 0, phase = 0;
+      uint32_t due_stage = NS, due_phase = 0;            // NS: none is due
+      bool due_begin = false, due_end = false, ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity & 1, p.err, &abort_flag); };
+      auto advance = [&]() {
+        phase ^= stage + 1 == NS;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+      };
+      // O += P V of half h of the block that is due
+      auto issue_pv = [&](int h) -> bool {
+        if (h == 0) {
+          if (due_begin) {
+            if (!wait(&o_free[t], (par >> 1) ^ 1)) return false;
+            par ^= 2;
+          }
+          if (!wait(&full[due_stage], due_phase)) return false;
+        }
+        if (!wait(&p_full[2 * t + h], par)) return false;
         tc_fence_after();
+        const uint32_t v_lo = (ring_lo + due_stage * (L::kTile >> 4) + h * 512) | ((kPagedBox >> 4) << 16);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_f16_ts(tO, tS + kk * 8, desc(v_lo + kk * 128), id_pv, (!due_begin || kk > 0) ? 1u : 0u);
-        if (!wait(&p_full[t], sn++ & 1)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 4; kk < 8; ++kk) umma_f16_ts(tO, tS + kk * 8, desc(v_lo + kk * 128), id_pv, 1u);
+          umma_f16_ts(tO, tS + h * 64 + kk * 8, desc(v_lo + kk * 128), id_pv, (!due_begin || h > 0 || kk > 0) ? 1u : 0u);
         return true;
       };
-      // the stage of V is free and, after an item's last block, O is done, with what was issued
-      auto commit_pv = [&]() {
-        umma_commit(&empty[due_u % NS]);
+      // after an item's last block O is done; the stage of V is free
+      auto commit_pv = [&](int h) {
+        umma_commit(&pv_done[t]);
+        if (h == 0) return;
+        umma_commit(&empty[due_stage]);
         if (due_end) umma_commit(&o_done[t]);
+        par ^= 1;
       };
+#pragma unroll 1
       for (int it = first; ok && it < last; ++it) {
         const int i0 = p.items[it].i0, i1 = p.items[it].i1;
         if (i0 == i1) continue;
         const bool active = t == 0 || p.items[it].ntok > tq;
-        if (active) ok = wait(&q_full[t], qn++ & 1);
-        for (int i = i0; ok && i < i1; ++i, ++x) {
-          const uint32_t u = 2 * x, s = u % NS;
-          ok = wait(&full[s], (u / NS) & 1) && (!due || issue_pv());
-          if (!ok) break;
-          if (active) {
-            tc_fence_after();
-            const uint32_t k_lo = (ring_lo + s * (L::kTile >> 4)) | (1u << 16);
+        if (active) {
+          ok = wait(&q_full[t], par >> 2);
+          par ^= 4;
+        }
+#pragma unroll 1
+        for (int left = i1 - i0; ok && left > 0; --left) {
+          ok = wait(&full[stage], phase);
+#pragma unroll 1
+          for (int h = 0; ok && h < 2; ++h) {
+            if (due_stage != NS) ok = issue_pv(h);
+            if (!ok) break;
+            if (active) {
+              tc_fence_after();
+              const uint32_t k_lo = (ring_lo + stage * (L::kTile >> 4) + h * 512) | (1u << 16);
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              umma_f16(tS, desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
-                       desc(k_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id_s, kk > 0 ? 1u : 0u);
-            umma_commit(&s_full[t]);
-            umma_commit(&empty[s]);
-            if (i + 1 == i1) umma_commit(&q_empty[t]);
+              for (int kk = 0; kk < HD / 16; ++kk)
+                umma_f16(tS + h * 64, desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
+                         desc(k_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id_s, kk > 0 ? 1u : 0u);
+              umma_commit(&s_full[2 * t + h]);
+              if (h == 1) {
+                umma_commit(&empty[stage]);
+                if (left == 1) umma_commit(&q_empty[t]);
+              }
+            } else if (h == 1) {
+              mbar_arrive(&empty[stage]);
+            }
+            if (due_stage != NS) commit_pv(h);
+          }
+          if (!ok) break;
+          advance();
+          if (active) {
+            due_stage = stage;
+            due_phase = phase;
+            due_begin = left == i1 - i0;
+            due_end = left == 1;
           } else {
-            mbar_arrive(&empty[s]);
+            due_stage = NS;
+            ok = wait(&full[stage], phase);
+            mbar_arrive(&empty[stage]);
           }
-          if (due) commit_pv();
-          due = active;
-          due_u = u + 1;
-          due_begin = i == i0;
-          due_end = i + 1 == i1;
-          if (!active) {
-            ok = wait(&full[(u + 1) % NS], ((u + 1) / NS) & 1);
-            mbar_arrive(&empty[(u + 1) % NS]);
-          }
+          advance();
         }
       }
-      if (ok && due) {
-        ok = issue_pv();
-        if (ok) commit_pv();
+      for (int h = 0; ok && due_stage != NS && h < 2; ++h) {
+        ok = issue_pv(h);
+        if (ok) commit_pv(h);
       }
       if (!ok) abort_flag = 1;
       umma_commit(&drain[t]);
@@ -291,7 +318,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- output
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     uint32_t on[2] = {0, 0};
@@ -318,14 +344,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int64_t prow = static_cast<int64_t>(w.slot) * p.rows + t * 128 + r;
         const float f = w.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
-          float o[16];
+        for (int c = 0; c < HD; c += 8) {
+          float o[8];
           __syncwarp();
           if (any) {
-            tmem_ld16(tmem + 256 + t * 128 + lane_off + c, o);
+            tmem_ld8(tmem + 256 + t * 128 + lane_off + c, o);
             tmem_ld_wait();
           }
-          if (any && c + 16 == HD) {                     // O is read: the next item may begin
+          if (any && c + 8 == HD) {                      // O is read: the next item may begin
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_free[t]);
@@ -333,18 +359,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (r < rows) {
             if (!any || f == 0.f) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = 0.f;
+              for (int j = 0; j < 8; ++j) o[j] = 0.f;
             }
             if (w.slot >= 0) {
               float4* dst = reinterpret_cast<float4*>(p.part_O + prow * HD + c);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+              dst[1] = make_float4(o[4], o[5], o[6], o[7]);
             } else {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * HD + c);
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                dst[j] = make_uint4(pack_bf16(o[8 * j] * f, o[8 * j + 1] * f), pack_bf16(o[8 * j + 2] * f, o[8 * j + 3] * f),
-                                    pack_bf16(o[8 * j + 4] * f, o[8 * j + 5] * f), pack_bf16(o[8 * j + 6] * f, o[8 * j + 7] * f));
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * HD + c) =
+                  make_uint4(pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f),
+                             pack_bf16(o[4] * f, o[5] * f), pack_bf16(o[6] * f, o[7] * f));
             }
           }
         }
@@ -361,7 +385,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (!ok) abort_flag = 1;
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
@@ -382,14 +405,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int i = w.i0; i < w.i1; ++i, ++n, ++x) {
         const int k0 = w.block(i) * kPagedKB;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[t], n & 1, p.err, &abort_flag));
-        if (!ok) break;
-        tc_fence_after();
         // the keys of this block that no row sees hold whatever their pages do: weight 0 times
-        // that must be 0 (thread r clears row r of V; the other tile clears the same rows)
+        // that must be 0 (thread r clears row r of V; others that do write the same zeros)
         if ((k0 < range.lo || k0 + kPagedKB > range.hi) && !range.has(k0 + r)) {
           const uint32_t u = 2 * x + 1;
-          ok = mbar_wait(&full[u % NS], (u / NS) & 1, p.err);
+          wait_or_abort(&full[u % NS], (u / NS) & 1, p.err, &abort_flag);
           unsigned char* row = sm + L::ring + (u % NS) * L::kTile + r * 128;
 #pragma unroll
           for (int c = 0; c < KCH; ++c)
@@ -398,34 +418,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           fence_async_shared();
         }
         const bool edge = k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks);
-        const int h = hi - k0, b = lo - k0, f = range.sinks - k0;
-        float v2[64];                                    // scores of the second half of the keys
-        tmem_ld32(tS + 64, v2);
-        tmem_ld32(tS + 96, v2 + 32);
-        uint32_t w1[32];                                 // weights of the first half
-        uint64_t sum;
-        const uint64_t scale2 = pair(sl2, sl2);
-        bool exact = i == w.i0;
-        while (true) {
-          float v1[64];
-          tmem_ld32(tS, v1);
-          tmem_ld32(tS + 32, v1 + 32);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          ok = __all_sync(0xffffffffu, ok && wait_or_abort(&s_full[2 * t + half], n & 1, p.err, &abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tH = tS + half * 64;
+          float v[64];
+          tmem_ld32(tH, v);
+          tmem_ld32(tH + 32, v + 32);
           tmem_ld_wait();
           if (edge) {
+            const int c0 = k0 + half * 64, h = hi - c0, b = lo - c0, f = range.sinks - c0;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              if (!(j < h && (j >= b || j < f))) v1[j] = -INFINITY;
-              if (!(j + 64 < h && (j + 64 >= b || j + 64 < f))) v2[j] = -INFINITY;
-            }
+            for (int j = 0; j < 64; ++j)
+              if (!(j < h && (j >= b || j < f))) v[j] = -INFINITY;
           }
-          const float mx2 = max64(v2) * sl2;
-          if (exact) {
-            const float mx = max3(max64(v1) * sl2, mx2, mx2);
+          const float mx = max64(v) * sl2;
+          if (!__all_sync(0xffffffffu, !valid || mx <= m + kGrowthLog2)) {
             const bool grew = valid && !(mx <= m + 8.f);
             const float alpha = grew ? ex2(m - mx) : 1.f;
             if (grew) m = mx;
             l *= alpha;
-            if (i > w.i0) {
+            if (valid && !(mx < INFINITY)) l = NAN;      // an infinite or NaN score in the row
+            if (i > w.i0 || half > 0) {
+              // the P V of the half before, the last to add to O, must be done
+              wait_or_abort(&pv_done[t], half ^ 1, p.err, &abort_flag);
+              __syncwarp();
+              tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD; c += 16) {
                 float o[16];
@@ -439,58 +459,36 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
           }
           const float ref = m == -INFINITY ? 0.f : m;
-          const uint64_t ref2 = pair(-ref, -ref);
-          sum = pair(0.f, 0.f);
+          const uint64_t scale2 = pair(sl2, sl2), ref2 = pair(-ref, -ref);
+          uint64_t sum = pair(l, 0.f);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            float e0, e1;
-            unpair(fma2(pair(v1[2 * j], v1[2 * j + 1]), scale2, ref2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            sum = add2(sum, pair(e0, e1));
-            w1[j] = pack_bf16(e0, e1);
-          }
-          if (exact) break;
-          float s0, s1;
-          unpair(sum, s0, s1);
-          const bool fine = !valid || (m > -INFINITY && s0 + s1 <= kGrowth && mx2 <= m + kGrowthLog2);
-          if (__all_sync(0xffffffffu, fine)) break;
-          exact = true;
-        }
-        tmem_st16(tS, w1);
-        tmem_st16(tS + 16, w1 + 16);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_half[t]);          // half of the keys: P V may begin
-        const float ref = m == -INFINITY ? 0.f : m;
-        const uint64_t ref2 = pair(-ref, -ref);
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t e[16];
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          uint32_t e[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const uint64_t y = fma2(pair(v2[c + 2 * j], v2[c + 2 * j + 1]), scale2, ref2);
-            float e0, e1;
-            if ((j & 7) < kPolyPairs) {
-              unpair(exp2_pair(y), e0, e1);
-            } else {
-              unpair(y, e0, e1);
-              e0 = ex2(e0);
-              e1 = ex2(e1);
+            for (int j = 0; j < 16; ++j) {
+              const uint64_t y = fma2(pair(v[c + 2 * j], v[c + 2 * j + 1]), scale2, ref2);
+              float e0, e1;
+              if ((j & 7) < kPolyPairs) {
+                unpair(exp2_pair(y), e0, e1);
+              } else {
+                unpair(y, e0, e1);
+                e0 = ex2(e0);
+                e1 = ex2(e1);
+              }
+              sum = add2(sum, pair(e0, e1));
+              e[j] = pack_bf16(e0, e1);
             }
-            sum = add2(sum, pair(e0, e1));
-            e[j] = pack_bf16(e0, e1);
+            tmem_st16(tH + c / 2, e);
           }
-          tmem_st16(tS + 32 + c / 2, e);
+          float l_even, l_odd;
+          unpair(sum, l_even, l_odd);
+          l = l_even + l_odd;
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
         }
-        float s0, s1;
-        unpair(sum, s0, s1);
-        l += s0 + s1;
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (!ok) break;
       }
       ok = __all_sync(0xffffffffu, ok && wait_or_abort(&ml_free[t], (items & 1) ^ 1, p.err, &abort_flag));
       if (!ok) break;
