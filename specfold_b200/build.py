@@ -21,7 +21,7 @@ LIB = os.path.join(LIBDIR, "libspecfold_b200.so")
 SOURCES = ["gate.cu", "gemm.cu", "gemm_tc.cu", "attention.cu", "attention_tc.cu",
            "attention_rows_mma.cu", "attention_rows_tc.cu", "merge.cu", "tp.cu", "capi.cu", "ffn_static.cu", "sample.cu",
            "draft.cu", "paged_plan.cu", "paged_cache.cu", "paged_attention_simt.cu",
-           "paged_attention_tokens.cu", "paged_attention_chunk.cu"]
+           "paged_attention_tokens.cu", "paged_attention_chunk.cu", "paged_mass_tc.cu"]
 HEADERS = ["sf_common.cuh", "sf_kernels.cuh", "paged.cuh", "paged_tc.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -147,6 +147,7 @@ cudaError_t launch_paged_attention_tokens(const PagedAttnParams& p, int copies, 
 cudaError_t launch_paged_attention_chunk(const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st);
+cudaError_t launch_paged_mass_tc(const PagedMassParams& p, cudaStream_t st);
 
 // {sequence, position} of every new token
 struct PagedAppendParams {

@@ -27,24 +27,6 @@ constexpr int kChunkThreads = 512;
 // Of every 8 pairs of weights, this many take the polynomial instead of the special-function unit.
 constexpr int kPolyPairs = 1;
 
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ void unpair(uint64_t d, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // the larger of three, NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -87,14 +69,6 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   unpair(y, ya, yb);
   return pair(__int_as_float(__float_as_int(ya) + (__float_as_int(za) << 23)),
               __int_as_float(__float_as_int(yb) + (__float_as_int(zb) << 23)));
-}
-
-// shared-memory matrix descriptors of sf_common.cuh, in the two words an issue loop steps
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint64_t desc(uint32_t lo) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(kDescHi));
-  return d;
 }
 
 template <int HD>

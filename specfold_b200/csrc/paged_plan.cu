@@ -43,8 +43,8 @@ Tiling tiling(const sf_paged_plan& p) {
     t.per_tile[0] = t.tokens[0];
     t.per_tile[1] = 2 * t.tokens[1];
     t.workers[0] = t.workers[1] = p.sms;
-    t.mass_workers = 2 * p.sms;
-    t.mass_rows = 64;
+    t.mass_workers = p.sms;
+    t.mass_rows = 128;
     return t;
   }
   t.rows[0] = 16;
@@ -506,7 +506,9 @@ int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool
   p.sinks = plan->sinks;
   p.scale = scale;
   p.err = plan->err;
-  return status(launch_paged_mass_simt(plan->dtype, p, static_cast<cudaStream_t>(stream)), "paged_attention_mass");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return status(plan->dtype == SF_DTYPE_BF16 ? launch_paged_mass_tc(p, st) : launch_paged_mass_simt(plan->dtype, p, st),
+                "paged_attention_mass");
 }
 
 int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_table, int64_t dst_stride,
