@@ -368,7 +368,7 @@ typedef struct sf_paged_plan {
   int32_t tokens;                    /* offset of the {sequence, position} list */
   sf_paged_list attn[2], mass;       /* [0]: few query rows per kv head, [1]: many */
   int64_t words;                     /* words of the plan */
-  size_t ws_bytes;                   /* scratch of sf_paged_attention */
+  size_t ws_bytes;                   /* scratch of the calls below */
   /* set by the caller before the first use */
   const int32_t* dev;                /* the plan's words in device memory */
   void* ws;                          /* ws_bytes of device memory */

@@ -37,10 +37,17 @@ struct alignas(16) PagedMerge {
   int32_t kvh, tok0, ntok, slot0;
   int32_t n, q0, pad0, pad1;
 };
-// Key blocks [kb0, kb1) of one (sequence, kv head), for the weight accumulation
+// Weight accumulation: two key blocks of one (sequence, kv head) against tiles [i0, i1) of the
+// tokens from t0 on (t0: the first that sees either block, t1: behind the last)
+constexpr int kMassBlocks = 2;
 struct alignas(16) PagedMassItem {
-  int32_t seq, kvh, kb0, kb1;
+  int32_t seq, kvh, kb0, t0;
+  int32_t t1, i0, i1, slot;           // slot < 0: adds to the weights itself
   int32_t q0, q_len, kv_len, pad;
+};
+struct alignas(16) PagedMassMerge {
+  int32_t seq, kvh, kb0, slot0;
+  int32_t n, q_len, kv_len, pad;
 };
 
 // The keys that some token of a range sees: [lo, hi) and [0, sinks)
@@ -65,6 +72,24 @@ struct PagedMask {
     if (window == 0) return 0;
     const int l = pos(i) - window + 1;
     return l > 0 ? l : 0;
+  }
+  // keys that some token sees in block kb
+  __host__ __device__ PagedRange block_range(int kb) const {
+    int f, l;
+    tokens(kb, &f, &l);
+    return f < l ? range(f, l) : PagedRange{0, 0, 0};
+  }
+  // the tokens that see a key of any block of a pair
+  __host__ __device__ void pair_tokens(int kb0, int* first, int* last) const {
+    *first = q_len;
+    *last = 0;
+    for (int kb = kb0; kb < kb0 + kMassBlocks && kb * kPagedKB < kv_len; ++kb) {
+      int f, l;
+      tokens(kb, &f, &l);
+      if (f >= l) continue;
+      if (f < *first) *first = f;
+      if (l > *last) *last = l;
+    }
   }
   __host__ __device__ PagedRange range(int t0, int t1) const { return {lo(t0), hi(t1 - 1), window > 0 ? sinks : 0}; }
   // the tokens of the chunk that see any key of block kb: [first, last)
@@ -126,6 +151,9 @@ struct PagedMassParams {
   const PagedMassItem* items;
   const int32_t* first;
   int workers;
+  const PagedMassMerge* merges;
+  int n_merges;
+  float* part;                      // [slots][2 * 128] sums of the pieces
   int H, Hkv, G, hd, T;
   int block, window, sinks;
   float scale;
@@ -148,6 +176,7 @@ cudaError_t launch_paged_attention_chunk(const PagedAttnParams& p, cudaStream_t 
 cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st);
 cudaError_t launch_paged_mass_tc(const PagedMassParams& p, cudaStream_t st);
+cudaError_t launch_paged_mass_merge(const PagedMassParams& p, cudaStream_t st);
 
 // {sequence, position} of every new token
 struct PagedAppendParams {

@@ -303,6 +303,12 @@ cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cud
 }
 
 // ------------------------------------------------------------------ weight accumulation
+__device__ __forceinline__ float* mass_slot(const PagedMassParams& p, int seq, int kvh, int key) {
+  const int page = paged_page(p.pool, seq, key >> p.pool.page_shift, p.err);
+  return p.pool.mass + ((static_cast<int64_t>(page) * p.Hkv + kvh) << p.pool.page_shift) +
+         (key & ((1 << p.pool.page_shift) - 1));
+}
+
 // A key's weight over all rows that see it: sum of exp(s - lse).  A CTA owns a key block and
 // walks the query rows, so each weight is summed in one place, in one order, without atomics.
 template <typename T, int HD, int RM>
@@ -319,19 +325,17 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedM
   for (int it = p.first[blockIdx.x]; it < last; ++it) {
     const PagedMassItem w = p.items[it];
     const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
-    for (int kb = w.kb0; kb < w.kb1; ++kb) {
-      int t0, t1;
-      mask.tokens(kb, &t0, &t1);
-      if (t0 >= t1) continue;
-      const PagedRange range = mask.range(t0, t1);
+    for (int kb = w.kb0; kb < w.kb0 + kMassBlocks && kb * kPagedKB < w.kv_len; ++kb) {
+      const PagedRange range = mask.block_range(kb);
       for (int sub = 0; sub < kPagedKB / kSimtKeys; ++sub) {
         const int k0 = kb * kPagedKB + sub * kSimtKeys;
         if (k0 >= range.hi) break;
         __syncthreads();
         simt_load_keys<T, HD>(sK, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int t = t0; t < t1; t += tile) {
-          const int rows = min(tile, t1 - t) * p.G;
+        for (int x = w.i0; x < w.i1; ++x) {
+          const int t = w.t0 + x * tile;
+          const int rows = min(tile, w.t1 - t) * p.G;
           __syncthreads();
           simt_load_q<T, HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + t, w.kvh, p.G, rows);
           __syncthreads();
@@ -359,13 +363,31 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedM
           float sum = 0.f;
           for (int y = 0; y < 16; ++y) sum += sR[y * kSimtKeys + threadIdx.x];
           const int j = k0 + threadIdx.x;
-          const int page = paged_page(p.pool, w.seq, j >> p.pool.page_shift, p.err);
-          p.pool.mass[((static_cast<int64_t>(page) * p.Hkv + w.kvh) << p.pool.page_shift) +
-                      (j & ((1 << p.pool.page_shift) - 1))] += sum;
+          if (w.slot >= 0)
+            p.part[static_cast<int64_t>(w.slot) * kMassBlocks * kPagedKB + j - w.kb0 * kPagedKB] = sum;
+          else
+            *mass_slot(p, w.seq, w.kvh, j) += sum;
         }
       }
     }
   }
+}
+
+// Adds the pieces of the pairs of key blocks that were cut, in order.
+__global__ void __launch_bounds__(kMassBlocks * kPagedKB) paged_mass_merge_kernel(PagedMassParams p) {
+  const PagedMassMerge w = p.merges[blockIdx.x];
+  const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
+  const int key = w.kb0 * kPagedKB + threadIdx.x;
+  if (key >= w.kv_len || !mask.block_range(key / kPagedKB).has(key)) return;
+  float sum = 0.f;
+  for (int i = 0; i < w.n; ++i) sum += p.part[static_cast<int64_t>(w.slot0 + i) * kMassBlocks * kPagedKB + threadIdx.x];
+  *mass_slot(p, w.seq, w.kvh, key) += sum;
+}
+
+cudaError_t launch_paged_mass_merge(const PagedMassParams& p, cudaStream_t st) {
+  if (p.n_merges == 0) return cudaSuccess;
+  paged_mass_merge_kernel<<<p.n_merges, kMassBlocks * kPagedKB, 0, st>>>(p);
+  return launched();
 }
 
 template <typename T, int HD, int RM>

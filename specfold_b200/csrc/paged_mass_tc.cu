@@ -5,10 +5,12 @@
 // MMA, so that a key is a TMEM lane: a thread adds up its own key's weights over the columns (the
 // query rows), tile after tile, in registers.  A weight is therefore summed in one place, in one
 // order, and written once; no atomics.  lse is a per-column constant: the exponent is one fma.
-//   warps 4-7, 8-11   exponentials and sums of columns 0-63 and 64-127 of every tile
+// A CTA works on two key blocks at a time, so that a query tile, which streams from L2, feeds two
+// products.  A pair whose tiles were cut between CTAs leaves its sums for the merge.
+//   warps 4-7, 8-11   exponentials and sums of the first and of the second block
 //   warp 0            TMA: key blocks and query tiles, through rings of their own
-//   warp 1            tcgen05.mma into four S^T buffers of 128 columns (all of TMEM)
-//   warp 2            lse and the mask's bounds of the query tile's rows into shared memory
+//   warp 1            tcgen05.mma, two S^T buffers of 128 columns for each block (all of TMEM)
+//   warp 2            lse and the mask's bounds of the tile's rows into shared memory
 // Bound: for chunks by the special-function unit, one exponential per (row, key): 1024 cycles for
 // a 128 x 128 tile against 512 of products; for single tokens by the bytes of the keys.
 #include "paged_tc.cuh"
@@ -21,14 +23,24 @@ template <int HD>
 struct MassSmem {
   static constexpr int kTile = HD / 64 * kPagedBox;      // 128 rows
   static constexpr int kStages = 3;                      // of keys, of queries
+  static constexpr int kRows = 4;                        // stages of lse and bounds
   static constexpr int k = 0;                            // [kStages][kTile]
   static constexpr int q = k + kStages * kTile;          // [kStages][kTile]
-  static constexpr int lse = q + kStages * kTile;        // [kStages][128] floats
-  static constexpr int hi = lse + kStages * 512;         // [kStages][128] ints
-  static constexpr int lo = hi + kStages * 512;
-  static constexpr int part = lo + kStages * 512;        // [2][128] floats
-  static constexpr int bars = part + 2 * 512;
+  static constexpr int lse = q + kStages * kTile;        // [kRows][128] floats
+  static constexpr int hi = lse + kRows * 512;           // [kRows][128] ints
+  static constexpr int lo = hi + kRows * 512;
+  static constexpr int bars = lo + kRows * 512;
   static constexpr int bytes = bars + 256 + 1024;        // + alignment of the base
+};
+
+// The tiles of an item that meet block kb (0 or 1 of the pair): those with tokens [f, l) that see
+// a key of it.
+struct MassBlock {
+  int kb, f, l;
+  __device__ __forceinline__ MassBlock(const PagedMask& mask, int kb_, int kv_len) : kb(kb_), f(0), l(0) {
+    if (kb * kPagedKB < kv_len) mask.tokens(kb, &f, &l);
+  }
+  __device__ __forceinline__ bool meets(int t, int t_end) const { return t < l && t_end > f; }
 };
 
 template <int HD>
@@ -36,7 +48,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     paged_mass_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       PagedMassParams p) {
   typedef MassSmem<HD> L;
-  constexpr int KCH = HD / 64, NS = L::kStages;
+  constexpr int KCH = HD / 64, NS = L::kStages, NR = L::kRows;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                        ~static_cast<uintptr_t>(1023));
@@ -45,9 +57,11 @@ __global__ void __launch_bounds__(kMassThreads, 1)
   uint64_t* k_empty = bars + NS;                         // [NS]
   uint64_t* q_full = bars + 2 * NS;                      // [NS]
   uint64_t* q_empty = bars + 3 * NS;                     // [NS]
-  uint64_t* s_full = bars + 4 * NS;                      // [4]
-  uint64_t* s_empty = s_full + 4;                        // [4]
-  uint64_t* drain = s_full + 8;
+  uint64_t* r_full = bars + 4 * NS;                      // [NR]
+  uint64_t* r_empty = r_full + NR;                       // [NR]
+  uint64_t* s_full = r_empty + NR;                       // [2 blocks][2 buffers]
+  uint64_t* s_empty = s_full + 4;
+  uint64_t* drain = s_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -58,12 +72,16 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
-      mbar_init(&q_full[s], 2);                          // the tile, the rows' bounds
-      mbar_init(&q_empty[s], 9);                         // the products, the sums' warps
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+    }
+    for (int s = 0; s < NR; ++s) {
+      mbar_init(&r_full[s], 1);
+      mbar_init(&r_empty[s], 8);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_empty[s], 8);
+      mbar_init(&s_empty[s], 4);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -94,25 +112,25 @@ __global__ void __launch_bounds__(kMassThreads, 1)
       PagedItem w{};
       w.seq = m.seq;
       w.kvh = m.kvh;
-      for (int kb = m.kb0; ok && kb < m.kb1; ++kb) {
-        int t0, t1;
-        mask.tokens(kb, &t0, &t1);
-        if (t0 >= t1) continue;
-        const uint32_t s = kn % NS;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[s], ((kn / NS) & 1) ^ 1, p.err, abort_flag));
+      for (int x = m.i0; ok && x < m.i1; ++x, ++qn) {
+        if (x == m.i0)
+          for (int kb = m.kb0; ok && kb < m.kb0 + kMassBlocks; ++kb) {
+            const PagedRange range = mask.block_range(kb);
+            if (kb * kPagedKB >= m.kv_len || range.hi == 0) continue;
+            const uint32_t s = kn % NS;
+            ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[s], ((kn / NS) & 1) ^ 1, p.err, abort_flag));
+            if (!ok) break;
+            load_key_block<HD>(sm + L::k + s * L::kTile, &tmK, &k_full[s], p.pool, w, range, kb, lane, p.err);
+            ++kn;
+          }
+        const uint32_t s = qn % NS;
+        ok = ok && __all_sync(0xffffffffu, wait_or_abort(&q_empty[s], ((qn / NS) & 1) ^ 1, p.err, abort_flag));
         if (!ok) break;
-        load_key_block<HD>(sm + L::k + s * L::kTile, &tmK, &k_full[s], p.pool, w, mask.range(t0, t1), kb, lane, p.err);
-        ++kn;
-        for (int t = t0; t < t1; t += tq) {
-          const uint32_t x = qn % NS;
-          ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[x], ((qn / NS) & 1) ^ 1, p.err, abort_flag));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&q_full[x], KCH * tq * p.G * 128);
-          __syncwarp();
-          if (lane < KCH)
-            tma_load_3d(sm + L::q + x * L::kTile + lane * kPagedBox, &tmQ, &q_full[x], lane * 64, m.kvh * p.G, m.q0 + t);
-          ++qn;
-        }
+        if (lane == 0) mbar_arrive_expect_tx(&q_full[s], KCH * tq * p.G * 128);
+        __syncwarp();
+        if (lane < KCH)
+          tma_load_3d(sm + L::q + s * L::kTile + lane * kPagedBox, &tmQ, &q_full[s], lane * 64, m.kvh * p.G,
+                      m.q0 + m.t0 + x * tq);
       }
     }
     if (!ok && lane == 0) {                              // no load may be in flight at exit
@@ -123,36 +141,49 @@ __global__ void __launch_bounds__(kMassThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
     if (elect_one()) {
+      uint32_t bn[2] = {0, 0};                           // scores of each block so far
       for (int it = first; ok && it < last; ++it) {
         const PagedMassItem m = p.items[it];
         const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
-        for (int kb = m.kb0; ok && kb < m.kb1; ++kb) {
-          int t0, t1;
-          mask.tokens(kb, &t0, &t1);
-          if (t0 >= t1) continue;
-          const uint32_t s = kn % NS;
-          ok = wait_or_abort(&k_full[s], (kn / NS) & 1, p.err, abort_flag);
-          const uint32_t k_lo = ((smem_u32(sm + L::k) + s * L::kTile) >> 4) | (1u << 16);
-          for (int t = t0; ok && t < t1; t += tq) {
-            const uint32_t x = qn % NS, b = qn & 3;
-            ok = wait_or_abort(&q_full[x], (qn / NS) & 1, p.err, abort_flag) &&
-                 wait_or_abort(&s_empty[b], ((qn >> 2) & 1) ^ 1, p.err, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            const int cols = (min(tq, t1 - t) * p.G + 15) / 16 * 16;
-            const uint32_t id = idesc_bf16(128, 16) + (static_cast<uint32_t>(cols / 8 - 2) << 17);
-            const uint32_t q_lo = ((smem_u32(sm + L::q) + x * L::kTile) >> 4) | (1u << 16);
+        const MassBlock blk[2] = {MassBlock(mask, m.kb0, m.kv_len), MassBlock(mask, m.kb0 + 1, m.kv_len)};
+        uint32_t k_lo[2];
+        uint32_t ks[2];
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              umma_f16(tmem + b * 128, desc(k_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
-                       desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id, kk > 0 ? 1u : 0u);
-            umma_commit(&s_full[b]);
-            umma_commit(&q_empty[x]);
-            if (t + tq >= t1) umma_commit(&k_empty[s]);
-            ++qn;
-          }
+        for (int y = 0; ok && y < 2; ++y) {
+          if (blk[y].f >= blk[y].l) continue;
+          ks[y] = kn % NS;
+          ok = wait_or_abort(&k_full[ks[y]], (kn / NS) & 1, p.err, abort_flag);
+          k_lo[y] = ((smem_u32(sm + L::k) + ks[y] * L::kTile) >> 4) | (1u << 16);
           ++kn;
         }
+        for (int x = m.i0; ok && x < m.i1; ++x, ++qn) {
+          const uint32_t s = qn % NS;
+          const int t = m.t0 + x * tq, t_end = min(t + tq, m.t1);
+          const int cols = ((t_end - t) * p.G + 15) / 16 * 16;
+          const uint32_t id = idesc_bf16(128, 16) + (static_cast<uint32_t>(cols / 8 - 2) << 17);
+          const uint32_t q_lo = ((smem_u32(sm + L::q) + s * L::kTile) >> 4) | (1u << 16);
+          ok = wait_or_abort(&q_full[s], (qn / NS) & 1, p.err, abort_flag);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            if (!ok || !blk[y].meets(t, t_end)) continue;
+            const uint32_t b = 2 * y + (bn[y] & 1);
+            ok = wait_or_abort(&s_empty[b], ((bn[y] >> 1) & 1) ^ 1, p.err, abort_flag);
+            if (!ok) continue;
+            ++bn[y];
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              umma_f16(tmem + b * 128, desc(k_lo[y] + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
+                       desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id, kk > 0 ? 1u : 0u);
+            umma_commit(&s_full[b]);
+          }
+          if (!ok) break;
+          umma_commit(&q_empty[s]);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          if (blk[y].f < blk[y].l) umma_commit(&k_empty[ks[y]]);
       }
       if (!ok) *abort_flag = 1;
       umma_commit(drain);
@@ -163,123 +194,120 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     float* s_lse = reinterpret_cast<float*>(sm + L::lse);
     int* s_hi = reinterpret_cast<int*>(sm + L::hi);
     int* s_lo = reinterpret_cast<int*>(sm + L::lo);
+    int tok[4], head[4];                                 // of this lane's four rows
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      tok[j] = (lane + 32 * j) / p.G;
+      head[j] = (lane + 32 * j) % p.G;
+    }
     for (int it = first; ok && it < last; ++it) {
       const PagedMassItem m = p.items[it];
       const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
-      for (int kb = m.kb0; ok && kb < m.kb1; ++kb) {
-        int t0, t1;
-        mask.tokens(kb, &t0, &t1);
-        for (int t = t0; ok && t < t1; t += tq, ++qn) {
-          const uint32_t x = qn % NS;
-          const int rows = min(tq, t1 - t) * p.G;
-          float v[4];
+      for (int x = m.i0; x < m.i1; ++x, ++qn) {
+        const uint32_t s = qn % NR;
+        const int t = m.t0 + x * tq, n = min(tq, m.t1 - t);
+        float v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {                  // ahead of the wait: the loads take their time
-            const int c = lane + 32 * j;
-            v[j] = INFINITY;                             // a column that is no row: weight 0
-            if (c < rows)
-              v[j] = p.lse[static_cast<int64_t>(m.q0 + t + c / p.G) * p.H + m.kvh * p.G + c % p.G] * 1.4426950408889634f;
-          }
-          ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[x], ((qn / NS) & 1) ^ 1, p.err, abort_flag));
-          if (!ok) break;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = lane + 32 * j, i = t + min(c, rows - 1) / p.G;
-            s_lse[x * 128 + c] = -v[j];
-            s_hi[x * 128 + c] = mask.hi(i);
-            s_lo[x * 128 + c] = mask.lo(i);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[x]);
+        for (int j = 0; j < 4; ++j) {                    // ahead of the wait: the loads take their time
+          v[j] = INFINITY;                               // a column that is no row: weight 0
+          if (tok[j] < n)
+            v[j] = p.lse[static_cast<int64_t>(m.q0 + t + tok[j]) * p.H + m.kvh * p.G + head[j]] * 1.4426950408889634f;
         }
+        ok = __all_sync(0xffffffffu, wait_or_abort(&r_empty[s], ((qn / NR) & 1) ^ 1, p.err, abort_flag));
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = s * 128 + lane + 32 * j, i = t + min(tok[j], n - 1);
+          s_lse[c] = -v[j];
+          s_hi[c] = mask.hi(i);
+          s_lo[c] = mask.lo(i);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&r_full[s]);
       }
     }
     if (!ok) *abort_flag = 1;
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- exponentials and sums
-    const int half = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
-    const uint32_t tS = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
+    const int y = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t tS = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + y * 256;
     const float* s_lse = reinterpret_cast<const float*>(sm + L::lse);
     const int* s_hi = reinterpret_cast<const int*>(sm + L::hi);
     const int* s_lo = reinterpret_cast<const int*>(sm + L::lo);
-    float* part = reinterpret_cast<float*>(sm + L::part);
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint64_t scale2 = pair(sl2, sl2);
-    for (int it = first; it < last; ++it) {
+    uint32_t bn = 0;                                     // this block's scores so far
+    for (int it = first; ok && it < last; ++it) {
       const PagedMassItem m = p.items[it];
       const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
-      for (int kb = m.kb0; kb < m.kb1; ++kb) {
-        int t0, t1;
-        mask.tokens(kb, &t0, &t1);
-        if (t0 >= t1) continue;
-        const PagedRange range = mask.range(t0, t1);
-        const int k0 = kb * kPagedKB, key = k0 + r;
-        float* dst = nullptr;                            // this key's weight, read while the tiles run
-        float old = 0.f;
-        if (half == 0 && range.has(key)) {
+      const MassBlock blk(mask, m.kb0 + y, m.kv_len);
+      const PagedRange range = mask.block_range(blk.f < blk.l ? m.kb0 + y : 0);
+      const int k0 = (m.kb0 + y) * kPagedKB, key = k0 + r;
+      const bool seen = blk.f < blk.l && range.has(key);
+      float* dst = nullptr;                              // this key's weight, read while the tiles run
+      float old = 0.f;
+      if (seen) {
+        if (m.slot >= 0) {
+          dst = p.part + static_cast<int64_t>(m.slot) * kMassBlocks * kPagedKB + y * kPagedKB + r;
+        } else {
           const int page = paged_page(p.pool, m.seq, key >> p.pool.page_shift, p.err);
           dst = p.pool.mass + ((static_cast<int64_t>(page) * p.Hkv + m.kvh) << p.pool.page_shift) +
                 (key & ((1 << p.pool.page_shift) - 1));
           old = *dst;
         }
-        uint64_t sum = pair(0.f, 0.f);
-        for (int t = t0; t < t1; t += tq, ++qn) {
-          const uint32_t x = qn % NS, b = qn & 3;
-          const int rows = min(tq, t1 - t) * p.G;
-          // (a warp whose wait failed goes on: the halves meet at the block's end)
-          ok = __all_sync(0xffffffffu, ok && wait_or_abort(&s_full[b], (qn >> 2) & 1, p.err, abort_flag) &&
-                                           wait_or_abort(&q_full[x], (qn / NS) & 1, p.err, abort_flag));
-          if (ok && half * 64 < rows) {
-            tc_fence_after();
-            const int tl = min(t + tq, t1) - 1;
-            const bool edge = k0 + kPagedKB > mask.hi(t) || (k0 < mask.lo(tl) && k0 + kPagedKB > range.sinks);
+      }
+      uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
+      for (int x = m.i0; x < m.i1; ++x, ++qn) {
+        const uint32_t s = qn % NR, b = bn & 1;
+        const int t = m.t0 + x * tq, t_end = min(t + tq, m.t1);
+        const int rows = (t_end - t) * p.G;
+        const bool mine = blk.meets(t, t_end);
+        ok = __all_sync(0xffffffffu, (!mine || wait_or_abort(&s_full[2 * y + b], (bn >> 1) & 1, p.err, abort_flag)) &&
+                                         wait_or_abort(&r_full[s], (qn / NR) & 1, p.err, abort_flag));
+        if (!ok) break;
+        if (mine) {
+          tc_fence_after();
+          const bool edge = k0 + kPagedKB > mask.hi(t) || (k0 < mask.lo(t_end - 1) && k0 + kPagedKB > range.sinks);
 #pragma unroll 1
-            for (int c = half * 64; c < min(rows, half * 64 + 64); c += 32) {
-              float v[32];
-              tmem_ld32(tS + b * 128 + (c & 32), v);
-              tmem_ld_wait();
-              const float4* lse4 = reinterpret_cast<const float4*>(s_lse + x * 128 + c);
-              if (c + 32 > rows) {                       // columns that are no rows may hold anything
+          for (int c = 0; c < rows; c += 32) {
+            float v[32];
+            tmem_ld32(tS + b * 128 + c, v);
+            const float4* lse4 = reinterpret_cast<const float4*>(s_lse + s * 128 + c);
+            tmem_ld_wait();
+            if (c + 32 > rows) {                         // columns that are no rows may hold anything
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (c + j >= rows) v[j] = 0.f;         // (their -lse is -inf)
-              }
-              if (edge) {
+              for (int j = 0; j < 32; ++j)
+                if (c + j >= rows) v[j] = 0.f;           // (their -lse is -inf)
+            }
+            if (edge) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  const int h = s_hi[x * 128 + c + j], l = s_lo[x * 128 + c + j];
-                  if (!(key < h && (key >= l || key < range.sinks))) v[j] = -INFINITY;
-                }
+              for (int j = 0; j < 32; ++j) {
+                const int h = s_hi[s * 128 + c + j], l = s_lo[s * 128 + c + j];
+                if (!(key < h && (key >= l || key < range.sinks))) v[j] = -INFINITY;
               }
+            }
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 e = lse4[j / 4];
-                float a0, a1, a2, a3;
-                unpair(fma2(pair(v[j], v[j + 1]), scale2, pair(e.x, e.y)), a0, a1);
-                unpair(fma2(pair(v[j + 2], v[j + 3]), scale2, pair(e.z, e.w)), a2, a3);
-                a0 = ex2(a0);
-                a1 = ex2(a1);
-                a2 = ex2(a2);
-                a3 = ex2(a3);
-                sum = add2(sum, add2(pair(a0, a1), pair(a2, a3)));
-              }
+            for (int j = 0; j < 32; j += 4) {
+              const float4 e = lse4[j / 4];
+              float a0, a1, a2, a3;
+              unpair(fma2(pair(v[j], v[j + 1]), scale2, pair(e.x, e.y)), a0, a1);
+              unpair(fma2(pair(v[j + 2], v[j + 3]), scale2, pair(e.z, e.w)), a2, a3);
+              sum0 = add2(sum0, pair(ex2(a0), ex2(a1)));
+              sum1 = add2(sum1, pair(ex2(a2), ex2(a3)));
             }
           }
           tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&s_empty[b]);
-            mbar_arrive(&q_empty[x]);
-          }
+          ++bn;
         }
-        float even, odd;
-        unpair(sum, even, odd);
-        // the halves' sums (two buffers: the next block's may come while this one is read)
-        if (half == 1) part[(kn & 1) * 128 + r] = even + odd;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (dst != nullptr && ok) *dst = old + (even + odd + part[(kn & 1) * 128 + r]);
-        ++kn;
+        __syncwarp();
+        if (lane == 0) {
+          if (mine) mbar_arrive(&s_empty[2 * y + b]);
+          mbar_arrive(&r_empty[s]);
+        }
       }
+      float a0, a1;
+      unpair(add2(sum0, sum1), a0, a1);
+      if (dst != nullptr && ok) *dst = old + (a0 + a1);
     }
     if (!ok) *abort_flag = 1;
   }

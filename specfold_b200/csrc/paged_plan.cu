@@ -3,7 +3,6 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
-#include <queue>
 #include <vector>
 
 #include "paged.cuh"
@@ -24,6 +23,7 @@ int bad(const char* fmt, ...) {
 constexpr int kItemWords = sizeof(PagedItem) / 4;
 constexpr int kMergeWords = sizeof(PagedMerge) / 4;
 constexpr int kMassWords = sizeof(PagedMassItem) / 4;
+constexpr int kMassMergeWords = sizeof(PagedMassMerge) / 4;
 constexpr int64_t kMaxWords = int64_t{1} << 30;
 
 int64_t up4(int64_t x) { return (x + 3) & ~int64_t{3}; }
@@ -91,62 +91,58 @@ int device_sms(int asked) {
 
 int which(const Tiling& t, int q_len, int G) { return static_cast<int64_t>(q_len) * G <= t.rows[0] ? 0 : 1; }
 
-struct Tile {
-  PagedItem item;   // i0 = 0, i1 = its key blocks
+// A share of something that is cut into units [0, units): the piece [i0, i1), and where its
+// partial result goes (-1: it is whole)
+struct Piece {
+  int what, i0, i1, slot;
+};
+struct Cut {
+  int what, slot0, n;
 };
 
-// Deals the tiles out in order: each worker takes its share of (key blocks + 1 per tile), and a
-// tile that does not fit goes on with the next one.
-void deal(const std::vector<PagedItem>& tiles, int workers, std::vector<PagedItem>* items,
-          std::vector<int32_t>* first, std::vector<PagedMerge>* merges, int* slots) {
+// Deals things out in order: each worker takes its share of their units (and `extra` per thing),
+// and what does not fit goes on with the next one.
+void deal(const std::vector<int>& units, int extra, int workers, std::vector<Piece>* pieces,
+          std::vector<int32_t>* first, std::vector<Cut>* cuts, int* slots) {
   int64_t total = 0;
-  for (const PagedItem& t : tiles) total += t.i1 + 1;
+  for (int u : units) total += u + extra;
   const int64_t w = std::max<int64_t>(1, std::min<int64_t>(workers, total));
   first->push_back(0);
   *slots = 0;
-  int64_t done = 0, worker = 0;   // cost dealt out; end of this worker's share: (worker+1)*total/w
-  for (const PagedItem& t : tiles) {
-    int at = 0, pieces = 0;
-    const size_t from = items->size();
+  int64_t done = 0, worker = 0;   // dealt out; this worker's share ends at (worker + 1) * total / w
+  for (size_t x = 0; x < units.size(); ++x) {
+    int at = 0, n = 0;
+    const size_t from = pieces->size();
     do {
-      // what is left of this worker's share; a full one, or one too small to be worth a piece,
-      // ends here
+      // what is left of this worker's share; one too small to be worth a piece ends here
       int64_t room = (worker + 1) * total / w - done;
-      while (room <= 1 && worker + 1 < w) {
-        first->push_back(static_cast<int32_t>(items->size()));
+      while (room <= extra && worker + 1 < w) {
+        first->push_back(static_cast<int32_t>(pieces->size()));
         ++worker;
         room = (worker + 1) * total / w - done;
       }
-      const int need = t.i1 - at;
+      const int need = units[x] - at;
       int take = need;
-      if (worker + 1 < w && need + 1 > room) take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(need, room - 1)));
-      PagedItem it = t;
-      it.i0 = at;
-      it.i1 = at + take;
-      items->push_back(it);
+      if (worker + 1 < w && need + extra > room)
+        take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(need, room - extra)));
+      pieces->push_back({static_cast<int>(x), at, at + take, -1});
       at += take;
-      done += take + (pieces == 0 ? 1 : 0);
-      ++pieces;
-    } while (at < t.i1);
-    if (pieces > 1) {
-      PagedMerge m{};
-      m.kvh = t.kvh;
-      m.tok0 = t.tok0;
-      m.ntok = t.ntok;
-      m.slot0 = *slots;
-      m.n = pieces;
-      m.q0 = t.q0;
-      merges->push_back(m);
-      for (size_t i = from; i < items->size(); ++i) (*items)[i].slot = (*slots)++;
+      done += take + (n == 0 ? extra : 0);
+      ++n;
+    } while (at < units[x]);
+    if (n > 1) {
+      cuts->push_back({static_cast<int>(x), *slots, n});
+      for (size_t i = from; i < pieces->size(); ++i) (*pieces)[i].slot = (*slots)++;
     }
   }
-  while (static_cast<int64_t>(first->size()) <= w) first->push_back(static_cast<int32_t>(items->size()));
-  first->back() = static_cast<int32_t>(items->size());
+  while (static_cast<int64_t>(first->size()) <= w) first->push_back(static_cast<int32_t>(pieces->size()));
+  first->back() = static_cast<int32_t>(pieces->size());
 }
 
 size_t list_ws(const sf_paged_list& l, int hd) {
   return (static_cast<size_t>(l.slots) * l.rows * (hd + 2) * 4 + 255) / 256 * 256;
 }
+size_t mass_ws(const sf_paged_list& l) { return static_cast<size_t>(l.slots) * kMassBlocks * kPagedKB * 4; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -219,12 +215,13 @@ int64_t sf_paged_plan_words(const sf_paged_plan* plan, const int32_t* q_lens, co
   for (int b = 0; b < p.B; ++b) {
     const int k = which(t, q_lens[b], p.H / p.Hkv);
     items += static_cast<int64_t>((q_lens[b] + t.per_tile[k] - 1) / t.per_tile[k]) * p.Hkv;
-    if (q_lens[b] > 0) mass += static_cast<int64_t>((kv_lens[b] + kPagedKB - 1) / kPagedKB) * p.Hkv;
+    if (q_lens[b] > 0) mass += static_cast<int64_t>(kv_lens[b] / (kMassBlocks * kPagedKB) + 1) * p.Hkv;
     tokens += q_lens[b];
   }
   const int64_t w = t.workers[0] + t.workers[1];
-  const int64_t words = (items + w) * kItemWords + w * kMergeWords + 2 * (w + 16) + mass * kMassWords +
-                        (t.mass_workers + p.B * static_cast<int64_t>(p.Hkv)) * kMassWords + t.mass_workers + 16 + 2 * tokens + 64;
+  const int64_t m = t.mass_workers;
+  const int64_t words = (items + w) * kItemWords + w * kMergeWords + 2 * (w + 16) + (mass + m) * kMassWords +
+                        m * kMassMergeWords + m + 16 + 2 * tokens + 64;
   if (words > kMaxWords) {
     bad("paged plan: the step is too large");
     return 0;
@@ -261,8 +258,10 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
     at = up4(at);
     p.ws_bytes = 0;
     for (int k = 0; k < 2; ++k) {
-      std::vector<PagedItem> tiles, items;
-      std::vector<PagedMerge> merges;
+      std::vector<PagedItem> tiles;
+      std::vector<int> units;
+      std::vector<Piece> pieces;
+      std::vector<Cut> cuts;
       std::vector<int32_t> first;
       int q0 = 0;
       for (int b = 0; b < p.B; q0 += q_lens[b], ++b) {
@@ -285,6 +284,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
             it.q_len = q_lens[b];
             it.kv_len = kv_lens[b];
             tiles.push_back(it);
+            units.push_back(it.i1);
           }
       }
       sf_paged_list& l = p.attn[k];
@@ -294,102 +294,91 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       for (const PagedItem& it : tiles) l.max_rows = std::max(l.max_rows, it.ntok * G);
       if (!tiles.empty()) {
         int slots = 0;
-        deal(tiles, t.workers[k], &items, &first, &merges, &slots);
+        deal(units, 1, t.workers[k], &pieces, &first, &cuts, &slots);
         l.slots = slots;
-        l.n_items = static_cast<int32_t>(items.size());
+        l.n_items = static_cast<int32_t>(pieces.size());
         l.workers = static_cast<int32_t>(first.size()) - 1;
-        l.n_merges = static_cast<int32_t>(merges.size());
+        l.n_merges = static_cast<int32_t>(cuts.size());
       }
       l.items = static_cast<int32_t>(at);
-      memcpy(words + at, items.data(), items.size() * sizeof(PagedItem));
-      at += static_cast<int64_t>(items.size()) * kItemWords;
+      for (const Piece& x : pieces) {
+        PagedItem it = tiles[x.what];
+        it.i0 = x.i0;
+        it.i1 = x.i1;
+        it.slot = x.slot;
+        memcpy(words + at, &it, sizeof(it));
+        at += kItemWords;
+      }
       l.merges = static_cast<int32_t>(at);
-      memcpy(words + at, merges.data(), merges.size() * sizeof(PagedMerge));
-      at += static_cast<int64_t>(merges.size()) * kMergeWords;
+      for (const Cut& c : cuts) {
+        const PagedItem& it = tiles[c.what];
+        const PagedMerge m{it.kvh, it.tok0, it.ntok, c.slot0, c.n, it.q0, 0, 0};
+        memcpy(words + at, &m, sizeof(m));
+        at += kMergeWords;
+      }
       l.first = static_cast<int32_t>(at);
       memcpy(words + at, first.data(), first.size() * 4);
       at = up4(at + static_cast<int64_t>(first.size()));
       p.ws_bytes += list_ws(l, p.hd);
     }
-    // weight accumulation: runs of key blocks of equal cost (query tiles + 1 per block)
+    // weight accumulation: pairs of key blocks, their unit a tile of tokens
     {
-      std::vector<PagedMassItem> items;
+      std::vector<PagedMassItem> pairs;
+      std::vector<int> units;
+      std::vector<Piece> pieces;
+      std::vector<Cut> cuts;
       std::vector<int32_t> first;
       const int tile = std::max(1, t.mass_rows / G);
-      struct Unit {
-        int64_t cost;
-        PagedMassItem item;
-      };
-      std::vector<Unit> units;
-      int64_t total = 0, top = 0;
       int q0 = 0;
       for (int b = 0; b < p.B; q0 += q_lens[b], ++b) {
         if (q_lens[b] == 0) continue;
         const PagedMask mask{p.block, p.window, p.sinks, q_lens[b], kv_lens[b]};
-        const int nb = (kv_lens[b] + kPagedKB - 1) / kPagedKB;
         for (int h = 0; h < p.Hkv; ++h)
-          for (int kb = 0; kb < nb; ++kb) {
-            int f, e;
-            mask.tokens(kb, &f, &e);
-            if (f >= e) continue;
-            Unit u{(e - f + tile - 1) / tile + 1, {b, h, kb, kb + 1, q0, q_lens[b], kv_lens[b], 0}};
-            total += u.cost;
-            top = std::max(top, u.cost);
-            units.push_back(u);
+          for (int kb = 0; kb * kPagedKB < kv_lens[b]; kb += kMassBlocks) {
+            PagedMassItem it{};
+            mask.pair_tokens(kb, &it.t0, &it.t1);
+            if (it.t0 >= it.t1) continue;
+            it.seq = b;
+            it.kvh = h;
+            it.kb0 = kb;
+            it.q0 = q0;
+            it.q_len = q_lens[b];
+            it.kv_len = kv_lens[b];
+            pairs.push_back(it);
+            units.push_back((it.t1 - it.t0 + tile - 1) / tile);
           }
       }
       sf_paged_list& l = p.mass;
       l = sf_paged_list{};
-      if (!units.empty()) {
-        const int w = static_cast<int>(std::min<int64_t>(t.mass_workers, static_cast<int64_t>(units.size())));
-        if (top * 4 * w > total) {
-          // blocks that are a good part of a worker's share: the dearest first, each to the
-          // worker with the least so far
-          std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.cost > b.cost; });
-          std::vector<std::vector<PagedMassItem>> of(w);
-          typedef std::pair<int64_t, int> Load;
-          std::priority_queue<Load, std::vector<Load>, std::greater<Load>> least;
-          for (int i = 0; i < w; ++i) least.push({0, i});
-          for (const Unit& u : units) {
-            Load x = least.top();
-            least.pop();
-            of[x.second].push_back(u.item);
-            x.first += u.cost;
-            least.push(x);
-          }
-          for (int i = 0; i < w; ++i) {
-            first.push_back(static_cast<int32_t>(items.size()));
-            items.insert(items.end(), of[i].begin(), of[i].end());
-          }
-        } else {
-          int64_t done = 0;
-          int worker = -1;
-          for (const Unit& u : units) {
-            const int mine = static_cast<int>(std::min<int64_t>(w - 1, done * w / total));
-            const bool fresh = mine != worker;
-            while (worker < mine) {
-              first.push_back(static_cast<int32_t>(items.size()));
-              ++worker;
-            }
-            if (!fresh && !items.empty() && items.back().seq == u.item.seq && items.back().kvh == u.item.kvh &&
-                items.back().kb1 == u.item.kb0)
-              items.back().kb1 = u.item.kb1;
-            else
-              items.push_back(u.item);
-            done += u.cost;
-          }
-          while (static_cast<int>(first.size()) < w) first.push_back(static_cast<int32_t>(items.size()));
-        }
-        first.push_back(static_cast<int32_t>(items.size()));
-        l.workers = w;
-        l.n_items = static_cast<int32_t>(items.size());
+      if (!pairs.empty()) {
+        int slots = 0;
+        // loading two key blocks takes about as long as two tiles
+        deal(units, 2, t.mass_workers, &pieces, &first, &cuts, &slots);
+        l.slots = slots;
+        l.n_items = static_cast<int32_t>(pieces.size());
+        l.workers = static_cast<int32_t>(first.size()) - 1;
+        l.n_merges = static_cast<int32_t>(cuts.size());
       }
       l.items = static_cast<int32_t>(at);
-      memcpy(words + at, items.data(), items.size() * sizeof(PagedMassItem));
-      at += static_cast<int64_t>(items.size()) * kMassWords;
+      for (const Piece& x : pieces) {
+        PagedMassItem it = pairs[x.what];
+        it.i0 = x.i0;
+        it.i1 = x.i1;
+        it.slot = x.slot;
+        memcpy(words + at, &it, sizeof(it));
+        at += kMassWords;
+      }
+      l.merges = static_cast<int32_t>(at);
+      for (const Cut& c : cuts) {
+        const PagedMassItem& it = pairs[c.what];
+        const PagedMassMerge m{it.seq, it.kvh, it.kb0, c.slot0, c.n, it.q_len, it.kv_len, 0};
+        memcpy(words + at, &m, sizeof(m));
+        at += kMassMergeWords;
+      }
       l.first = static_cast<int32_t>(at);
       memcpy(words + at, first.data(), first.size() * 4);
       at = up4(at + static_cast<int64_t>(first.size()));
+      p.ws_bytes = std::max(p.ws_bytes, mass_ws(l));
     }
     p.words = std::max<int64_t>(at, 4);
     p.dev = nullptr;
@@ -496,6 +485,9 @@ int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool
   p.items = reinterpret_cast<const PagedMassItem*>(plan->dev + plan->mass.items);
   p.first = plan->dev + plan->mass.first;
   p.workers = plan->mass.workers;
+  p.merges = reinterpret_cast<const PagedMassMerge*>(plan->dev + plan->mass.merges);
+  p.n_merges = plan->mass.n_merges;
+  p.part = static_cast<float*>(plan->ws);
   p.H = plan->H;
   p.Hkv = plan->Hkv;
   p.G = plan->H / plan->Hkv;
@@ -507,8 +499,9 @@ int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool
   p.scale = scale;
   p.err = plan->err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return status(plan->dtype == SF_DTYPE_BF16 ? launch_paged_mass_tc(p, st) : launch_paged_mass_simt(plan->dtype, p, st),
-                "paged_attention_mass");
+  cudaError_t e = plan->dtype == SF_DTYPE_BF16 ? launch_paged_mass_tc(p, st) : launch_paged_mass_simt(plan->dtype, p, st);
+  if (e == cudaSuccess) e = launch_paged_mass_merge(p, st);
+  return status(e, "paged_attention_mass");
 }
 
 int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_table, int64_t dst_stride,

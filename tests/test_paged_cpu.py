@@ -9,7 +9,7 @@ from specfold_b200 import _lib
 from specfold_b200 import kernels as K
 from tests import paged_reference as ref
 
-ITEM, MERGE, MASS = 12, 8, 8                      # words of the plan's records
+ITEM, MERGE, MASS, MASS_MERGE = 12, 8, 12, 8                      # words of the plan's records
 
 
 def build(q_lens, kv_lens, **kw):
@@ -79,17 +79,28 @@ def test_a_plan_covers_every_row_and_key_once(seed):
         merged = [w[part.merges + MERGE * x:][:MERGE] for x in range(part.n_merges)]
         assert [s for m in merged for s in range(m[3], m[3] + m[4])] == used
     assert len(rows) == sum(q) * Hkv
-    units = set()
+    # weights: pairs of key blocks against tiles of tokens
+    per, seen, used = max(1, (128 if c.dtype else 64) // G), {}, []
     for x in range(c.mass.n_items):
-        seq, kvh, k0, k1, q0, ql, kv, _ = w[c.mass.items + MASS * x:][:MASS]
-        assert (ql, kv, q0) == (q[seq], n[seq], sum(q[:seq]))
-        for kb in range(k0, k1):
-            assert (seq, kvh, kb) not in units and kb * 128 < n[seq]
-            units.add((seq, kvh, kb))
+        seq, kvh, kb, t0, t1, i0, i1, slot, q0, ql, kv, _ = w[c.mass.items + MASS * x:][:MASS]
+        assert (ql, kv, q0) == (q[seq], n[seq], sum(q[:seq])) and kb % 2 == 0 and kb * 128 < kv
+        seen.setdefault((seq, kvh, kb), []).append((i0, i1, slot, t0, t1))
+        used += [slot] if slot >= 0 else []
+    assert used == list(range(c.mass.slots))
+    for pieces in seen.values():
+        at = 0
+        for i0, i1, slot, t0, t1 in pieces:
+            assert i0 == at and i1 > i0 and (slot >= 0) == (len(pieces) > 1)
+            at = i1
+        assert at == -(-(t1 - t0) // per)
+    merged = [w[c.mass.merges + MASS_MERGE * x:][:MASS_MERGE] for x in range(c.mass.n_merges)]
+    assert [s for m in merged for s in range(m[3], m[3] + m[4])] == used
     for b in range(len(q)):
         for t in range(q[b]):
             for kb in visible_blocks(q[b], n[b], t, block, window, sinks):
-                assert all((b, h, kb) in units for h in range(Hkv))
+                for h in range(Hkv):
+                    t0, t1 = seen[b, h, kb // 2 * 2][0][3:]
+                    assert t0 <= t < t1
 
 
 GOOD = dict(dtype=1, H=8, Hkv=2, hd=128, page_size=64, block=1)
