@@ -73,6 +73,15 @@ struct PagedMask {
     const int l = pos(i) - window + 1;
     return l > 0 ? l : 0;
   }
+  // the tokens that see one key, 0 <= key < kv_len: [first, last), empty when last <= first
+  __host__ __device__ void key_tokens(int key, int* first, int* last) const {
+    const int64_t off = static_cast<int64_t>(key) - (kv_len - q_len);   // its place in the chunk
+    int f = 0, l = q_len;
+    if (block > 0 && off >= 0) f = static_cast<int>(off / block * block);
+    if (window > 0 && key >= sinks && off + window < l) l = off + window > 0 ? static_cast<int>(off + window) : 0;
+    *first = f;
+    *last = l;
+  }
   // keys that some token sees in block kb
   __host__ __device__ PagedRange block_range(int kb) const {
     int f, l;

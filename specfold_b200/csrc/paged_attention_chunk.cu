@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           __syncwarp();
           if (any) {
             tmem_ld8(tmem + 256 + t * 128 + lane_off + c, o);
-            tmem_ld_wait();
+            tmem_wait<8>(o);
           }
           if (any && c + 8 == HD) {                      // O is read: the next item may begin
             tc_fence_before();
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           float v[64];
           tmem_ld32(tH, v);
           tmem_ld32(tH + 32, v + 32);
-          tmem_ld_wait();
+          tmem_wait<64>(v);
           if (edge) {
             const int c0 = k0 + half * 64, h = hi - c0, b = lo - c0, f = range.sinks - c0;
 #pragma unroll
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               for (int c = 0; c < HD; c += 16) {
                 float o[16];
                 tmem_ld16(tO + c, o);
-                tmem_ld_wait();
+                tmem_wait<16>(o);
                 uint32_t e[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) e[j] = __float_as_uint(o[j] * alpha);

@@ -378,7 +378,10 @@ __global__ void __launch_bounds__(kMassBlocks * kPagedKB) paged_mass_merge_kerne
   const PagedMassMerge w = p.merges[blockIdx.x];
   const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
   const int key = w.kb0 * kPagedKB + threadIdx.x;
-  if (key >= w.kv_len || !mask.block_range(key / kPagedKB).has(key)) return;
+  if (key >= w.kv_len) return;
+  int f, l;
+  mask.key_tokens(key, &f, &l);
+  if (f >= l) return;                                   // no token sees it
   float sum = 0.f;
   for (int i = 0; i < w.n; ++i) sum += p.part[static_cast<int64_t>(w.slot0 + i) * kMassBlocks * kPagedKB + threadIdx.x];
   *mass_slot(p, w.seq, w.kvh, key) += sum;

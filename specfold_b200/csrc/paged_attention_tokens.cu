@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 10);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
       const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
       const int qb = qn & 1;
-      ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&q_empty[qb], ((qn >> 1) & 1) ^ 1, p.err));
+      ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[qb], ((qn >> 1) & 1) ^ 1, p.err, abort_flag));
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(&q_full[qb], REP * KCH * (RC / p.G) * p.G * 128);
       __syncwarp();
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       for (int i = w.i0; ok && i < w.i1; ++i)
         for (int kv = 0; kv < 2; ++kv, ++u) {
           const int s = u % NS;
-          ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&empty[s], ((u / NS) & 1) ^ 1, p.err));
+          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((u / NS) & 1) ^ 1, p.err, abort_flag));
           if (!ok) break;
           load_key_block<HD>(sm + L::ring + s * L::kTile, kv ? &tmV : &tmK, &full[s], p.pool, w, range,
                              w.block(i), lane, p.err);
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t id_s = idesc_bf16(128, kPagedKB);
       const uint32_t id_pv = idesc_bf16(128, HD, 0, 1);
       uint32_t n = 0;                                    // key blocks whose S was issued
@@ -148,18 +148,18 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       // O += P V of block x (its place in the stream of blocks)
       auto issue_pv = [&](uint32_t x, bool begin) -> bool {
         if (begin) {
-          if (*abort_flag || !mbar_wait(o_free, (items & 1) ^ 1, p.err)) return false;
+          if (!wait_or_abort(o_free, (items & 1) ^ 1, p.err, abort_flag)) return false;
           ++items;
         }
         const uint32_t u = 2 * x + 1;
-        if (*abort_flag || !mbar_wait(p_full, x & 1, p.err) || !mbar_wait(&full[u % NS], (u / NS) & 1, p.err))
+        if (!wait_or_abort(&full[u % NS], (u / NS) & 1, p.err, abort_flag) ||
+            !wait_or_abort(p_full, x & 1, p.err, abort_flag))
           return false;
         tc_fence_after();
-        const uint32_t v_s = smem_u32(sm + L::ring + (u % NS) * L::kTile);
+        const uint32_t v_lo = ((smem_u32(sm + L::ring) + (u % NS) * L::kTile) >> 4) | ((kPagedBox >> 4) << 16);
 #pragma unroll
         for (int kk = 0; kk < kPagedKB / 16; ++kk)
-          umma_f16_ts(tO, tP + kk * 8, sdesc_mnmajor_sw128(v_s + kk * 2048, kPagedBox), id_pv,
-                      (!begin || kk > 0) ? 1u : 0u);
+          umma_f16_ts(tO, tP + kk * 8, desc(v_lo + kk * 128), id_pv, (!begin || kk > 0) ? 1u : 0u);
         umma_commit(pv_done);
         umma_commit(&empty[u % NS]);
         return true;
@@ -169,20 +169,20 @@ __global__ void __launch_bounds__(kTokThreads, 1)
         const int i0 = p.items[it].i0, i1 = p.items[it].i1;
         if (i0 == i1) continue;
         const int qb = qn & 1;
-        ok = !*abort_flag && mbar_wait(&q_full[qb], (qn >> 1) & 1, p.err);
-        const uint32_t q_s = smem_u32(sm + L::q + qb * L::kTile);
+        ok = wait_or_abort(&q_full[qb], (qn >> 1) & 1, p.err, abort_flag);
+        const uint32_t q_lo = ((smem_u32(sm + L::q) + qb * L::kTile) >> 4) | (1u << 16);
         for (int i = i0; ok && i < i1; ++i) {
           const uint32_t u = 2 * n;
           // S buffer n & 1 was read by the softmax of block n - 2 before it handed over its P,
           // which the P V of that block, issued before, has waited for
-          ok = !*abort_flag && mbar_wait(&full[u % NS], (u / NS) & 1, p.err);
+          ok = wait_or_abort(&full[u % NS], (u / NS) & 1, p.err, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t k_s = smem_u32(sm + L::ring + (u % NS) * L::kTile);
+          const uint32_t k_lo = ((smem_u32(sm + L::ring) + (u % NS) * L::kTile) >> 4) | (1u << 16);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
-            umma_f16(tmem + (n & 1) * 128, sdesc_kmajor_sw128(q_s + (kk >> 2) * kPagedBox + (kk & 3) * 32),
-                     sdesc_kmajor_sw128(k_s + (kk >> 2) * kPagedBox + (kk & 3) * 32), id_s, kk > 0 ? 1u : 0u);
+            umma_f16(tmem + (n & 1) * 128, desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
+                     desc(k_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id_s, kk > 0 ? 1u : 0u);
           umma_commit(&s_full[n & 1]);
           umma_commit(&empty[u % NS]);
           if (i + 1 == i1) umma_commit(&q_empty[qb]);
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int i = w.i0; i < w.i1; ++i, ++n) {
         const int k0 = w.block(i) * kPagedKB;
-        ok = __all_sync(0xffffffffu, ok && !*abort_flag && mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.err));
+        ok = __all_sync(0xffffffffu, ok && wait_or_abort(&s_full[n & 1], (n >> 1) & 1, p.err, abort_flag));
         if (!ok) break;
         tc_fence_after();
         float v[NC];
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
         if (busy) {
 #pragma unroll
           for (int c = 0; c < NC; c += 32) tmem_ld32(tmem + (n & 1) * 128 + lane_off + copy * NC + c, v + c);
-          tmem_ld_wait();
+          tmem_wait<NC>(v);
           if (k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks)) {
             const int h = hi - k0 - copy * NC, b = lo - k0 - copy * NC, f = range.sinks - k0 - copy * NC;
 #pragma unroll
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
               for (int c = 0; c < HD; c += 32) {
                 float o[32];
                 tmem_ld32(tO + lane_off + c, o);
-                tmem_ld_wait();
+                tmem_wait<32>(o);
                 uint32_t b[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) b[j] = __float_as_uint(o[j] * alpha);
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
         float o[32];
         if (any && busy) {
           tmem_ld32(tO + lane_off + c, o);
-          tmem_ld_wait();
+          tmem_wait<32>(o);
         }
 #pragma unroll
         for (int j = 0; j < 32; ++j) red[r * kRedLd + j] = any && f != 0.f ? o[j] * f : 0.f;

@@ -10,7 +10,7 @@
 //   warps 4-7, 8-11   exponentials and sums of the first and of the second block
 //   warp 0            TMA: key blocks and query tiles, through rings of their own
 //   warp 1            tcgen05.mma, two S^T buffers of 128 columns for each block (all of TMEM)
-//   warp 2            lse and the mask's bounds of the tile's rows into shared memory
+//   warp 2            lse of the tile's rows into shared memory
 // Bound: for chunks by the special-function unit, one exponential per (row, key): 1024 cycles for
 // a 128 x 128 tile against 512 of products; for single tokens by the bytes of the keys.
 #include "paged_tc.cuh"
@@ -23,13 +23,11 @@ template <int HD>
 struct MassSmem {
   static constexpr int kTile = HD / 64 * kPagedBox;      // 128 rows
   static constexpr int kStages = 3;                      // of keys, of queries
-  static constexpr int kRows = 4;                        // stages of lse and bounds
+  static constexpr int kRows = 4;                        // stages of lse
   static constexpr int k = 0;                            // [kStages][kTile]
   static constexpr int q = k + kStages * kTile;          // [kStages][kTile]
   static constexpr int lse = q + kStages * kTile;        // [kRows][128] floats
-  static constexpr int hi = lse + kRows * 512;           // [kRows][128] ints
-  static constexpr int lo = hi + kRows * 512;
-  static constexpr int bars = lo + kRows * 512;
+  static constexpr int bars = lse + kRows * 512;
   static constexpr int bytes = bars + 256 + 1024;        // + alignment of the base
 };
 
@@ -190,10 +188,8 @@ __global__ void __launch_bounds__(kMassThreads, 1)
       mbar_wait(drain, 0, p.err);
     }
   } else if (warp == 2) {
-    // ---------------------------------------------------------------- lse and bounds of the rows
+    // ---------------------------------------------------------------- lse of the rows
     float* s_lse = reinterpret_cast<float*>(sm + L::lse);
-    int* s_hi = reinterpret_cast<int*>(sm + L::hi);
-    int* s_lo = reinterpret_cast<int*>(sm + L::lo);
     int tok[4], head[4];                                 // of this lane's four rows
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -202,7 +198,6 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     }
     for (int it = first; ok && it < last; ++it) {
       const PagedMassItem m = p.items[it];
-      const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
       for (int x = m.i0; x < m.i1; ++x, ++qn) {
         const uint32_t s = qn % NR;
         const int t = m.t0 + x * tq, n = min(tq, m.t1 - t);
@@ -216,12 +211,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
         ok = __all_sync(0xffffffffu, wait_or_abort(&r_empty[s], ((qn / NR) & 1) ^ 1, p.err, abort_flag));
         if (!ok) break;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = s * 128 + lane + 32 * j, i = t + min(tok[j], n - 1);
-          s_lse[c] = -v[j];
-          s_hi[c] = mask.hi(i);
-          s_lo[c] = mask.lo(i);
-        }
+        for (int j = 0; j < 4; ++j) s_lse[s * 128 + lane + 32 * j] = -v[j];
         __syncwarp();
         if (lane == 0) mbar_arrive(&r_full[s]);
       }
@@ -232,30 +222,47 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     const int y = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t tS = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + y * 256;
     const float* s_lse = reinterpret_cast<const float*>(sm + L::lse);
-    const int* s_hi = reinterpret_cast<const int*>(sm + L::hi);
-    const int* s_lo = reinterpret_cast<const int*>(sm + L::lo);
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint64_t scale2 = pair(sl2, sl2);
     uint32_t bn = 0;                                     // this block's scores so far
+    // One item ahead: which key is this thread's, the tokens that see it, and where its sum goes
+    // (the page id, then the weight so far, are on their way while the item before is worked on).
+    struct Ahead {
+      PagedMassItem m;
+      int f, l, id;                                      // tokens [f, l) see the key; its page
+    };
+    auto begin = [&](int it) {
+      Ahead a;
+      a.m = p.items[it];
+      const int key = (a.m.kb0 + y) * kPagedKB + r;
+      a.f = a.l = a.id = 0;
+      if (key < a.m.kv_len) {
+        const PagedMask mask{p.block, p.window, p.sinks, a.m.q_len, a.m.kv_len};
+        mask.key_tokens(key, &a.f, &a.l);
+        if (a.f < a.l && a.m.slot < 0) a.id = p.pool.table[a.m.seq * p.pool.table_stride + (key >> p.pool.page_shift)];
+      }
+      return a;
+    };
+    auto target = [&](const Ahead& a) -> float* {
+      if (a.f >= a.l) return nullptr;
+      if (a.m.slot >= 0) return p.part + static_cast<int64_t>(a.m.slot) * kMassBlocks * kPagedKB + y * kPagedKB + r;
+      const int key = (a.m.kb0 + y) * kPagedKB + r;
+      int id = a.id;
+      if (id < 0 || id >= p.pool.num_pages) {            // flagged, and nothing is written
+        flag_error(p.err, SF_DEV_ERR_INDEX);
+        return nullptr;
+      }
+      return p.pool.mass + ((static_cast<int64_t>(id) * p.Hkv + a.m.kvh) << p.pool.page_shift) +
+             (key & ((1 << p.pool.page_shift) - 1));
+    };
+    Ahead cur = begin(first < last ? first : 0);
+    float* dst = target(cur);
+    float old = dst != nullptr && cur.m.slot < 0 ? *dst : 0.f;
     for (int it = first; ok && it < last; ++it) {
-      const PagedMassItem m = p.items[it];
+      const PagedMassItem& m = cur.m;
+      const Ahead next = begin(it + 1 < last ? it + 1 : it);
       const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
       const MassBlock blk(mask, m.kb0 + y, m.kv_len);
-      const PagedRange range = mask.block_range(blk.f < blk.l ? m.kb0 + y : 0);
-      const int k0 = (m.kb0 + y) * kPagedKB, key = k0 + r;
-      const bool seen = blk.f < blk.l && range.has(key);
-      float* dst = nullptr;                              // this key's weight, read while the tiles run
-      float old = 0.f;
-      if (seen) {
-        if (m.slot >= 0) {
-          dst = p.part + static_cast<int64_t>(m.slot) * kMassBlocks * kPagedKB + y * kPagedKB + r;
-        } else {
-          const int page = paged_page(p.pool, m.seq, key >> p.pool.page_shift, p.err);
-          dst = p.pool.mass + ((static_cast<int64_t>(page) * p.Hkv + m.kvh) << p.pool.page_shift) +
-                (key & ((1 << p.pool.page_shift) - 1));
-          old = *dst;
-        }
-      }
       uint64_t sum0 = pair(0.f, 0.f), sum1 = sum0;
       for (int x = m.i0; x < m.i1; ++x, ++qn) {
         const uint32_t s = qn % NR, b = bn & 1;
@@ -267,33 +274,42 @@ __global__ void __launch_bounds__(kMassThreads, 1)
         if (!ok) break;
         if (mine) {
           tc_fence_after();
-          const bool edge = k0 + kPagedKB > mask.hi(t) || (k0 < mask.lo(t_end - 1) && k0 + kPagedKB > range.sinks);
-#pragma unroll 1
-          for (int c = 0; c < rows; c += 32) {
-            float v[32];
-            tmem_ld32(tS + b * 128 + c, v);
+          // columns [c_lo, c_hi) are rows that see this thread's key
+          const int c_lo = max(cur.f - t, 0) * p.G, c_hi = max(min(cur.l, t_end) - t, 0) * p.G;
+          // the weights of columns [c, c + 32); what is no row of the tile is outside [c_lo, c_hi)
+          auto add = [&](float* v, int c) {
             const float4* lse4 = reinterpret_cast<const float4*>(s_lse + s * 128 + c);
-            tmem_ld_wait();
-            if (c + 32 > rows) {                         // columns that are no rows may hold anything
+            if (__any_sync(0xffffffffu, c < c_lo || c + 32 > c_hi)) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (c + j >= rows) v[j] = 0.f;           // (their -lse is -inf)
+                if (c + j < c_lo || c + j >= c_hi) v[j] = -INFINITY;
             }
-            if (edge) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int h = s_hi[s * 128 + c + j], l = s_lo[s * 128 + c + j];
-                if (!(key < h && (key >= l || key < range.sinks))) v[j] = -INFINITY;
+            for (int g = 0; g < 32; g += 8) {
+              if (c + g >= rows) break;
+#pragma unroll
+              for (int j = g; j < g + 8; j += 4) {
+                const float4 e = lse4[j / 4];
+                float a0, a1, a2, a3;
+                unpair(fma2(pair(v[j], v[j + 1]), scale2, pair(e.x, e.y)), a0, a1);
+                unpair(fma2(pair(v[j + 2], v[j + 3]), scale2, pair(e.z, e.w)), a2, a3);
+                sum0 = add2(sum0, pair(ex2(a0), ex2(a1)));
+                sum1 = add2(sum1, pair(ex2(a2), ex2(a3)));
               }
             }
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 e = lse4[j / 4];
-              float a0, a1, a2, a3;
-              unpair(fma2(pair(v[j], v[j + 1]), scale2, pair(e.x, e.y)), a0, a1);
-              unpair(fma2(pair(v[j + 2], v[j + 3]), scale2, pair(e.z, e.w)), a2, a3);
-              sum0 = add2(sum0, pair(ex2(a0), ex2(a1)));
-              sum1 = add2(sum1, pair(ex2(a2), ex2(a3)));
+          };
+          const uint32_t tB = tS + b * 128;
+          float va[32], vb[32];                          // one of them on its way
+          tmem_ld32(tB, va);
+#pragma unroll 1
+          for (int c = 0; c < rows; c += 64) {
+            tmem_wait<32>(va);
+            if (c + 32 < rows) tmem_ld32(tB + c + 32, vb);
+            add(va, c);
+            if (c + 32 < rows) {
+              tmem_wait<32>(vb);
+              if (c + 64 < rows) tmem_ld32(tB + c + 64, va);
+              add(vb, c + 32);
             }
           }
           tc_fence_before();
@@ -305,9 +321,14 @@ __global__ void __launch_bounds__(kMassThreads, 1)
           mbar_arrive(&r_empty[s]);
         }
       }
+      float* next_dst = target(next);
+      const float next_old = it + 1 < last && next_dst != nullptr && next.m.slot < 0 ? *next_dst : 0.f;
       float a0, a1;
       unpair(add2(sum0, sum1), a0, a1);
       if (dst != nullptr && ok) *dst = old + (a0 + a1);
+      cur = next;
+      dst = next_dst;
+      old = next_old;
     }
     if (!ok) *abort_flag = 1;
   }

@@ -51,6 +51,16 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Waits for this thread's TMEM loads; the N values of v count as written here, so that no use of
+// them can be scheduled before the wait.
+template <int N>
+__device__ __forceinline__ void tmem_wait(float* v) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+    asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]),
+                 "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
 __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
