@@ -369,6 +369,7 @@ typedef struct sf_paged_plan {
   sf_paged_list attn[2], mass;       /* [0]: few query rows per kv head, [1]: many */
   int64_t words;                     /* words of the plan */
   size_t ws_bytes;                   /* scratch of the calls below */
+  size_t ws_zero;                    /* its first bytes that must be zero before the first call */
   /* set by the caller before the first use */
   const int32_t* dev;                /* the plan's words in device memory */
   void* ws;                          /* ws_bytes of device memory */
@@ -379,7 +380,9 @@ typedef struct sf_paged_plan {
  * the mask alone, so one plan serves every layer of the step.  q_lens, kv_lens and words are
  * HOST arrays; words must hold sf_paged_plan_words(...) words (0: an argument is wrong, see
  * sf_last_error).  The caller copies plan->words words to device memory and sets dev, ws and
- * err.  Calls that share a plan share its scratch: they must not overlap on the GPU. */
+ * err; the first ws_zero bytes of ws must be zero (counters, which the calls leave at zero; after
+ * a device error they may not be: zero them again).  Calls that share a plan share its scratch:
+ * they must not overlap on the GPU. */
 int64_t sf_paged_plan_words(const sf_paged_plan* plan, const int32_t* q_lens,
                             const int32_t* kv_lens);
 int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_t* kv_lens,

@@ -16,6 +16,10 @@
 // order of the pieces, so results do not depend on timing.
 #pragma once
 
+#include <mutex>
+#include <utility>
+#include <vector>
+
 #include "../../include/specfold_b200.h"
 #include "sf_kernels.cuh"
 
@@ -30,6 +34,7 @@ struct alignas(16) PagedItem {
   int32_t seq, kvh, tok0, ntok;       // the tile: tokens [tok0, tok0 + ntok) of the chunk
   int32_t i0, i1, slot, sink_blks;    // slot < 0: writes the output itself
   int32_t lo_blk, q0, q_len, kv_len;  // q0: the chunk's first row in q / out
+  int32_t cut, pad0, pad1, pad2;      // which cut tile this is a piece of
   __host__ __device__ int block(int i) const { return i < sink_blks ? i : i - sink_blks + lo_blk; }
 };
 // A tile whose run was cut into n pieces, in slots [slot0, slot0 + n)
@@ -143,6 +148,7 @@ struct PagedAttnParams {
   int workers;
   const PagedMerge* merges;
   int n_merges;
+  int32_t* arrived;                 // [n_merges] pieces of each cut tile that are done (zero between calls)
   float* part_O;                    // [slots][rows][hd]
   float* part_ml;                   // [slots][rows][2]
   int rows, tile_tokens;            // rows of a slot; tokens of 128 (64) rows
@@ -169,6 +175,28 @@ struct PagedMassParams {
   int* err;
 };
 
+// Raises a kernel's dynamic shared memory limit, once per kernel and device.
+template <typename F>
+inline cudaError_t allow_smem(F* kernel, int bytes) {
+  static std::mutex mu;
+  static std::vector<std::pair<const void*, uint64_t>> seen;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const void* key = reinterpret_cast<const void*>(kernel);
+  std::lock_guard<std::mutex> lock(mu);
+  for (auto& x : seen)
+    if (x.first == key) {
+      if (dev < 64 && (x.second >> dev & 1)) return cudaSuccess;
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      if (e == cudaSuccess && dev < 64) x.second |= uint64_t{1} << dev;
+      return e;
+    }
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) seen.push_back({key, uint64_t{1} << dev});
+  return e;
+}
+
 // page id of position pos; an id outside the pool is flagged and read as page 0
 __device__ __forceinline__ int paged_page(const PagedPool& p, int seq, int idx, int* err) {
   const int id = p.table[seq * p.table_stride + idx];
@@ -177,6 +205,39 @@ __device__ __forceinline__ int paged_page(const PagedPool& p, int seq, int idx, 
     return 0;
   }
   return id;
+}
+
+// One warp joins the pieces of row r (row pr of the slots) of a cut tile, in their order.
+template <typename T, int HD>
+__device__ __forceinline__ void paged_join_row(const PagedAttnParams& p, const PagedMerge& w, int r, int pr, int lane) {
+  constexpr int E = HD / 32;
+  float m = -INFINITY;
+  for (int i = lane; i < w.n; i += 32)
+    m = fmaxf(m, p.part_ml[2 * (static_cast<int64_t>(w.slot0 + i) * p.rows + pr)]);
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < w.n; ++i) {
+    const int64_t at = static_cast<int64_t>(w.slot0 + i) * p.rows + pr;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+    const float f = exp2f(ml.x - ref);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p.part_O + at * HD + lane * E + e);
+      o[e] = fmaf(v.x, f, o[e]);
+      o[e + 1] = fmaf(v.y, f, o[e + 1]);
+    }
+  }
+  const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + r / p.G) * p.H + w.kvh * p.G + r % p.G;
+  const float inv = l == 0.f ? 0.f : 1.f / l;           // a NaN sum stays one
+  T* dst = static_cast<T*>(p.out) + row * HD + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = Elt<T>::from_f(o[e] * inv);
+  if (lane == 0) p.lse[row] = m * 0.6931471805599453f + logf(l);
 }
 
 cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cudaStream_t st);

@@ -486,8 +486,7 @@ static cudaError_t attention_chunk(const PagedAttnParams& p, cudaStream_t st) {
   if (!query_tmap(&tq, p.q, p.q_tok, p.q_head, p.T, p.H, HD, p.G, p.tile_tokens) ||
       !pool_tmap(&tk, p.pool.k, p.pool, p.Hkv, HD) || !pool_tmap(&tv, p.pool.v, p.pool, p.Hkv, HD))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(paged_attention_chunk_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       ChunkSmem<HD>::bytes);
+  cudaError_t e = allow_smem(paged_attention_chunk_kernel<HD>, ChunkSmem<HD>::bytes);
   if (e != cudaSuccess) return e;
   paged_attention_chunk_kernel<HD><<<p.workers, kChunkThreads, ChunkSmem<HD>::bytes, st>>>(tq, tk, tv, p);
   return launched();

@@ -232,40 +232,12 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
 // Joins the pieces of the tiles that were cut: one warp per row, pieces in order.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnParams p) {
-  constexpr int E = HD / 32;
-  pdl_wait();
   const PagedMerge w = p.merges[blockIdx.y];
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (r >= w.ntok * p.G) return;
-  const int t = r / p.G, g = r % p.G;
-  const int half = t / p.tile_tokens;
-  const int pr = half * 128 + (t - half * p.tile_tokens) * p.G + g;
-  float m = -INFINITY;
-  for (int i = 0; i < w.n; ++i)
-    m = fmaxf(m, p.part_ml[2 * (static_cast<int64_t>(w.slot0 + i) * p.rows + pr)]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < w.n; ++i) {
-    const int64_t at = static_cast<int64_t>(w.slot0 + i) * p.rows + pr;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    const float f = exp2f(ml.x - ref);
-    l = fmaf(ml.y, f, l);
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_O + at * HD + lane * E + e);
-      o[e] = fmaf(v.x, f, o[e]);
-      o[e + 1] = fmaf(v.y, f, o[e + 1]);
-    }
-  }
-  const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + t) * p.H + w.kvh * p.G + g;
-  const float inv = l == 0.f ? 0.f : 1.f / l;           // a NaN sum stays one
-  T* dst = static_cast<T*>(p.out) + row * HD + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = Elt<T>::from_f(o[e] * inv);
-  if (lane == 0) p.lse[row] = m * 0.6931471805599453f + logf(l);
+  const int t = r / p.G, half = t / p.tile_tokens;
+  const int pr = half * 128 + (t - half * p.tile_tokens) * p.G + r % p.G;
+  paged_join_row<T, HD>(p, w, r, pr, lane);
 }
 
 cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st) {
@@ -284,8 +256,7 @@ template <typename T, int HD, int RM>
 static cudaError_t attention_simt(const PagedAttnParams& p, cudaStream_t st) {
   constexpr int R = 16 * RM;
   constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + R * (kSimtKeys + 4)) * 4;
-  cudaError_t e = cudaFuncSetAttribute(paged_attention_simt_kernel<T, HD, RM>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem(paged_attention_simt_kernel<T, HD, RM>, smem);
   if (e != cudaSuccess) return e;
   paged_attention_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
   return launched();
@@ -397,8 +368,7 @@ template <typename T, int HD, int RM>
 static cudaError_t mass_simt(const PagedMassParams& p, cudaStream_t st) {
   constexpr int R = 16 * RM;
   constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + 16 * kSimtKeys) * 4;
-  cudaError_t e = cudaFuncSetAttribute(paged_mass_simt_kernel<T, HD, RM>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem(paged_mass_simt_kernel<T, HD, RM>, smem);
   if (e != cudaSuccess) return e;
   paged_mass_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
   return launched();

@@ -12,7 +12,8 @@
 // rate); the softmax would not, with all of a row's 128 exponentials in one thread.  So with at
 // most 32 (64) rows they are loaded 4 (2) times, copy c takes the keys [c, c + 1) * 128 / REP of
 // every block, its weights elsewhere stay zero, and each copy accumulates its own (m, l, O);
-// they are joined once per item.
+// they are joined once per item.  The pieces of a tile that was cut between CTAs are joined by the
+// CTA that finishes last.
 //
 // The rescaling of O waits until a row's maximum has grown by 2^8: until then the weights are
 // merely up to 2^8 instead of 1, relative to the same reference in l and O, and lose nothing.
@@ -364,6 +365,30 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       }
     }
     if (!ok) *abort_flag = 1;
+    // The piece of a cut tile that comes last joins them all, in their order: the result does not
+    // depend on which one that is.  A share is contiguous, so only its first and its last item can
+    // be such pieces.
+    if (vote128(ok) && last > first && (p.items[first].slot >= 0 || p.items[last - 1].slot >= 0)) {
+      __threadfence();
+      vote128(true);
+#pragma unroll 1
+      for (int it = first; it < last; it += max(1, last - 1 - first)) {
+        const PagedItem w = p.items[it];
+        if (w.slot < 0) continue;
+        const PagedMerge g = p.merges[w.cut];
+        if (threadIdx.x == 64) {
+          const bool all = atomicAdd(&p.arrived[w.cut], 1) == g.n - 1;
+          if (all) p.arrived[w.cut] = 0;                 // for the next call
+          s_m[0] = all ? 1.f : 0.f;
+        }
+        vote128(true);
+        if (s_m[0] != 0.f) {
+          __threadfence();
+          for (int row = quarter; row < w.ntok * p.G; row += 4) paged_join_row<__nv_bfloat16, HD>(p, g, row, row, lane);
+        }
+        vote128(true);
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -377,8 +402,7 @@ static cudaError_t attention_tokens(const PagedAttnParams& p, cudaStream_t st) {
   if (!query_tmap(&tq, p.q, p.q_tok, p.q_head, p.T, p.H, HD, p.G, 128 / REP / p.G) ||
       !pool_tmap(&tk, p.pool.k, p.pool, p.Hkv, HD) || !pool_tmap(&tv, p.pool.v, p.pool, p.Hkv, HD))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(paged_attention_tokens_kernel<HD, REP>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, TokSmem<HD>::bytes);
+  cudaError_t e = allow_smem(paged_attention_tokens_kernel<HD, REP>, TokSmem<HD>::bytes);
   if (e != cudaSuccess) return e;
   paged_attention_tokens_kernel<HD, REP><<<p.workers, kTokThreads, TokSmem<HD>::bytes, st>>>(tq, tk, tv, p);
   return launched();

@@ -344,8 +344,7 @@ static cudaError_t mass_tc(const PagedMassParams& p, cudaStream_t st) {
   if (!query_tmap(&tq, p.q, p.q_tok, p.q_head, p.T, p.H, HD, p.G, 128 / p.G) ||
       !pool_tmap(&tk, p.pool.k, p.pool, p.Hkv, HD))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(paged_mass_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       MassSmem<HD>::bytes);
+  cudaError_t e = allow_smem(paged_mass_kernel<HD>, MassSmem<HD>::bytes);
   if (e != cudaSuccess) return e;
   paged_mass_kernel<HD><<<p.workers, kMassThreads, MassSmem<HD>::bytes, st>>>(tq, tk, p);
   return launched();

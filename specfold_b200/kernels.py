@@ -323,16 +323,24 @@ class _OnStream:
         self.device = device
         self._tensors = tensors
         self._home = torch.cuda.current_stream(device)
+        self._home_raw = self._home.cuda_stream
         self._ready = self._home.record_event()
 
-    def _stream(self) -> int:
-        st = torch.cuda.current_stream(self.device)
+    def _call(self, fn, what: str, *args) -> None:
+        """fn(*args, the current stream) on the plan's device"""
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self._call(fn, what, *args)
+        raw = torch._C._cuda_getCurrentRawStream(self.device.index)
         # (a capture begins after a synchronisation and may not wait for what it did not record)
-        if st != self._home and not torch.cuda.is_current_stream_capturing():
+        if raw != self._home_raw and not torch.cuda.is_current_stream_capturing():
+            st = torch.cuda.current_stream(self.device)
             st.wait_event(self._ready)
             for t in self._tensors:
                 t.record_stream(st)
-        return st.cuda_stream
+        status = fn(*args, raw)
+        if status:
+            _lib.check(status, what)
 
     def check(self) -> None:
         """Raises what the kernels reported (a page id outside the pool, a wait that ran out).
@@ -374,8 +382,10 @@ class PagedPlan(_OnStream):
         self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
         self._dev = words[:c.words].to(device)
         self._ws = torch.empty(max(c.ws_bytes, 256), dtype=torch.uint8, device=device)
+        self._ws[:c.ws_zero].zero_()
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
         c.dev, c.ws, c.err = self._dev.data_ptr(), self._ws.data_ptr(), self.err.data_ptr()
+        self._f32 = self.err.view(torch.float32)
         self._c = c
         self._ref = ctypes.byref(c)
         self._made(device, self._dev, self._ws, self.err)
@@ -408,47 +418,51 @@ class EvictPlan(_OnStream):
         self._made(device, self._lens, self.err)
 
 
-def _aligned_rows(t: torch.Tensor, what: str) -> Tuple[int, int]:
-    """(outer, head) strides of [N, H, hd] rows; those of an axis of one element are not used"""
-    if t.stride(2) != 1:
-        raise ValueError(f"{what}: head_dim must be contiguous")
-    H, hd = t.shape[1], t.shape[2]
-    head = t.stride(1) if H > 1 else hd
-    return (t.stride(0) if t.shape[0] > 1 else H * head), head
-
-
 def _paged_pool(k_pages, v_pages, table, mass_pages, plan, dtype):
-    if k_pages.dim() != 4:
+    shape, dev = k_pages.shape, plan.device
+    if len(shape) != 4:
         raise ValueError("pools are [pages, kv heads, page size, head_dim]")
-    N, Hkv, ps, hd = k_pages.shape
-    if Hkv != plan.kv_heads or ps != plan.page_size or k_pages.dtype != dtype or k_pages.stride(3) != 1:
+    N, Hkv, ps, hd = shape
+    stride = k_pages.stride()
+    if Hkv != plan.kv_heads or ps != plan.page_size or k_pages.dtype != dtype or stride[3] != 1:
         raise ValueError(f"the plan is for {dtype} pools of {plan.kv_heads} kv heads and pages of "
-                         f"{plan.page_size}, got {k_pages.dtype} {tuple(k_pages.shape)}")
-    if v_pages is not None and (v_pages.shape != k_pages.shape or v_pages.dtype != dtype
-                                or v_pages.stride() != k_pages.stride()):
+                         f"{plan.page_size}, got {k_pages.dtype} {tuple(shape)}")
+    if v_pages is None:
+        v_ptr = None
+    elif v_pages.shape != shape or v_pages.dtype != dtype or v_pages.stride() != stride:
         raise ValueError("k_pages and v_pages must share shape, dtype and strides")
-    if mass_pages is not None and (mass_pages.shape != (N, Hkv, ps) or mass_pages.dtype != torch.float32
-                                   or not mass_pages.is_contiguous()):
-        raise ValueError(f"mass_pages must be contiguous float32 {(N, Hkv, ps)}")
-    if (table.dim() != 2 or table.shape[0] != plan.sequences or table.dtype != torch.int32
-            or (table.shape[1] > 1 and table.stride(1) != 1)):
+    else:
+        v_ptr = v_pages.data_ptr()
+    if mass_pages is None:
+        m_ptr = None
+    elif (mass_pages.shape != (N, Hkv, ps) or mass_pages.dtype != torch.float32
+          or not mass_pages.is_contiguous() or mass_pages.device != dev):
+        raise ValueError(f"mass_pages must be contiguous float32 {(N, Hkv, ps)} on {dev}")
+    else:
+        m_ptr = mass_pages.data_ptr()
+    rows, width = table.shape if table.dim() == 2 else (-1, 0)
+    if rows != plan.sequences or table.dtype != torch.int32 or (width > 1 and table.stride(1) != 1):
         raise ValueError(f"the table must be int32 [{plan.sequences}, pages], rows contiguous")
-    dev = plan.device
-    for t in (k_pages, v_pages, mass_pages, table):
-        if t is not None and t.device != dev:
-            raise ValueError(f"the plan lives on {dev}, got a tensor on {t.device}")
+    if k_pages.device != dev or table.device != dev or (v_pages is not None and v_pages.device != dev):
+        raise ValueError(f"the plan lives on {dev}, got a tensor elsewhere")
+    # the stride of an axis of one element is not used (torch keeps odd ones)
     return _lib.SfPagedPool(
-        k_pages.data_ptr(), _ptr(v_pages), _ptr(mass_pages),
-        k_pages.stride(0) if N > 1 else Hkv * ps * hd, k_pages.stride(1) if Hkv > 1 else ps * hd,
-        k_pages.stride(2), table.data_ptr(),
-        table.stride(0) if table.shape[0] > 1 else table.shape[1], N, table.shape[1])
+        k_pages.data_ptr(), v_ptr, m_ptr, stride[0] if N > 1 else Hkv * ps * hd,
+        stride[1] if Hkv > 1 else ps * hd, stride[2], table.data_ptr(),
+        table.stride(0) if rows > 1 else width, N, width)
 
 
 def _paged_rows(t: torch.Tensor, heads: int, plan: PagedPlan, what: str) -> Tuple[int, int]:
+    """(token, head) strides of the new tokens' rows"""
     if t.shape != (plan.tokens, heads, plan.head_dim) or t.dtype != plan.dtype or t.device != plan.device:
         raise ValueError(f"{what} must be {plan.dtype} {(plan.tokens, heads, plan.head_dim)} on "
                          f"{plan.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return _aligned_rows(t, what)
+    tok, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{what}: head_dim must be contiguous")
+    if heads == 1:
+        head = plan.head_dim
+    return (tok if plan.tokens > 1 else heads * head), head
 
 
 def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k_new: torch.Tensor,
@@ -461,10 +475,8 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k_new: torch.T
     tok, head = _paged_rows(k_new, plan.kv_heads, plan, "k_new")
     if _paged_rows(v_new, plan.kv_heads, plan, "v_new") != (tok, head):
         raise ValueError("k_new and v_new must share their strides")
-    with torch.cuda.device(plan.device):
-        _lib.check(_lib.load().sf_paged_kv_append(plan._ref, ctypes.byref(pool), k_new.data_ptr(),
-                                                  v_new.data_ptr(), tok, head, plan._stream()),
-                   "paged_kv_append")
+    plan._call(_lib.load().sf_paged_kv_append, "paged_kv_append", plan._ref, ctypes.byref(pool),
+               k_new.data_ptr(), v_new.data_ptr(), tok, head)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -477,17 +489,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     pool = _paged_pool(k_pages, v_pages, table, None, plan, plan.dtype)
     tok, head = _paged_rows(q, plan.heads, plan, "q")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != q.device:
         raise ValueError("out must be contiguous, of q's shape, dtype and device")
     if lse is None:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        lse = plan._f32.new_empty((plan.tokens, plan.heads))
     elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse must be contiguous float32 [T, H] on q's device")
-    with torch.cuda.device(plan.device):
-        _lib.check(_lib.load().sf_paged_attention(
-            plan._ref, ctypes.byref(pool), q.data_ptr(), tok, head, out.data_ptr(), lse.data_ptr(),
-            plan.head_dim ** -0.5 if scale is None else scale, plan._stream()), "paged_attention")
+    plan._call(_lib.load().sf_paged_attention, "paged_attention", plan._ref, ctypes.byref(pool),
+               q.data_ptr(), tok, head, out.data_ptr(), lse.data_ptr(),
+               plan.head_dim ** -0.5 if scale is None else scale)
     return out, lse
 
 
@@ -501,11 +512,9 @@ def paged_attention_mass(q: torch.Tensor, k_pages: torch.Tensor, table: torch.Te
     tok, head = _paged_rows(q, plan.heads, plan, "q")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse must be contiguous float32 [T, H] on q's device")
-    with torch.cuda.device(plan.device):
-        _lib.check(_lib.load().sf_paged_attention_mass(
-            plan._ref, ctypes.byref(pool), q.data_ptr(), tok, head, lse.data_ptr(),
-            plan.head_dim ** -0.5 if scale is None else scale, plan._stream()),
-            "paged_attention_mass")
+    plan._call(_lib.load().sf_paged_attention_mass, "paged_attention_mass", plan._ref,
+               ctypes.byref(pool), q.data_ptr(), tok, head, lse.data_ptr(),
+               plan.head_dim ** -0.5 if scale is None else scale)
 
 
 def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass_pages: torch.Tensor,
@@ -520,12 +529,10 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, mass_pages: torch.
     if (dst_table.dim() != 2 or dst_table.shape[0] != plan.sequences or dst_table.dtype != torch.int32
             or (dst_table.shape[1] > 1 and dst_table.stride(1) != 1) or dst_table.device != plan.device):
         raise ValueError(f"dst_table must be int32 [{plan.sequences}, pages] on {plan.device}")
-    kept = torch.empty(plan.sequences, plan.kv_heads, plan.kept, dtype=torch.int32, device=plan.device)
-    with torch.cuda.device(plan.device):
-        _lib.check(_lib.load().sf_paged_evict(
-            code, ctypes.byref(pool), dst_table.data_ptr(),
-            dst_table.stride(0) if plan.sequences > 1 else dst_table.shape[1], dst_table.shape[1],
-            plan._lens.data_ptr(), plan.max_len, plan.max_keep, plan.sequences, plan.kv_heads,
-            k_pages.shape[3], plan.page_size, plan.sinks, plan.recent, kept.data_ptr(), plan.kept,
-            plan.err.data_ptr(), plan._stream()), "paged_evict")
+    kept = plan._lens.new_empty((plan.sequences, plan.kv_heads, plan.kept))
+    plan._call(_lib.load().sf_paged_evict, "paged_evict", code, ctypes.byref(pool), dst_table.data_ptr(),
+               dst_table.stride(0) if plan.sequences > 1 else dst_table.shape[1], dst_table.shape[1],
+               plan._lens.data_ptr(), plan.max_len, plan.max_keep, plan.sequences, plan.kv_heads,
+               k_pages.shape[3], plan.page_size, plan.sinks, plan.recent, kept.data_ptr(), plan.kept,
+               plan.err.data_ptr())
     return kept
