@@ -356,7 +356,7 @@ int sf_parent_map(const int64_t* ids, int B1, int N, int64_t* par_idx, void* str
  *
  * head_dim 64 or 128, H / Hkv <= 16, page_size a power of two in [16, 256].               */
 typedef struct sf_paged_list {       /* one kernel's share of a plan (offsets in words) */
-  int32_t items, n_items, first, workers, merges, n_merges, slots, rows, tile_tokens, max_rows;
+  int32_t items, n_items, heads, first, workers, merges, n_merges, slots, rows, tile_tokens, max_rows;
 } sf_paged_list;
 
 typedef struct sf_paged_plan {
@@ -369,7 +369,6 @@ typedef struct sf_paged_plan {
   sf_paged_list attn[2], mass;       /* [0]: few query rows per kv head, [1]: many */
   int64_t words;                     /* words of the plan */
   size_t ws_bytes;                   /* scratch of the calls below */
-  size_t ws_zero;                    /* its first bytes that must be zero before the first call */
   /* set by the caller before the first use */
   const int32_t* dev;                /* the plan's words in device memory */
   void* ws;                          /* ws_bytes of device memory */
@@ -380,9 +379,7 @@ typedef struct sf_paged_plan {
  * the mask alone, so one plan serves every layer of the step.  q_lens, kv_lens and words are
  * HOST arrays; words must hold sf_paged_plan_words(...) words (0: an argument is wrong, see
  * sf_last_error).  The caller copies plan->words words to device memory and sets dev, ws and
- * err; the first ws_zero bytes of ws must be zero (counters, which the calls leave at zero; after
- * a device error they may not be: zero them again).  Calls that share a plan share its scratch:
- * they must not overlap on the GPU. */
+ * err.  Calls that share a plan share its scratch: they must not overlap on the GPU. */
 int64_t sf_paged_plan_words(const sf_paged_plan* plan, const int32_t* q_lens,
                             const int32_t* kv_lens);
 int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_t* kv_lens,

@@ -47,7 +47,7 @@ class SfVerifyArgs(C.Structure):
 
 
 class SfPagedList(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("items", "n_items", "first", "workers", "merges", "n_merges",
+    _fields_ = [(n, C.c_int32) for n in ("items", "n_items", "heads", "first", "workers", "merges", "n_merges",
                                          "slots", "rows", "tile_tokens", "max_rows")]
 
 
@@ -55,7 +55,6 @@ class SfPagedPlan(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("dtype", "B", "H", "Hkv", "hd", "page_size", "block", "window",
                                          "sinks", "sms", "T", "max_kv", "short_chunk", "tokens")] + [
         ("attn", SfPagedList * 2), ("mass", SfPagedList), ("words", c_int64), ("ws_bytes", c_size_t),
-        ("ws_zero", c_size_t),
         ("dev", c_void_p), ("ws", c_void_p), ("err", c_void_p),
     ]
 

@@ -34,7 +34,6 @@ struct alignas(16) PagedItem {
   int32_t seq, kvh, tok0, ntok;       // the tile: tokens [tok0, tok0 + ntok) of the chunk
   int32_t i0, i1, slot, sink_blks;    // slot < 0: writes the output itself
   int32_t lo_blk, q0, q_len, kv_len;  // q0: the chunk's first row in q / out
-  int32_t cut, pad0, pad1, pad2;      // which cut tile this is a piece of
   __host__ __device__ int block(int i) const { return i < sink_blks ? i : i - sink_blks + lo_blk; }
 };
 // A tile whose run was cut into n pieces, in slots [slot0, slot0 + n)
@@ -144,11 +143,11 @@ struct PagedAttnParams {
   void* out;                        // [T, H, hd] contiguous
   float* lse;                       // [T, H]
   const PagedItem* items;
-  const int32_t* first;             // [workers + 1] first item of every CTA
+  const PagedItem* heads;           // [workers] a copy of every CTA's first item
+  const int32_t* first;             // [workers + 1] its index
   int workers;
   const PagedMerge* merges;
   int n_merges;
-  int32_t* arrived;                 // [n_merges] pieces of each cut tile that are done (zero between calls)
   float* part_O;                    // [slots][rows][hd]
   float* part_ml;                   // [slots][rows][2]
   int rows, tile_tokens;            // rows of a slot; tokens of 128 (64) rows
@@ -207,29 +206,48 @@ __device__ __forceinline__ int paged_page(const PagedPool& p, int seq, int idx, 
   return id;
 }
 
-// One warp joins the pieces of row r (row pr of the slots) of a cut tile, in their order.
+// One warp joins the pieces of row r (row pr of the slots) of a cut tile, in their order.  Lane x
+// fetches the state of piece x; the first pieces' values are on their way meanwhile.
 template <typename T, int HD>
 __device__ __forceinline__ void paged_join_row(const PagedAttnParams& p, const PagedMerge& w, int r, int pr, int lane) {
-  constexpr int E = HD / 32;
+  constexpr int E = HD / 32, AHEAD = 8;
+  const int64_t at0 = static_cast<int64_t>(w.slot0) * p.rows + pr;
+  float2 v[AHEAD][E / 2];
+  auto fetch = [&](int i, int j) {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e)
+      v[j][e] = i < w.n ? reinterpret_cast<const float2*>(p.part_O + (at0 + static_cast<int64_t>(i) * p.rows) * HD + lane * E)[e]
+                        : make_float2(0.f, 0.f);
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) fetch(j, j);
   float m = -INFINITY;
-  for (int i = lane; i < w.n; i += 32)
-    m = fmaxf(m, p.part_ml[2 * (static_cast<int64_t>(w.slot0 + i) * p.rows + pr)]);
+  for (int i = lane; i < w.n; i += 32) m = fmaxf(m, p.part_ml[2 * (at0 + static_cast<int64_t>(i) * p.rows)]);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < w.n; ++i) {
-    const int64_t at = static_cast<int64_t>(w.slot0 + i) * p.rows + pr;
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
-    const float f = exp2f(ml.x - ref);
-    l = fmaf(ml.y, f, l);
+  for (int i0 = 0; i0 < w.n; i0 += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (i0 + lane < w.n) ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (at0 + static_cast<int64_t>(i0 + lane) * p.rows));
+    const float f_lane = exp2f(ml.x - ref);
+    const int n = min(32, w.n - i0);
+    for (int j0 = 0; j0 < n; j0 += AHEAD) {
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(p.part_O + at * HD + lane * E + e);
-      o[e] = fmaf(v.x, f, o[e]);
-      o[e + 1] = fmaf(v.y, f, o[e + 1]);
+      for (int j = 0; j < AHEAD; ++j) {
+        const float f = __shfl_sync(0xffffffffu, f_lane, (j0 + j) & 31), lj = __shfl_sync(0xffffffffu, ml.y, (j0 + j) & 31);
+        if (j0 + j < n) {
+          l = fmaf(lj, f, l);
+#pragma unroll
+          for (int e = 0; e < E / 2; ++e) {
+            o[2 * e] = fmaf(v[j][e].x, f, o[2 * e]);
+            o[2 * e + 1] = fmaf(v[j][e].y, f, o[2 * e + 1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) fetch(i0 + j0 + AHEAD + j, j);
     }
   }
   const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + r / p.G) * p.H + w.kvh * p.G + r % p.G;

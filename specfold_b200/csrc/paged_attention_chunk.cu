@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* s_full = q_full + 16;                        // [2 tiles][2 halves]
   uint64_t* p_full = q_full + 20;
 
+  pdl_trigger();                                         // the join of cut tiles may line up
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
@@ -169,7 +170,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         w.q0 + w.tok0 + t * tq);
           ++qn[t];
         };
-        for (int i = w.i0; ok && i < w.i1; ++i)
+        KeyPages pages(p.pool, w, range, w.block(w.i0), KCH, lane, p.err);
+        for (int i = w.i0; ok && i < w.i1; ++i) {
+          const KeyPages now = pages;
+          if (i + 1 < w.i1) pages = KeyPages(p.pool, w, range, w.block(i + 1), KCH, lane, p.err);
           for (int kv = 0; ok && kv < 2; ++kv, ++u) {
             // the first block's order: tile 0's queries, K, tile 1's queries, V
             if (i == w.i0 && kv < tiles) load_q(kv);
@@ -177,9 +181,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const int s = u % NS;
             ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((u / NS) & 1) ^ 1, p.err, &abort_flag));
             if (!ok) break;
-            load_key_block<HD>(sm + L::ring + s * L::kTile, kv ? &tmV : &tmK, &full[s], p.pool, w, range, w.block(i),
-                               lane, p.err);
+            load_key_block(sm + L::ring + s * L::kTile, kv ? &tmV : &tmK, &full[s], now, w.kvh, lane);
           }
+        }
       }
       if (!ok && lane == 0) {                            // no load may be in flight at exit
         abort_flag = 1;

@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnParams p) {
   const PagedMerge w = p.merges[blockIdx.y];
+  pdl_wait();
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (r >= w.ntok * p.G) return;
   const int t = r / p.G, half = t / p.tile_tokens;
@@ -243,9 +244,19 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnParams p) {
 cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st) {
   if (p.n_merges == 0) return cudaSuccess;
   const dim3 grid((p.rows + 7) / 8, p.n_merges);
+  // lines up behind the pieces' kernel (which lets it) and waits for its end on the device
   auto go = [&](auto* kernel) {
-    kernel<<<grid, 256, 0, st>>>(p);
-    return launched();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    return e == cudaSuccess ? launched() : e;
   };
   if (dtype == BF16)
     return p.hd == 128 ? go(paged_merge_kernel<__nv_bfloat16, 128>) : go(paged_merge_kernel<__nv_bfloat16, 64>);

@@ -12,8 +12,7 @@
 // rate); the softmax would not, with all of a row's 128 exponentials in one thread.  So with at
 // most 32 (64) rows they are loaded 4 (2) times, copy c takes the keys [c, c + 1) * 128 / REP of
 // every block, its weights elsewhere stay zero, and each copy accumulates its own (m, l, O);
-// they are joined once per item.  The pieces of a tile that was cut between CTAs are joined by the
-// CTA that finishes last.
+// they are joined once per item.
 //
 // The rescaling of O waits until a row's maximum has grown by 2^8: until then the weights are
 // merely up to 2^8 instead of 1, relative to the same reference in l and O, and lose nothing.
@@ -71,6 +70,10 @@ __global__ void __launch_bounds__(kTokThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 10);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  pdl_trigger();                                         // the join of cut tiles may line up
+  // (on its way while the barriers are set up)
+  const PagedItem head = p.heads[blockIdx.x];
+  const int first = p.first[blockIdx.x], last = p.first[blockIdx.x + 1];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
@@ -102,14 +105,13 @@ __global__ void __launch_bounds__(kTokThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const uint32_t tO = tmem + 256, tP = tmem + 384;       // S buffers at columns 0 and 128
 
-  const int first = p.first[blockIdx.x], last = p.first[blockIdx.x + 1];
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
     uint32_t u = 0;                                      // ring units issued (K and V blocks)
     int qn = 0;                                          // query tiles issued
     bool ok = true;
     for (int it = first; ok && it < last; ++it) {
-      const PagedItem w = p.items[it];
+      const PagedItem w = it == first ? head : p.items[it];
       if (w.i0 == w.i1) continue;
       const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
       const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
@@ -122,14 +124,17 @@ __global__ void __launch_bounds__(kTokThreads, 1)
         tma_load_3d(sm + L::q + qb * L::kTile + (lane % KCH) * kPagedBox + (lane / KCH) * RC * 128, &tmQ,
                     &q_full[qb], (lane % KCH) * 64, w.kvh * p.G, w.q0 + w.tok0);
       ++qn;
-      for (int i = w.i0; ok && i < w.i1; ++i)
+      KeyPages pages(p.pool, w, range, w.block(w.i0), KCH, lane, p.err);
+      for (int i = w.i0; ok && i < w.i1; ++i) {
+        const KeyPages now = pages;
+        if (i + 1 < w.i1) pages = KeyPages(p.pool, w, range, w.block(i + 1), KCH, lane, p.err);
         for (int kv = 0; kv < 2; ++kv, ++u) {
           const int s = u % NS;
           ok = __all_sync(0xffffffffu, wait_or_abort(&empty[s], ((u / NS) & 1) ^ 1, p.err, abort_flag));
           if (!ok) break;
-          load_key_block<HD>(sm + L::ring + s * L::kTile, kv ? &tmV : &tmK, &full[s], p.pool, w, range,
-                             w.block(i), lane, p.err);
+          load_key_block(sm + L::ring + s * L::kTile, kv ? &tmV : &tmK, &full[s], now, w.kvh, lane);
         }
+      }
     }
     if (!ok) {                                           // no load may be in flight at exit
       if (lane == 0) {
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       };
       bool begin = false, waiting = false;               // the block before: begins an item; P V due
       for (int it = first; ok && it < last; ++it) {
-        const int i0 = p.items[it].i0, i1 = p.items[it].i1;
+        const int i0 = it == first ? head.i0 : p.items[it].i0, i1 = it == first ? head.i1 : p.items[it].i1;
         if (i0 == i1) continue;
         const int qb = qn & 1;
         ok = wait_or_abort(&q_full[qb], (qn >> 1) & 1, p.err, abort_flag);
@@ -218,7 +223,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
     uint32_t n = 0;                                      // key blocks done
     bool ok = true;
     for (int it = first; it < last; ++it) {
-      const PagedItem w = p.items[it];
+      const PagedItem w = it == first ? head : p.items[it];
       const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
       const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
       const int rows = w.ntok * p.G;
@@ -324,32 +329,42 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       }
       const int64_t slot_row = static_cast<int64_t>(w.slot) * p.rows;
       if (w.slot < 0) f *= L_row == 0.f ? 0.f : 1.f / L_row;
+      // Through shared memory, so that a warp writes rows and the copies meet: all columns at once
+      // where the rows are few, else 32 at a time.
+      const int turn = REP * rows * (HD + 1) <= 128 * kRedLd ? HD : 32, ld = turn + 1;
+      float* mine = red + (copy * rows + rr) * ld;
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
-        float o[32];
-        if (any && busy) {
-          tmem_ld32(tO + lane_off + c, o);
-          tmem_wait<32>(o);
-        }
+      for (int c0 = 0; c0 < HD; c0 += turn) {
+#pragma unroll 1
+        for (int c = c0; c < c0 + turn; c += 32) {
+          float o[32];
+          if (any && busy) {
+            tmem_ld32(tO + lane_off + c, o);
+            tmem_wait<32>(o);
+          }
+          if (valid)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) red[r * kRedLd + j] = any && f != 0.f ? o[j] * f : 0.f;
-        if (c + 32 == HD) {                              // O is read: the next item may begin
+            for (int j = 0; j < 32; ++j) mine[c - c0 + j] = any && f != 0.f ? o[j] * f : 0.f;
+          __syncwarp();
+        }
+        if (c0 + turn == HD) {                           // O is read: the next item may begin
           tc_fence_before();
           __syncwarp();
           if (any && lane == 0) mbar_arrive(o_free);
         }
         vote128(true);
         // 32 columns of a row per warp and turn, the copies added in their order
-        for (int row = quarter; row < rows; row += 4) {
-          float sum = red[row * kRedLd + lane];
+        for (int x = quarter; x < rows * (turn / 32); x += 4) {
+          const int row = x / (turn / 32), c = x % (turn / 32) * 32 + lane;
+          float sum = red[row * ld + c];
 #pragma unroll
-          for (int x = 1; x < REP; ++x) sum += red[(x * RC + row) * kRedLd + lane];
+          for (int y = 1; y < REP; ++y) sum += red[(y * rows + row) * ld + c];
           if (w.slot < 0) {
             const int64_t t = w.q0 + w.tok0 + row / p.G;
-            static_cast<__nv_bfloat16*>(p.out)[(t * p.H + w.kvh * p.G + row % p.G) * HD + c + lane] =
+            static_cast<__nv_bfloat16*>(p.out)[(t * p.H + w.kvh * p.G + row % p.G) * HD + c0 + c] =
                 __float2bfloat16_rn(sum);
           } else {
-            p.part_O[(slot_row + row) * HD + c + lane] = sum;
+            p.part_O[(slot_row + row) * HD + c0 + c] = sum;
           }
         }
         vote128(true);
@@ -365,30 +380,6 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       }
     }
     if (!ok) *abort_flag = 1;
-    // The piece of a cut tile that comes last joins them all, in their order: the result does not
-    // depend on which one that is.  A share is contiguous, so only its first and its last item can
-    // be such pieces.
-    if (vote128(ok) && last > first && (p.items[first].slot >= 0 || p.items[last - 1].slot >= 0)) {
-      __threadfence();
-      vote128(true);
-#pragma unroll 1
-      for (int it = first; it < last; it += max(1, last - 1 - first)) {
-        const PagedItem w = p.items[it];
-        if (w.slot < 0) continue;
-        const PagedMerge g = p.merges[w.cut];
-        if (threadIdx.x == 64) {
-          const bool all = atomicAdd(&p.arrived[w.cut], 1) == g.n - 1;
-          if (all) p.arrived[w.cut] = 0;                 // for the next call
-          s_m[0] = all ? 1.f : 0.f;
-        }
-        vote128(true);
-        if (s_m[0] != 0.f) {
-          __threadfence();
-          for (int row = quarter; row < w.ntok * p.G; row += 4) paged_join_row<__nv_bfloat16, HD>(p, g, row, row, lane);
-        }
-        vote128(true);
-      }
-    }
   }
   tc_fence_before();
   __syncthreads();

@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(kMassThreads, 1)
             const uint32_t s = kn % NS;
             ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[s], ((kn / NS) & 1) ^ 1, p.err, abort_flag));
             if (!ok) break;
-            load_key_block<HD>(sm + L::k + s * L::kTile, &tmK, &k_full[s], p.pool, w, range, kb, lane, p.err);
+            load_key_block(sm + L::k + s * L::kTile, &tmK, &k_full[s], KeyPages(p.pool, w, range, kb, KCH, lane, p.err),
+                           m.kvh, lane);
             ++kn;
           }
         const uint32_t s = qn % NS;

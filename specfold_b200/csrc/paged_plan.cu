@@ -94,7 +94,7 @@ int which(const Tiling& t, int q_len, int G) { return static_cast<int64_t>(q_len
 // A share of something that is cut into units [0, units): the piece [i0, i1), and where its
 // partial result goes (-1: it is whole)
 struct Piece {
-  int what, i0, i1, slot, cut;
+  int what, i0, i1, slot;
 };
 struct Cut {
   int what, slot0, n;
@@ -125,25 +125,20 @@ void deal(const std::vector<int>& units, int extra, int workers, std::vector<Pie
       int take = need;
       if (worker + 1 < w && need + extra > room)
         take = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(need, room - extra)));
-      pieces->push_back({static_cast<int>(x), at, at + take, -1, 0});
+      pieces->push_back({static_cast<int>(x), at, at + take, -1});
       at += take;
       done += take + (n == 0 ? extra : 0);
       ++n;
     } while (at < units[x]);
     if (n > 1) {
       cuts->push_back({static_cast<int>(x), *slots, n});
-      for (size_t i = from; i < pieces->size(); ++i) {
-        (*pieces)[i].slot = (*slots)++;
-        (*pieces)[i].cut = static_cast<int>(cuts->size()) - 1;
-      }
+      for (size_t i = from; i < pieces->size(); ++i) (*pieces)[i].slot = (*slots)++;
     }
   }
   while (static_cast<int64_t>(first->size()) <= w) first->push_back(static_cast<int32_t>(pieces->size()));
   first->back() = static_cast<int32_t>(pieces->size());
 }
 
-// the counters of the cut tiles come first: the zeroed part of the scratch
-size_t counter_bytes(int n) { return (static_cast<size_t>(n) * 4 + 255) / 256 * 256; }
 size_t list_ws(const sf_paged_list& l, int hd) {
   return (static_cast<size_t>(l.slots) * l.rows * (hd + 2) * 4 + 255) / 256 * 256;
 }
@@ -225,7 +220,7 @@ int64_t sf_paged_plan_words(const sf_paged_plan* plan, const int32_t* q_lens, co
   }
   const int64_t w = t.workers[0] + t.workers[1];
   const int64_t m = t.mass_workers;
-  const int64_t words = (items + w) * kItemWords + w * kMergeWords + 2 * (w + 16) + (mass + m) * kMassWords +
+  const int64_t words = (items + 2 * w) * kItemWords + w * kMergeWords + 2 * (w + 16) + (mass + m) * kMassWords +
                         m * kMassMergeWords + m + 16 + 2 * tokens + 64;
   if (words > kMaxWords) {
     bad("paged plan: the step is too large");
@@ -261,7 +256,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       if (q_lens[b] > kv_lens[b]) p.short_chunk = 1;
     }
     at = up4(at);
-    p.ws_bytes = p.ws_zero = 0;
+    p.ws_bytes = 0;
     for (int k = 0; k < 2; ++k) {
       std::vector<PagedItem> tiles;
       std::vector<int> units;
@@ -311,8 +306,13 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
         it.i0 = x.i0;
         it.i1 = x.i1;
         it.slot = x.slot;
-        it.cut = x.cut;
         memcpy(words + at, &it, sizeof(it));
+        at += kItemWords;
+      }
+      // (a CTA finds its first item without knowing its index)
+      l.heads = static_cast<int32_t>(at);
+      for (int x = 0; x < l.workers; ++x) {
+        memcpy(words + at, words + l.items + static_cast<int64_t>(std::min(first[x], l.n_items - 1)) * kItemWords, sizeof(PagedItem));
         at += kItemWords;
       }
       l.merges = static_cast<int32_t>(at);
@@ -326,7 +326,6 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       memcpy(words + at, first.data(), first.size() * 4);
       at = up4(at + static_cast<int64_t>(first.size()));
       p.ws_bytes += list_ws(l, p.hd);
-      if (k == 0) p.ws_zero = counter_bytes(l.n_merges);
     }
     // weight accumulation: pairs of key blocks, their unit a tile of tokens
     {
@@ -385,7 +384,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       l.first = static_cast<int32_t>(at);
       memcpy(words + at, first.data(), first.size() * 4);
       at = up4(at + static_cast<int64_t>(first.size()));
-      p.ws_bytes = p.ws_zero + std::max(p.ws_bytes, mass_ws(l));
+      p.ws_bytes = std::max(p.ws_bytes, mass_ws(l));
     }
     p.words = std::max<int64_t>(at, 4);
     p.dev = nullptr;
@@ -430,7 +429,7 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
   if (!out || !lse || !aligned16(out)) return bad("paged_attention: out and lse must be given, out 16-byte aligned");
   if (!(scale > 0.f) || scale > 3.0e38f) return bad("paged_attention: scale must be positive");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  size_t off = plan->ws_zero;
+  size_t off = 0;
   for (int k = 0; k < 2; ++k) {
     const sf_paged_list& l = plan->attn[k];
     if (l.n_items == 0) continue;
@@ -442,11 +441,11 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
     p.out = out;
     p.lse = lse;
     p.items = reinterpret_cast<const PagedItem*>(plan->dev + l.items);
+    p.heads = reinterpret_cast<const PagedItem*>(plan->dev + l.heads);
     p.first = plan->dev + l.first;
     p.workers = l.workers;
     p.merges = reinterpret_cast<const PagedMerge*>(plan->dev + l.merges);
     p.n_merges = l.n_merges;
-    p.arrived = static_cast<int32_t*>(plan->ws);
     p.part_O = reinterpret_cast<float*>(static_cast<char*>(plan->ws) + off);
     p.part_ml = p.part_O + static_cast<size_t>(l.slots) * l.rows * plan->hd;
     off += list_ws(l, plan->hd);
@@ -463,12 +462,9 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
     p.scale = scale;
     p.err = plan->err;
     cudaError_t e;
-    if (plan->dtype == SF_DTYPE_BF16 && k == 0) {       // joins its pieces itself
+    if (plan->dtype == SF_DTYPE_BF16 && k == 0)
       e = launch_paged_attention_tokens(p, l.max_rows <= 32 ? 4 : l.max_rows <= 64 ? 2 : 1, st);
-      if (e != cudaSuccess) return status(e, "paged_attention");
-      continue;
-    }
-    if (plan->dtype == SF_DTYPE_BF16)
+    else if (plan->dtype == SF_DTYPE_BF16)
       e = launch_paged_attention_chunk(p, st);
     else
       e = launch_paged_attention_simt(plan->dtype, p, st);
@@ -498,7 +494,7 @@ int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool
   p.workers = plan->mass.workers;
   p.merges = reinterpret_cast<const PagedMassMerge*>(plan->dev + plan->mass.merges);
   p.n_merges = plan->mass.n_merges;
-  p.part = reinterpret_cast<float*>(static_cast<char*>(plan->ws) + plan->ws_zero);
+  p.part = static_cast<float*>(plan->ws);
   p.H = plan->H;
   p.Hkv = plan->Hkv;
   p.G = plan->H / plan->Hkv;

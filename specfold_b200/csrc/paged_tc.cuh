@@ -123,27 +123,32 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, in
 
 constexpr int kPagedBox = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzled
 
-// One warp loads the 128 rows of key block kb: [hd / 64][128 rows][64], 128-byte swizzle, a box
-// per page (or half page) and 64 columns.  Pages that no row of the tile sees are not read.
-// Completes on `bar` (one arrival with the bytes).
-template <int HD>
-__device__ __forceinline__ void load_key_block(unsigned char* dst, const void* map, uint64_t* bar,
-                                               const PagedPool& pool, const PagedItem& w,
-                                               const PagedRange& range, int kb, int lane, int* err) {
-  constexpr int KCH = HD / 64;
-  const int ps = 1 << pool.page_shift;
-  const int br = ps < 128 ? ps : 128;                   // rows of a box
-  const int boxes = 128 / br;
-  // lane l fetches box l / KCH, column chunk l % KCH
-  const int x = lane / KCH, c = lane % KCH;
-  const int k0 = kb * kPagedKB + x * br;
-  const bool mine = x < boxes && range.meets(k0, k0 + br);
-  int page = 0;
-  if (mine) page = paged_page(pool, w.seq, k0 >> pool.page_shift, err);
+// What a lane of the loading warp fetches of a key block: box lane / chunks (a page, or half of a
+// large one), 64 columns lane % chunks.  Pages that no row of the tile sees are not read.
+struct KeyPages {
+  int page, row, at, rows;                               // page < 0: nothing; first row; place; rows of a box
+  __device__ __forceinline__ KeyPages(const PagedPool& pool, const PagedItem& w, const PagedRange& range, int kb,
+                                      int chunks, int lane, int* err) {
+    const int ps = 1 << pool.page_shift;
+    rows = ps < 128 ? ps : 128;
+    const int x = lane / chunks, k0 = kb * kPagedKB + x * rows;
+    at = x * rows;
+    row = k0 & (ps - 1);
+    page = -1;
+    if (x < 128 / rows && range.meets(k0, k0 + rows)) page = paged_page(pool, w.seq, k0 >> pool.page_shift, err);
+    at |= (lane % chunks) << 16;
+  }
+};
+// One warp loads the 128 rows of a key block: [hd / 64][128 rows][64], 128-byte swizzle.  Completes
+// on `bar` (one arrival with the bytes).
+__device__ __forceinline__ void load_key_block(unsigned char* dst, const void* map, uint64_t* bar, const KeyPages& k,
+                                               int kvh, int lane) {
+  const bool mine = k.page >= 0;
   const unsigned n = __popc(__ballot_sync(0xffffffffu, mine));
-  if (lane == 0) mbar_arrive_expect_tx(bar, n * br * 128);
+  if (lane == 0) mbar_arrive_expect_tx(bar, n * k.rows * 128);
   __syncwarp();
-  if (mine) tma_load_4d(dst + c * kPagedBox + x * br * 128, map, bar, c * 64, k0 & (ps - 1), w.kvh, page);
+  const int c = k.at >> 16, x = k.at & 0xffff;
+  if (mine) tma_load_4d(dst + c * kPagedBox + x * 128, map, bar, c * 64, k.row, kvh, k.page);
 }
 
 // ------------------------------------------------------------------ host side

@@ -382,7 +382,6 @@ class PagedPlan(_OnStream):
         self.heads, self.kv_heads, self.head_dim, self.page_size = heads, kv_heads, head_dim, page_size
         self._dev = words[:c.words].to(device)
         self._ws = torch.empty(max(c.ws_bytes, 256), dtype=torch.uint8, device=device)
-        self._ws[:c.ws_zero].zero_()
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
         c.dev, c.ws, c.err = self._dev.data_ptr(), self._ws.data_ptr(), self.err.data_ptr()
         self._f32 = self.err.view(torch.float32)

@@ -9,7 +9,7 @@ from specfold_b200 import _lib
 from specfold_b200 import kernels as K
 from tests import paged_reference as ref
 
-ITEM, MERGE, MASS, MASS_MERGE = 16, 8, 12, 8                      # words of the plan's records
+ITEM, MERGE, MASS, MASS_MERGE = 12, 8, 12, 8                      # words of the plan's records
 
 
 def build(q_lens, kv_lens, **kw):
@@ -56,14 +56,16 @@ def test_a_plan_covers_every_row_and_key_once(seed):
             continue
         first = w[part.first:part.first + part.workers + 1]
         assert first[0] == 0 and first[-1] == part.n_items and first == sorted(first)
+        for x, at in enumerate(first[:-1]):
+            if at < first[x + 1]:
+                assert w[part.heads + ITEM * x:][:ITEM] == w[part.items + ITEM * at:][:ITEM]
+            # only a share's first and last item can be pieces of a cut tile
+            assert all(w[part.items + ITEM * i + 6] < 0 for i in range(at + 1, first[x + 1] - 1))
         tiles, used = {}, []
         for x in range(part.n_items):
-            seq, kvh, t0, nt, i0, i1, slot, sink, lo, q0, ql, kv, cut = w[part.items + ITEM * x:][:13]
+            seq, kvh, t0, nt, i0, i1, slot, sink, lo, q0, ql, kv = w[part.items + ITEM * x:][:ITEM]
             assert (ql, kv, q0) == (q[seq], n[seq], sum(q[:seq])) and 0 < nt * G <= part.rows
             tiles.setdefault((seq, kvh, t0, nt), []).append((i0, i1, slot, sink, lo))
-            if slot >= 0:
-                merge = w[part.merges + MERGE * cut:][:MERGE]
-                assert merge[:3] == [kvh, t0, nt] and merge[3] <= slot < merge[3] + merge[4] and merge[5] == q0
         for (seq, kvh, t0, nt), pieces in tiles.items():
             at = 0
             for i0, i1, slot, _, _ in pieces:
