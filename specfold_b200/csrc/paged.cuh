@@ -285,7 +285,7 @@ struct PagedEvictParams {
   const int32_t* lens;              // [B][2]: cached keys, keys that stay
   int32_t* kept;                    // [B][Hkv][kept_stride]
   int kept_stride;
-  int B, Hkv, hd, sinks, recent, max_len, max_keep;
+  int B, Hkv, hd, sinks, recent, max_len, max_keep, sms;
   int* err;
 };
 cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_t st);

@@ -1,4 +1,6 @@
 // Paged prefix cache: the append of new rows and the eviction by accumulated weight.
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
 
 namespace sf {
@@ -54,30 +56,34 @@ cudaError_t launch_paged_append(int dtype, const PagedAppendParams& p, cudaStrea
 // Which keys stay.  Of n cached keys the first `sinks` and the last `recent` stay; of the rest
 // the m = keep - sinks - recent largest weights, equal ones by position.  A radix select over
 // the weights' order-preserving bits (11, 11 and 10 of them) finds the m-th largest value and
-// how many of its equals are taken; one scan over the positions then writes the list in order.
-// One CTA per (sequence, kv head).
+// how many of its equals are taken; a count over the positions then places every survivor.
+//
+// A cluster of 1 to 8 CTAs works on one (sequence, kv head), a contiguous range of positions
+// each: the weights are read once and stay in registers (kSelKeys a thread; what is beyond is
+// read again), every pass adds up the CTAs' histograms through distributed shared memory.
 constexpr int kSelThreads = 1024;
+constexpr int kSelKeys = 8;
 
 __device__ __forceinline__ uint32_t order_bits(float f) {
   const uint32_t u = __float_as_uint(f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// inclusive sum over the block of a 64-bit pair of counts
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* s_warp) {
+// inclusive sum over the block
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += u;
   }
   if (lane == 31) s_warp[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    uint64_t w = s_warp[lane];
+    uint32_t w = s_warp[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xffffffffu, w, o);
+      const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += u;
     }
     s_warp[lane] = w;
@@ -87,76 +93,194 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* s_warp) {
 }
 
 __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedEvictParams p) {
-  __shared__ uint32_t hist[2048];
-  __shared__ uint64_t s_warp[32];
-  __shared__ uint32_t s_bin, s_above;
-  const int h = blockIdx.x, b = blockIdx.y;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ uint32_t hist[2][2048];                     // of this pass and the next: two by turns
+  __shared__ uint32_t s_warp[32];
+  __shared__ uint32_t s_above[kSelKeys][32], s_equal[kSelKeys][32];
+  __shared__ uint32_t s_total[2];                        // of this CTA: above, equal
+  __shared__ uint32_t s_bin, s_before;
+  const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = p.lens[2 * b], keep = p.lens[2 * b + 1];
   int32_t* out = p.kept + (static_cast<int64_t>(b) * p.Hkv + h) * p.kept_stride;
-  for (int i = min(n, keep) + threadIdx.x; i < p.kept_stride; i += kSelThreads) out[i] = -1;
-  if (n <= keep) {
-    for (int i = threadIdx.x; i < n; i += kSelThreads) out[i] = i;
+  const int tid = rank * kSelThreads + threadIdx.x, all = C * kSelThreads;
+  pdl_trigger();                                         // the move may line up
+  for (int i = min(n, keep) + tid; i < p.kept_stride; i += all) out[i] = -1;
+  if (n <= keep) {                                       // (the whole cluster)
+    for (int i = tid; i < n; i += all) out[i] = i;
     return;
   }
   const int lo = p.sinks, hi = n - p.recent;            // the middle
   const int want = keep - p.sinks - p.recent;
-  auto key_of = [&](int pos) {
-    const int page = paged_page(p.pool, b, pos >> p.pool.page_shift, p.err);
-    return order_bits(p.pool.mass[mass_at(p.pool, page, p.Hkv, h, pos)]);
-  };
-  // the want-th largest: its bits from the top, `left` of the keys that share them still wanted
-  uint32_t prefix = 0, mask = 0;
-  int left = want;
-  const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-  if (want > 0) {
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      for (int i = threadIdx.x; i < 2048; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      const uint32_t field = (1u << bits[pass]) - 1;
-      for (int i = lo + threadIdx.x; i < hi; i += kSelThreads) {
-        const uint32_t k = key_of(i);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shifts[pass]) & field], 1u);
-      }
-      __syncthreads();
-      // thread t owns bins 2047 - 2t and 2046 - 2t: a scan from the largest bin down
-      const uint32_t c0 = hist[2047 - 2 * threadIdx.x], c1 = hist[2046 - 2 * threadIdx.x];
-      const uint64_t inc = block_scan(c0 + c1, s_warp);
-      const uint32_t before = static_cast<uint32_t>(inc) - c0 - c1;
-      const uint32_t l = static_cast<uint32_t>(left);
-      if (before < l && before + c0 >= l) {
-        s_bin = 2047 - 2 * threadIdx.x;
-        s_above = before;
-      } else if (before + c0 < l && before + c0 + c1 >= l) {
-        s_bin = 2046 - 2 * threadIdx.x;
-        s_above = before + c0;
-      }
-      __syncthreads();
-      prefix |= s_bin << shifts[pass];
-      mask |= field << shifts[pass];
-      left -= static_cast<int>(s_above);
-      __syncthreads();
-    }
-  }
-  for (int i = threadIdx.x; i < p.sinks; i += kSelThreads) out[i] = i;
-  for (int i = threadIdx.x; i < p.recent; i += kSelThreads) out[keep - p.recent + i] = hi + i;
+  for (int i = tid; i < p.sinks; i += all) out[i] = i;
+  for (int i = tid; i < p.recent; i += all) out[keep - p.recent + i] = hi + i;
   if (want == 0) return;
-  // positions in order: larger than the threshold, or one of the first `left` equal to it
-  uint32_t above = 0, equal = 0;
-  for (int i0 = lo; i0 < hi; i0 += kSelThreads) {
-    const int i = i0 + threadIdx.x;
-    const uint32_t k = i < hi ? key_of(i) : 0;
-    const bool gt = i < hi && k > prefix, eq = i < hi && k == prefix;
-    const uint64_t inc = block_scan((static_cast<uint64_t>(gt) << 32) | eq, s_warp);
-    const uint32_t g = above + static_cast<uint32_t>(inc >> 32) - gt;
-    const uint32_t q = equal + static_cast<uint32_t>(inc) - eq;
-    if (gt || (eq && q < static_cast<uint32_t>(left)))
-      out[p.sinks + g + min(q, static_cast<uint32_t>(left))] = i;
-    const uint64_t all = s_warp[31];
-    above += static_cast<uint32_t>(all >> 32);
-    equal += static_cast<uint32_t>(all);
+  // this CTA's positions [begin, end), kSelThreads side by side
+  const int span = (hi - lo + C - 1) / C;
+  const int begin = min(hi, lo + rank * span), end = min(hi, begin + span);
+  const int turns = (span + kSelThreads - 1) / kSelThreads;
+  auto read = [&](int i) {
+    const int page = paged_page(p.pool, b, i >> p.pool.page_shift, p.err);
+    return order_bits(p.pool.mass[mass_at(p.pool, page, p.Hkv, h, i)]);
+  };
+  uint32_t held[kSelKeys];
+#pragma unroll
+  for (int j = 0; j < kSelKeys; ++j) {
+    const int i = begin + j * kSelThreads + threadIdx.x;
+    held[j] = i < end ? read(i) : 0;
+  }
+  for (int i = threadIdx.x; i < 2 * 2048; i += kSelThreads) hist[0][i] = 0;
+  __syncthreads();
+  // the want-th largest: its bits from the top, `left` of the keys that share them still wanted
+  uint32_t prefix = 0, mask = 0, left = want;
+  const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    uint32_t* mine = hist[pass & 1];
+    const uint32_t field = (1u << bits[pass]) - 1;
+    // equal bins of a warp are counted together: a heavy tail has few leading bits
+    auto count = [&](uint32_t k, bool live) {
+      live = live && (k & mask) == prefix;
+      const unsigned who = __ballot_sync(0xffffffffu, live);
+      if (!live) return;
+      const uint32_t bin = (k >> shifts[pass]) & field;
+      const unsigned same = __match_any_sync(who, bin);
+      if (lane == __ffs(same) - 1) atomicAdd(&mine[bin], __popc(same));
+    };
+#pragma unroll
+    for (int j = 0; j < kSelKeys; ++j)
+      if (j < turns) {
+        count(held[j], begin + j * kSelThreads + threadIdx.x < end);
+        __syncwarp();
+      }
+    for (int j = kSelKeys; j < turns; ++j) {
+      const int i = begin + j * kSelThreads + threadIdx.x;
+      count(i < end ? read(i) : 0, i < end);
+      __syncwarp();
+    }
+    cluster.sync();                                      // every CTA's counts are there
+    // thread t owns bins 2047 - 2t and 2046 - 2t: a scan from the largest bin down
+    uint32_t c0 = 0, c1 = 0;
+    for (int c = 0; c < C; ++c) {
+      const uint2 x = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(mine, c) + 2046 - 2 * threadIdx.x);
+      c0 += x.y;
+      c1 += x.x;
+    }
+    const uint32_t before = block_scan(c0 + c1, s_warp) - c0 - c1;
+    if (before < left && before + c0 >= left) {
+      s_bin = 2047 - 2 * threadIdx.x;
+      s_before = before;
+    } else if (before + c0 < left && before + c0 + c1 >= left) {
+      s_bin = 2046 - 2 * threadIdx.x;
+      s_before = before + c0;
+    }
+    if (pass == 0) {                                     // the buffer of pass 2
+      cluster.sync();                                    // (nobody reads it any more)
+      for (int i = threadIdx.x; i < 2048; i += kSelThreads) mine[i] = 0;
+    }
+    __syncthreads();
+    prefix |= s_bin << shifts[pass];
+    mask |= field << shifts[pass];
+    left -= s_before;
     __syncthreads();
   }
+  // Positions in order: larger than the threshold, or one of the first `left` equal to it.  Counts
+  // per warp and turn, their sums over what comes before, then each survivor's place.
+  uint32_t above = 0, equal = 0;                         // in the turns before
+#pragma unroll 1
+  for (int j0 = 0; j0 < turns; j0 += kSelKeys) {
+    const int m = min(kSelKeys, turns - j0);
+    if (j0 > 0)
+#pragma unroll
+      for (int j = 0; j < kSelKeys; ++j) {
+        const int i = begin + (j0 + j) * kSelThreads + threadIdx.x;
+        held[j] = i < end ? read(i) : 0;
+      }
+    unsigned gt[kSelKeys], eq[kSelKeys];
+#pragma unroll
+    for (int j = 0; j < kSelKeys; ++j) {
+      const bool live = begin + (j0 + j) * kSelThreads + static_cast<int>(threadIdx.x) < end;
+      gt[j] = __ballot_sync(0xffffffffu, live && held[j] > prefix);
+      eq[j] = __ballot_sync(0xffffffffu, live && held[j] == prefix);
+      if (lane == 0) {
+        s_above[j][warp] = __popc(gt[j]);
+        s_equal[j][warp] = __popc(eq[j]);
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {                                     // sums over (turn, warp) in order
+      uint32_t run_a = above, run_e = equal;
+      for (int j = 0; j < m; ++j) {
+        const uint32_t a = s_above[j][lane], e = s_equal[j][lane];
+        uint32_t ia = a, ie = e;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t ua = __shfl_up_sync(0xffffffffu, ia, o), ue = __shfl_up_sync(0xffffffffu, ie, o);
+          if (lane >= o) {
+            ia += ua;
+            ie += ue;
+          }
+        }
+        s_above[j][lane] = run_a + ia - a;
+        s_equal[j][lane] = run_e + ie - e;
+        run_a += __shfl_sync(0xffffffffu, ia, 31);
+        run_e += __shfl_sync(0xffffffffu, ie, 31);
+      }
+      if (lane == 0) {
+        s_total[0] = run_a;
+        s_total[1] = run_e;
+      }
+    }
+    __syncthreads();
+    above = s_total[0];
+    equal = s_total[1];
+    // (the CTAs before this one: their totals are known once all have counted, which takes their
+    // last turn; what exceeds the registers is counted first and placed in a second walk)
+    if (turns > kSelKeys) continue;
+    cluster.sync();
+    uint32_t base_a = 0, base_e = 0;
+    for (int c = 0; c < rank; ++c) {
+      const uint32_t* t = cluster.map_shared_rank(s_total, c);
+      base_a += t[0];
+      base_e += t[1];
+    }
+#pragma unroll
+    for (int j = 0; j < kSelKeys; ++j) {
+      const unsigned below = (1u << lane) - 1;
+      const uint32_t g = base_a + s_above[j][warp] + __popc(gt[j] & below);
+      const uint32_t q = base_e + s_equal[j][warp] + __popc(eq[j] & below);
+      if ((gt[j] >> lane & 1) || ((eq[j] >> lane & 1) && q < left))
+        out[p.sinks + g + min(q, left)] = begin + j * kSelThreads + threadIdx.x;
+    }
+  }
+  if (turns > kSelKeys) {
+    cluster.sync();
+    uint32_t base_a = 0, base_e = 0;
+    for (int c = 0; c < rank; ++c) {
+      const uint32_t* t = cluster.map_shared_rank(s_total, c);
+      base_a += t[0];
+      base_e += t[1];
+    }
+#pragma unroll 1
+    for (int j = 0; j < turns; ++j) {
+      const int i = begin + j * kSelThreads + threadIdx.x;
+      const uint32_t k = i < end ? read(i) : 0;
+      const bool g = i < end && k > prefix, e = i < end && k == prefix;
+      const uint32_t ia = block_scan(g, s_warp);
+      const uint32_t ta = s_warp[31];
+      __syncthreads();
+      const uint32_t ie = block_scan(e, s_warp);
+      const uint32_t te = s_warp[31];
+      __syncthreads();
+      const uint32_t q = base_e + ie - e;
+      if (g || (e && q < left)) out[p.sinks + base_a + ia - g + min(q, left)] = i;
+      base_a += ta;
+      base_e += te;
+    }
+  }
+  cluster.sync();                                        // shared memory is read until here
 }
 
 // The survivors' rows to their new pages: a thread per 16-byte vector, kCopyRows keys in
@@ -175,6 +299,7 @@ __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvictParams p) {
   const int32_t* kept = p.kept + static_cast<int64_t>(bh) * p.kept_stride;
   const int base = blockIdx.x * per * kCopyRows + k0;
   if (base >= stay) return;
+  pdl_wait();
   T* pages = static_cast<T*>(const_cast<void*>(value ? p.pool.v : p.pool.k));
   uint4 d[kCopyRows];
   float a[kCopyRows];
@@ -203,18 +328,32 @@ __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvictParams p) {
 
 cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_t st) {
   if (p.B == 0) return cudaSuccess;
-  paged_select_kernel<<<dim3(p.Hkv, p.B), kSelThreads, 0, st>>>(p);
-  cudaError_t e = launched();
-  if (e != cudaSuccess) return e;
+  // CTAs of a cluster: at most 4 keys a thread, while the GPU has SMs to spare
   const int stay = p.max_len < p.max_keep ? p.max_len : p.max_keep;
-  if (stay == 0) return cudaSuccess;
+  int C = 1;
+  while (C < 8 && p.max_len > C * 4 * kSelThreads && C * p.B * p.Hkv < p.sms) C *= 2;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, p.Hkv, p.B);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_select_kernel, p);
+  if (e == cudaSuccess) e = launched();
+  if (e != cudaSuccess || stay == 0) return e;
   const int per = 256 / (2 * (p.hd / (dtype == BF16 ? 8 : 4))) * kCopyRows;
   const dim3 grid((stay + per - 1) / per, p.B * p.Hkv);
-  if (dtype == BF16)
-    paged_move_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  else
-    paged_move_kernel<float><<<grid, 256, 0, st>>>(p);
-  return launched();
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  e = dtype == BF16 ? cudaLaunchKernelEx(&cfg, paged_move_kernel<__nv_bfloat16>, p)
+                    : cudaLaunchKernelEx(&cfg, paged_move_kernel<float>, p);
+  return e == cudaSuccess ? launched() : e;
 }
 
 }  // namespace sf

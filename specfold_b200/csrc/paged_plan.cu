@@ -518,7 +518,7 @@ int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_tabl
   if (hd != 64 && hd != 128) return bad("paged_evict: head_dim %d must be 64 or 128", hd);
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
     return bad("paged_evict: page size %d must be a power of two in [16, 256]", page_size);
-  if (B < 0 || Hkv < 1 || static_cast<int64_t>(B) * Hkv > 65535) return bad("paged_evict: %d sequences of %d heads", B, Hkv);
+  if (B < 0 || Hkv < 1 || B > 65535 || static_cast<int64_t>(B) * Hkv > 65535) return bad("paged_evict: %d sequences of %d heads", B, Hkv);
   if (sinks < 0 || recent < 0 || max_len < 0 || max_keep < 0 || static_cast<int64_t>(sinks) + recent > max_keep)
     return bad("paged_evict: sinks %d + recent %d do not fit the %d keys that stay", sinks, recent, max_keep);
   if (B == 0) return SF_OK;
@@ -545,6 +545,7 @@ int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_tabl
   p.recent = recent;
   p.max_len = max_len;
   p.max_keep = max_keep;
+  p.sms = device_sms(0);
   p.err = err;
   return status(launch_paged_evict(dtype, p, static_cast<cudaStream_t>(stream)), "paged_evict");
 }
