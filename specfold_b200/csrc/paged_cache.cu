@@ -15,41 +15,41 @@ __device__ __forceinline__ int64_t mass_at(const PagedPool& p, int page, int Hkv
 
 // ------------------------------------------------------------------ append
 // One thread per 16-byte vector of a new row (key vectors, then value vectors): a row is read
-// once, coalesced, from wherever the projection left it and written once.
-template <typename T>
+// once, coalesced, from wherever the projection left it, while {sequence, position} and then the
+// page are looked up, and written once.  (Several vectors a thread were slower: 36 to 43 us
+// against 29 for 14000 rows of 8 heads.)  VPR: vectors of a row.
+template <typename T, int VPR>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedAppendParams p) {
   constexpr int V = Elt<T>::kVec;
-  const int vpr = p.hd / V;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t rows = static_cast<int64_t>(p.T) * p.Hkv;
-  const int e = static_cast<int>(i % vpr) * V;
-  const bool value = (i / vpr) & 1;
-  const int64_t row = i / (2 * vpr);
-  if (row >= rows) return;
-  const int t = static_cast<int>(row / p.Hkv), h = static_cast<int>(row % p.Hkv);
+  const unsigned row = blockIdx.x * (256 / (2 * VPR)) + threadIdx.x / (2 * VPR);
+  const unsigned t = row / p.Hkv, h = row % p.Hkv;
+  if (t >= static_cast<unsigned>(p.T)) return;
+  const int e = threadIdx.x % VPR * V;
+  const bool value = threadIdx.x / VPR & 1;
   const int2 at = reinterpret_cast<const int2*>(p.tokens)[t];
+  const T* src = static_cast<const T*>(value ? p.v_new : p.k_new) + t * p.new_tok + h * p.new_head + e;
+  const uint4 d = __ldcs(reinterpret_cast<const uint4*>(src));
   const int id = p.pool.table[at.x * p.pool.table_stride + (at.y >> p.pool.page_shift)];
   if (id < 0 || id >= p.pool.num_pages) {               // nowhere to write: flagged, left out
     flag_error(p.err, SF_DEV_ERR_INDEX);
     return;
   }
-  const T* src = static_cast<const T*>(value ? p.v_new : p.k_new) + t * p.new_tok + h * p.new_head + e;
   T* dst = static_cast<T*>(const_cast<void*>(value ? p.pool.v : p.pool.k)) + pool_row(p.pool, id, h, at.y) + e;
-  *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-  if (!value && e == 0 && p.pool.mass != nullptr)
-    p.pool.mass[mass_at(p.pool, id, p.Hkv, h, at.y)] = 0.f;
+  *reinterpret_cast<uint4*>(dst) = d;
+  if (!value && e == 0 && p.pool.mass != nullptr) p.pool.mass[mass_at(p.pool, id, p.Hkv, h, at.y)] = 0.f;
+}
+
+template <typename T, int VPR>
+static cudaError_t append_rows(const PagedAppendParams& p, cudaStream_t st) {
+  const int64_t threads = static_cast<int64_t>(p.T) * p.Hkv * 2 * VPR;   // T * Hkv < 2^31
+  paged_append_kernel<T, VPR><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, st>>>(p);
+  return launched();
 }
 
 cudaError_t launch_paged_append(int dtype, const PagedAppendParams& p, cudaStream_t st) {
   if (p.T == 0) return cudaSuccess;
-  const int vpr = p.hd / (dtype == BF16 ? 8 : 4);
-  const int64_t n = static_cast<int64_t>(p.T) * p.Hkv * 2 * vpr;
-  const int64_t blocks = (n + 255) / 256;
-  if (dtype == BF16)
-    paged_append_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p);
-  else
-    paged_append_kernel<float><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p);
-  return launched();
+  if (dtype == BF16) return p.hd == 128 ? append_rows<__nv_bfloat16, 16>(p, st) : append_rows<__nv_bfloat16, 8>(p, st);
+  return p.hd == 128 ? append_rows<float, 32>(p, st) : append_rows<float, 16>(p, st);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -283,55 +283,62 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedEvictPar
   cluster.sync();                                        // shared memory is read until here
 }
 
-// The survivors' rows to their new pages: a thread per 16-byte vector, kCopyRows keys in
-// flight each (key and value vectors of one key side by side, so a warp moves whole rows).
-constexpr int kCopyRows = 4;
+// The survivors' rows to their new pages.  A CTA takes kMoveKeys of one (sequence, kv head): first
+// a thread per key finds both rows (survivor, page, destination page: three loads one after the
+// other, paid once for 32 KB of bf16) and moves its weight, then all threads copy 16-byte vectors, a
+// key's key and value rows side by side, kMoveVecs of them in flight.
+constexpr int kMoveKeys = 64;
+constexpr int kMoveVecs = 4;
 
-template <typename T>
+template <typename T, int vpr>                          // vectors of a row
 __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvictParams p) {
   constexpr int V = Elt<T>::kVec;
-  const int vpr = p.hd / V, per = 256 / (2 * vpr);      // keys side by side in the CTA
+  constexpr int vpk = 2 * vpr;                          // vectors of a key
+  __shared__ int64_t s_src[kMoveKeys], s_dst[kMoveKeys];
   const int bh = blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
   const int stay = min(p.lens[2 * b], p.lens[2 * b + 1]);
-  const int x = threadIdx.x % (2 * vpr), k0 = threadIdx.x / (2 * vpr);
-  const bool value = x >= vpr;
-  const int e = (x % vpr) * V;
-  const int32_t* kept = p.kept + static_cast<int64_t>(bh) * p.kept_stride;
-  const int base = blockIdx.x * per * kCopyRows + k0;
-  if (base >= stay) return;
+  const int base = blockIdx.x * kMoveKeys, keys = min(kMoveKeys, stay - base);
+  if (keys <= 0) return;
   pdl_wait();
-  T* pages = static_cast<T*>(const_cast<void*>(value ? p.pool.v : p.pool.k));
-  uint4 d[kCopyRows];
-  float a[kCopyRows];
-#pragma unroll
-  for (int r = 0; r < kCopyRows; ++r) {
-    const int i = base + r * per;
-    if (i >= stay) continue;
-    const int pos = kept[i];
+  if (static_cast<int>(threadIdx.x) < keys) {
+    const int i = base + threadIdx.x, pos = p.kept[static_cast<int64_t>(bh) * p.kept_stride + i];
     const int page = paged_page(p.pool, b, pos >> p.pool.page_shift, p.err);
-    d[r] = *reinterpret_cast<const uint4*>(pages + pool_row(p.pool, page, h, pos) + e);
-    if (x == 0) a[r] = p.pool.mass[mass_at(p.pool, page, p.Hkv, h, pos)];
-  }
-#pragma unroll
-  for (int r = 0; r < kCopyRows; ++r) {
-    const int i = base + r * per;
-    if (i >= stay) continue;
     const int id = p.dst[b * p.dst_stride + (i >> p.pool.page_shift)];
-    if (id < 0 || id >= p.pool.num_pages) {
+    s_src[threadIdx.x] = pool_row(p.pool, page, h, pos);
+    if (id < 0 || id >= p.pool.num_pages) {             // flagged, left out
       flag_error(p.err, SF_DEV_ERR_INDEX);
-      continue;
+      s_dst[threadIdx.x] = -1;
+    } else {
+      s_dst[threadIdx.x] = pool_row(p.pool, id, h, i);
+      p.pool.mass[mass_at(p.pool, id, p.Hkv, h, i)] = p.pool.mass[mass_at(p.pool, page, p.Hkv, h, pos)];
     }
-    *reinterpret_cast<uint4*>(pages + pool_row(p.pool, id, h, i) + e) = d[r];
-    if (x == 0) p.pool.mass[mass_at(p.pool, id, p.Hkv, h, i)] = a[r];
+  }
+  __syncthreads();
+  T* const k = static_cast<T*>(const_cast<void*>(p.pool.k));
+  T* const v = static_cast<T*>(const_cast<void*>(p.pool.v));
+  for (int x0 = threadIdx.x; x0 < keys * vpk; x0 += 256 * kMoveVecs) {
+    uint4 d[kMoveVecs];
+#pragma unroll
+    for (int y = 0; y < kMoveVecs; ++y) {
+      const int x = x0 + y * 256;
+      if (x < keys * vpk) d[y] = __ldcs(reinterpret_cast<const uint4*>(((x / vpr) & 1 ? v : k) + s_src[x / vpk] + x % vpr * V));
+    }
+#pragma unroll
+    for (int y = 0; y < kMoveVecs; ++y) {
+      const int x = x0 + y * 256;
+      if (x < keys * vpk && s_dst[x / vpk] >= 0)
+        *reinterpret_cast<uint4*>(((x / vpr) & 1 ? v : k) + s_dst[x / vpk] + x % vpr * V) = d[y];
+    }
   }
 }
 
 cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_t st) {
   if (p.B == 0) return cudaSuccess;
-  // CTAs of a cluster: at most 4 keys a thread, while the GPU has SMs to spare
+  // CTAs of a cluster: at most 2 keys a thread, as long as all clusters run side by side (a CTA
+  // fills an SM: for 96 heads of 8200 keys the selection took 25 us with two CTAs each, 21 with one)
   const int stay = p.max_len < p.max_keep ? p.max_len : p.max_keep;
   int C = 1;
-  while (C < 8 && p.max_len > C * 4 * kSelThreads && C * p.B * p.Hkv < p.sms) C *= 2;
+  while (C < 8 && p.max_len > C * 2 * kSelThreads && 2 * C * p.B * p.Hkv <= p.sms) C *= 2;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = C;
@@ -345,14 +352,17 @@ cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_
   cudaError_t e = cudaLaunchKernelEx(&cfg, paged_select_kernel, p);
   if (e == cudaSuccess) e = launched();
   if (e != cudaSuccess || stay == 0) return e;
-  const int per = 256 / (2 * (p.hd / (dtype == BF16 ? 8 : 4))) * kCopyRows;
-  const dim3 grid((stay + per - 1) / per, p.B * p.Hkv);
+  const dim3 grid((stay + kMoveKeys - 1) / kMoveKeys, p.B * p.Hkv);
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = grid;
   cfg.blockDim = dim3(256);
-  e = dtype == BF16 ? cudaLaunchKernelEx(&cfg, paged_move_kernel<__nv_bfloat16>, p)
-                    : cudaLaunchKernelEx(&cfg, paged_move_kernel<float>, p);
+  if (dtype == BF16)
+    e = p.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_move_kernel<__nv_bfloat16, 16>, p)
+                    : cudaLaunchKernelEx(&cfg, paged_move_kernel<__nv_bfloat16, 8>, p);
+  else
+    e = p.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_move_kernel<float, 32>, p)
+                    : cudaLaunchKernelEx(&cfg, paged_move_kernel<float, 16>, p);
   return e == cudaSuccess ? launched() : e;
 }
 
