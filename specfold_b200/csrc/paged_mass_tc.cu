@@ -7,7 +7,10 @@
 // order, and written once; no atomics.  lse is a per-column constant: the exponent is one fma.
 // A CTA works on two key blocks at a time, so that a query tile, which streams from L2, feeds two
 // products.  A pair whose tiles were cut between CTAs leaves its sums for the merge.
-//   warps 4-7, 8-11   exponentials and sums of the first and of the second block
+//   warps 4-11, 12-19 exponentials and sums of the first and of the second block, two threads per
+//                     key: rows 0-63 and 64-127 of a tile.  Two warps on each scheduler for either
+//                     block hide each other's waits for TMEM and for the special-function unit: with
+//                     one thread per key the largest case took 292 us, with two 236
 //   warp 0            TMA: key blocks and query tiles, through rings of their own
 //   warp 1            tcgen05.mma, two S^T buffers of 128 columns for each block (all of TMEM)
 //   warp 2            lse of the tile's rows into shared memory
@@ -17,7 +20,7 @@
 
 namespace sf {
 
-constexpr int kMassThreads = 384;
+constexpr int kMassThreads = 640;
 
 template <int HD>
 struct MassSmem {
@@ -27,7 +30,8 @@ struct MassSmem {
   static constexpr int k = 0;                            // [kStages][kTile]
   static constexpr int q = k + kStages * kTile;          // [kStages][kTile]
   static constexpr int lse = q + kStages * kTile;        // [kRows][128] floats
-  static constexpr int bars = lse + kRows * 512;
+  static constexpr int half = lse + kRows * 512;         // [2 blocks][2][128] sums of rows 64-127
+  static constexpr int bars = half + 4 * 512;
   static constexpr int bytes = bars + 256 + 1024;        // + alignment of the base
 };
 
@@ -75,11 +79,11 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     }
     for (int s = 0; s < NR; ++s) {
       mbar_init(&r_full[s], 1);
-      mbar_init(&r_empty[s], 8);
+      mbar_init(&r_empty[s], 16);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&s_empty[s], 4);
+      mbar_init(&s_empty[s], 8);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     if (!ok) *abort_flag = 1;
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- exponentials and sums
-    const int y = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int y = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t tS = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + y * 256;
     const float* s_lse = reinterpret_cast<const float*>(sm + L::lse);
     const float sl2 = p.scale * 1.4426950408889634f;
@@ -258,8 +262,9 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     };
     Ahead cur = begin(first < last ? first : 0);
     float* dst = target(cur);
-    float old = dst != nullptr && cur.m.slot < 0 ? *dst : 0.f;
-    for (int it = first; ok && it < last; ++it) {
+    float old = half == 0 && dst != nullptr && cur.m.slot < 0 ? *dst : 0.f;
+    float* s_half = reinterpret_cast<float*>(sm + L::half) + y * 256;
+    for (int it = first; it < last; ++it) {              // (to the end whatever fails: the halves meet)
       const PagedMassItem& m = cur.m;
       const Ahead next = begin(it + 1 < last ? it + 1 : it);
       const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
@@ -270,10 +275,11 @@ __global__ void __launch_bounds__(kMassThreads, 1)
         const int t = m.t0 + x * tq, t_end = min(t + tq, m.t1);
         const int rows = (t_end - t) * p.G;
         const bool mine = blk.meets(t, t_end);
-        ok = __all_sync(0xffffffffu, (!mine || wait_or_abort(&s_full[2 * y + b], (bn >> 1) & 1, p.err, abort_flag)) &&
+        ok = __all_sync(0xffffffffu, ok && (!mine || wait_or_abort(&s_full[2 * y + b], (bn >> 1) & 1, p.err, abort_flag)) &&
                                          wait_or_abort(&r_full[s], (qn / NR) & 1, p.err, abort_flag));
         if (!ok) break;
-        if (mine) {
+        if (mine && half * 64 >= rows) ++bn;
+        else if (mine) {
           tc_fence_after();
           // columns [c_lo, c_hi) are rows that see this thread's key
           const int c_lo = max(cur.f - t, 0) * p.G, c_hi = max(min(cur.l, t_end) - t, 0) * p.G;
@@ -300,18 +306,12 @@ __global__ void __launch_bounds__(kMassThreads, 1)
             }
           };
           const uint32_t tB = tS + b * 128;
-          float va[32], vb[32];                          // one of them on its way
-          tmem_ld32(tB, va);
 #pragma unroll 1
-          for (int c = 0; c < rows; c += 64) {
-            tmem_wait<32>(va);
-            if (c + 32 < rows) tmem_ld32(tB + c + 32, vb);
-            add(va, c);
-            if (c + 32 < rows) {
-              tmem_wait<32>(vb);
-              if (c + 64 < rows) tmem_ld32(tB + c + 64, va);
-              add(vb, c + 32);
-            }
+          for (int c = half * 64; c < min(rows, half * 64 + 64); c += 32) {
+            float v[32];
+            tmem_ld32(tB + c, v);
+            tmem_wait<32>(v);
+            add(v, c);
           }
           tc_fence_before();
           ++bn;
@@ -323,10 +323,13 @@ __global__ void __launch_bounds__(kMassThreads, 1)
         }
       }
       float* next_dst = target(next);
-      const float next_old = it + 1 < last && next_dst != nullptr && next.m.slot < 0 ? *next_dst : 0.f;
+      const float next_old = half == 0 && it + 1 < last && next_dst != nullptr && next.m.slot < 0 ? *next_dst : 0.f;
       float a0, a1;
       unpair(add2(sum0, sum1), a0, a1);
-      if (dst != nullptr && ok) *dst = old + (a0 + a1);
+      float* other = s_half + (it - first & 1) * 128 + r;  // two by turns: read while the next is written
+      if (half == 1) *other = a0 + a1;
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + y) : "memory");
+      if (half == 0 && dst != nullptr && ok) *dst = old + (a0 + a1 + *other);
       cur = next;
       dst = next_dst;
       old = next_old;

@@ -305,3 +305,148 @@ def test_refusals():
     evict = K.EvictPlan([90, 30], 70, kv_heads=2, page_size=64)
     with pytest.raises(_lib.SpecFoldError, match="destination"):
         K.paged_evict(k, v, mass, table, table[:, :1], evict)
+
+
+# ---------------------------------------------------------------------------- the cache and its use
+def test_cache_steps_match_a_contiguous_cache():
+    """Chunks, tokens and idle sequences over several steps, against attention over the sequence's
+    whole history; pages come back when a sequence ends."""
+    from specfold_b200 import PagedKVCache
+    H, Hkv, hd = 8, 2, 64
+    cache = PagedKVCache(2, Hkv, hd, num_pages=40, page_size=16, dtype=F32)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    a, b, c = cache.add(), cache.add(), cache.add()
+    past = {s: [[torch.empty(0, Hkv, hd, device="cuda")] * 2 for _ in range(2)] for s in (a, b, c)}
+    for seqs, q_lens in (([a], [70]), ([b, a], [33, 1]), ([a, c, b], [1, 5, 0]), ([c, a, b], [20, 1, 1])):
+        step = cache.step(seqs, q_lens, heads=H)
+        T = sum(q_lens)
+        for layer in range(2):
+            q, k, v = (torch.randn(T, n, hd, generator=g, device="cuda") for n in (H, Hkv, Hkv))
+            cache.append(layer, k, v, step)
+            out, _ = cache.attend(layer, q, step)
+            t = 0
+            for s, n in zip(seqs, q_lens):
+                kk, vv = (torch.cat((p, x[t:t + n])) for p, x in zip(past[s][layer], (k, v)))
+                past[s][layer] = [kk, vv]
+                if n:
+                    want = torch.nn.functional.scaled_dot_product_attention(
+                        q[t:t + n].transpose(0, 1).double()[None],
+                        kk.transpose(0, 1).repeat_interleave(H // Hkv, 0).double()[None],
+                        vv.transpose(0, 1).repeat_interleave(H // Hkv, 0).double()[None],
+                        attn_mask=torch.ones(n, len(kk), dtype=torch.bool, device="cuda").tril(len(kk) - n))
+                    assert (out[t:t + n].double() - want[0].transpose(0, 1)).abs().max() < 1e-5
+                t += n
+        step.check()
+    assert [cache.length(s) for s in (a, b, c)] == [73, 34, 25]
+    assert cache.free_pages == 40 - 5 - 3 - 2
+    cache.remove(b)
+    assert cache.free_pages == 40 - 5 - 2
+    with pytest.raises(MemoryError):
+        cache.step([c], [40 * 16], heads=H)
+    assert cache.length(c) == 25 and cache.free_pages == 40 - 5 - 2
+    with pytest.raises(ValueError):
+        cache.step([a, a], [1, 1], heads=H)
+    with pytest.raises(ValueError):
+        cache.evict([a], 10)                               # made without track_mass
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_released_pages_are_not_missed(dtype):
+    """Pages that fell out of the window are taken by another sequence; the window's results stay
+    bit for bit."""
+    from specfold_b200 import PagedKVCache
+    H, Hkv, hd, window, sinks = 8, 2, 128, 100, 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = [torch.randn(500, n, hd, generator=g, device="cuda").to(dtype) for n in (H, Hkv, Hkv)]
+    outs = []
+    for free in (False, True):
+        cache = PagedKVCache(1, Hkv, hd, num_pages=64, page_size=16, dtype=dtype)
+        s, at, got = cache.add(), 0, []
+        for n in (300, 1, 150, 1, 40):
+            step = cache.step([s], [n], heads=H, window=window, sinks=sinks)
+            q, k, v = (x[at:at + n] for x in rows)
+            cache.append(0, k, v, step)
+            got.append(cache.attend(0, q, step))
+            step.check()
+            at += n
+            if free:
+                before = cache.free_pages
+                assert cache.release(s, window, sinks) == cache.free_pages - before
+                other = cache.add()                        # whoever gets the pages fills them
+                filler = cache.step([other], [cache.free_pages * 16], heads=H)
+                junk = torch.full((filler.plan.tokens, Hkv, hd), float("nan"), device="cuda").to(dtype)
+                cache.append(0, junk, junk, filler)
+                filler.check()
+                cache.remove(other)
+        outs.append(got)
+        assert not free or (-1 in cache.pages(s) and cache.pages(s)[0] >= 0)
+    for (o1, l1), (o2, l2) in zip(*outs):
+        assert torch.equal(o1, o2) and torch.equal(l1, l2)
+
+
+def test_cache_eviction_keeps_what_was_looked_at():
+    from specfold_b200 import PagedKVCache
+    H, Hkv, hd = 4, 2, 64
+    cache = PagedKVCache(2, Hkv, hd, num_pages=40, page_size=16, dtype=F32, track_mass=True)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    a, b = cache.add(), cache.add()
+    step = cache.step([a, b], [200, 30], heads=H)
+    for layer in range(2):
+        q, k, v = (torch.randn(230, n, hd, generator=g, device="cuda") for n in (H, Hkv, Hkv))
+        cache.append(layer, k, v, step)
+        _, lse = cache.attend(layer, q, step)
+        cache.accumulate(layer, q, lse, step)
+    step.check()
+    # all rows' weights add up to one each
+    total = sum(float(cache._mass[0, p].sum()) for s in (a, b) for p in cache.pages(s))
+    assert abs(total - 230 * H) < 1e-2
+    free = cache.free_pages
+    old = [cache._mass[layer][cache.pages(a)].transpose(0, 1).reshape(Hkv, -1)[:, :200].clone() for layer in range(2)]
+    kept = cache.evict([a, b], 64, sinks=4, recent=8)
+    assert cache.length(a) == 64 and cache.length(b) == 30 and cache.free_pages == free + 13 - 4
+    for layer in range(2):
+        for h in range(Hkv):
+            want = ref.evict_positions(old[layer][h].tolist(), 64, 4, 8)
+            assert kept[layer][0, h].tolist() == want
+            assert kept[layer][1, h].tolist() == list(range(30)) + [-1] * 34
+            now = cache._mass[layer][cache.pages(a), h].flatten()
+            assert torch.equal(now, old[layer][h][want])
+    with pytest.raises(ValueError):
+        cache.evict([a], 10, sinks=6, recent=5)
+    step = cache.step([a, b], [1, 1], heads=H)                # and the sequences go on
+    k = torch.randn(2, Hkv, hd, generator=g, device="cuda")
+    cache.append(0, k, k, step)
+    cache.attend(0, torch.randn(2, H, hd, generator=g, device="cuda"), step)
+    step.check()
+    assert cache.length(a) == 65
+
+
+@pytest.mark.parametrize("shape,dtype,tol", [("tiny", F32, 1e-4), ("tiny128", BF, 2e-2)])
+def test_serving_example_matches_the_dense_model(shape, dtype, tol):
+    """examples/paged_serving.py's decoder, chunk by chunk and token by token next to other
+    requests, against the model's own forward over the whole text (fp32 on the CPU)."""
+    import importlib.util
+    import os
+    from specfold_b200 import synthetic as syn
+    path = os.path.join(os.path.dirname(os.path.dirname(__file__)), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    dims = syn.SHAPES[shape]
+    model = syn.build_model(dims, family="fastdllm", dtype=dtype, seed=3)
+    dense = syn.build_model(dims, family="fastdllm", dtype=dtype, seed=3).float()
+    g = torch.Generator().manual_seed(4)
+    texts = [torch.randint(0, dims.vocab, (n,), generator=g).tolist() for n in (150, 21)]
+    dec = ex.PagedDecoder(model.cuda(), dims, num_pages=32, page_size=16)
+    a, b = dec.add(), dec.add()
+    dec.step([a], [texts[0][:100]])
+    dec.step([a, b], [texts[0][100:149], texts[1][:20]])
+    got = dec.step([b, a], [texts[1][20:], texts[0][149:]])
+    for row, text in ((1, texts[0]), (0, texts[1])):
+        with torch.no_grad():
+            want = dense(torch.tensor([text])).logits[0, -1]
+        off = (got[row].float().cpu() - want).abs().max() / want.abs().max()
+        assert off <= tol, float(off)
+    out = ex.serve(ex.PagedDecoder(model, dims, num_pages=64, page_size=16, track_mass=True),
+                   texts + [texts[0][:7]], 12, budget=64)
+    assert [len(o) for o in out] == [12] * 3
