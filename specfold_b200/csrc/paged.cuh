@@ -25,7 +25,8 @@
 
 namespace sf {
 
-constexpr int kPagedKB = 128;         // keys of one block: the unit the plan counts in
+constexpr int kPagedKB = 128;         // keys of one block: the unit the plan counts in ...
+constexpr int kPagedKeysF32 = 64;     // ... and that of the fp32 attention
 constexpr int kPagedMaxGroup = 16;    // query heads per kv head
 
 // A run [i0, i1) of the key blocks that a tile of query rows sees.  The blocks a tile sees
@@ -258,11 +259,11 @@ __device__ __forceinline__ void paged_join_row(const PagedAttnParams& p, const P
   if (lane == 0) p.lse[row] = m * 0.6931471805599453f + logf(l);
 }
 
-cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cudaStream_t st);
+cudaError_t launch_paged_attention_simt(const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_attention_tokens(const PagedAttnParams& p, int copies, cudaStream_t st);
 cudaError_t launch_paged_attention_chunk(const PagedAttnParams& p, cudaStream_t st);
 cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t st);
-cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st);
+cudaError_t launch_paged_mass_simt(const PagedMassParams& p, cudaStream_t st);
 cudaError_t launch_paged_mass_tc(const PagedMassParams& p, cudaStream_t st);
 cudaError_t launch_paged_mass_merge(const PagedMassParams& p, cudaStream_t st);
 

@@ -6,12 +6,16 @@
 // thread, the running maximum and sum of the softmax per row, P back through shared memory, and
 // O += P V with an RM x hd/16 register tile.  K and V share one buffer so that two CTAs fit an
 // SM and one's loads run under the other's products.
-#include "paged.cuh"
+//
+// Products are taken two at a time (fma.rn.f32x2): the kernel is bound by issue slots and shared
+// memory, not by the FMA pipe (45% busy with single ones).  Scores add up even and odd dims apart;
+// for P V each weight is stored twice, side by side.
+#include "paged_tc.cuh"
 
 namespace sf {
 
 constexpr int kSimtThreads = 256;
-constexpr int kSimtKeys = 64;
+constexpr int kSimtKeys = kPagedKeysF32;
 
 template <typename T>
 __device__ __forceinline__ void simt_store_row(float* dst, const T* src, int e);
@@ -73,27 +77,34 @@ __device__ __forceinline__ void simt_load_q(float* sQ, const void* q, int64_t q_
 template <int HD, int RM>
 __device__ __forceinline__ void simt_scores(const float* sQ, const float* sK, float (&s)[RM][4]) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  uint64_t s2[RM][4];
 #pragma unroll
   for (int a = 0; a < RM; ++a)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) s[a][c] = 0.f;
+    for (int c = 0; c < 4; ++c) s2[a][c] = 0;
 #pragma unroll 4
   for (int d = 0; d < HD; d += 4) {
-    float4 kf[4], qf[RM];
+    ulonglong2 kf[4], qf[RM];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const float4*>(sK + (tx + 16 * c) * (HD + 4) + d);
+    for (int c = 0; c < 4; ++c) kf[c] = *reinterpret_cast<const ulonglong2*>(sK + (tx + 16 * c) * (HD + 4) + d);
 #pragma unroll
-    for (int a = 0; a < RM; ++a) qf[a] = *reinterpret_cast<const float4*>(sQ + (ty + 16 * a) * (HD + 4) + d);
+    for (int a = 0; a < RM; ++a) qf[a] = *reinterpret_cast<const ulonglong2*>(sQ + (ty + 16 * a) * (HD + 4) + d);
 #pragma unroll
     for (int a = 0; a < RM; ++a)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        s[a][c] = fmaf(qf[a].x, kf[c].x, s[a][c]);
-        s[a][c] = fmaf(qf[a].y, kf[c].y, s[a][c]);
-        s[a][c] = fmaf(qf[a].z, kf[c].z, s[a][c]);
-        s[a][c] = fmaf(qf[a].w, kf[c].w, s[a][c]);
+        s2[a][c] = fma2(qf[a].x, kf[c].x, s2[a][c]);
+        s2[a][c] = fma2(qf[a].y, kf[c].y, s2[a][c]);
       }
   }
+#pragma unroll
+  for (int a = 0; a < RM; ++a)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float even, odd;
+      unpair(s2[a][c], even, odd);
+      s[a][c] = even + odd;
+    }
 }
 
 __device__ __forceinline__ float half_warp_max(float v) {
@@ -109,12 +120,12 @@ __device__ __forceinline__ float half_warp_sum(float v) {
 
 template <typename T, int HD, int RM>
 __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(PagedAttnParams p) {
-  constexpr int R = 16 * RM, LD = HD + 4, LP = kSimtKeys + 4;
+  constexpr int R = 16 * RM, LD = HD + 4, LP = 2 * kSimtKeys + 4;
   constexpr int DV = HD / 64;                           // float4 groups of O per thread
   extern __shared__ __align__(16) float sm[];
   float* sQ = sm;                                       // [R][LD]
   float* sKV = sQ + R * LD;                             // [64][LD]
-  float* sP = sKV + kSimtKeys * LD;                     // [R][LP]
+  float* sP = sKV + kSimtKeys * LD;                     // [R][LP], every weight twice
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float sl2 = p.scale * 1.4426950408889634f;
   const int last = p.first[blockIdx.x + 1];
@@ -122,14 +133,15 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
     const PagedItem w = p.items[it];
     const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
     const int rows = w.ntok * p.G;
-    float m[RM], l[RM], o[RM][DV][4];
+    float m[RM], l[RM];
+    uint64_t o[RM][DV][2];
     int hi[RM], lo[RM];
 #pragma unroll
     for (int a = 0; a < RM; ++a) {
       m[a] = -INFINITY;
       l[a] = 0.f;
 #pragma unroll
-      for (int d = 0; d < DV; ++d) o[a][d][0] = o[a][d][1] = o[a][d][2] = o[a][d][3] = 0.f;
+      for (int d = 0; d < DV; ++d) o[a][d][0] = o[a][d][1] = 0;
       const int r = ty + 16 * a;
       const int i = w.tok0 + r / p.G;
       hi[a] = r < rows ? mask.hi(i) : 0;
@@ -139,64 +151,61 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
     __syncthreads();                                    // the previous item's reads are done
     simt_load_q<T, HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + w.tok0, w.kvh, p.G, rows);
     for (int i = w.i0; i < w.i1; ++i) {
-      for (int sub = 0; sub < kPagedKB / kSimtKeys; ++sub) {
-        const int k0 = w.block(i) * kPagedKB + sub * kSimtKeys;
-        if (k0 >= range.hi) break;
-        __syncthreads();
-        simt_load_keys<T, HD>(sKV, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
-        __syncthreads();
-        float s[RM][4];
-        simt_scores<HD, RM>(sQ, sKV, s);
+      const int k0 = w.block(i) * kSimtKeys;
+      __syncthreads();
+      simt_load_keys<T, HD>(sKV, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
+      __syncthreads();
+      float s[RM][4];
+      simt_scores<HD, RM>(sQ, sKV, s);
 #pragma unroll
-        for (int a = 0; a < RM; ++a) {
-          float mx = -INFINITY;
+      for (int a = 0; a < RM; ++a) {
+        float mx = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int j = k0 + tx + 16 * c;
-            const bool see = j < hi[a] && (j >= lo[a] || j < p.sinks);
-            s[a][c] = see ? s[a][c] * sl2 : -INFINITY;
-            mx = fmaxf(mx, s[a][c]);
-          }
-          const float mn = fmaxf(m[a], half_warp_max(mx));
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          const float alpha = exp2f(m[a] - ref);
-          float sum = 0.f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float e = exp2f(s[a][c] - ref);
-            sum += e;
-            sP[(ty + 16 * a) * LP + tx + 16 * c] = e;
-          }
-          l[a] = l[a] * alpha + half_warp_sum(sum);
-          m[a] = mn;
-#pragma unroll
-          for (int d = 0; d < DV; ++d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[a][d][x] *= alpha;
+        for (int c = 0; c < 4; ++c) {
+          const int j = k0 + tx + 16 * c;
+          const bool see = j < hi[a] && (j >= lo[a] || j < p.sinks);
+          s[a][c] = see ? s[a][c] * sl2 : -INFINITY;
+          mx = fmaxf(mx, s[a][c]);
         }
-        __syncthreads();                                // K read, P written
-        simt_load_keys<T, HD>(sKV, p.pool.v, p.pool, w.seq, w.kvh, k0, range, p.err);
-        __syncthreads();
-        // a row of P is written and read by the same half-warp's 16 threads
-#pragma unroll 2
-        for (int j = 0; j < kSimtKeys; j += 4) {
-          float4 pf[RM];
+        const float mn = fmaxf(m[a], half_warp_max(mx));
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = exp2f(m[a] - ref);
+        float sum = 0.f;
 #pragma unroll
-          for (int a = 0; a < RM; ++a) pf[a] = *reinterpret_cast<const float4*>(sP + (ty + 16 * a) * LP + j);
+        for (int c = 0; c < 4; ++c) {
+          const float e = exp2f(s[a][c] - ref);
+          sum += e;
+          *reinterpret_cast<float2*>(sP + (ty + 16 * a) * LP + 2 * (tx + 16 * c)) = make_float2(e, e);
+        }
+        l[a] = l[a] * alpha + half_warp_sum(sum);
+        m[a] = mn;
+        const uint64_t alpha2 = pair(alpha, alpha);
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj)
+        for (int d = 0; d < DV; ++d) {
+          o[a][d][0] = fma2(o[a][d][0], alpha2, 0);
+          o[a][d][1] = fma2(o[a][d][1], alpha2, 0);
+        }
+      }
+      __syncthreads();                                  // K read, P written
+      simt_load_keys<T, HD>(sKV, p.pool.v, p.pool, w.seq, w.kvh, k0, range, p.err);
+      __syncthreads();
+      // a row of P is written and read by the same half-warp's 16 threads
+#pragma unroll 4
+      for (int j = 0; j < kSimtKeys; j += 2) {
+        ulonglong2 pf[RM];
 #pragma unroll
-            for (int d = 0; d < DV; ++d) {
-              const float4 v = *reinterpret_cast<const float4*>(sKV + (j + jj) * LD + d * 64 + tx * 4);
+        for (int a = 0; a < RM; ++a) pf[a] = *reinterpret_cast<const ulonglong2*>(sP + (ty + 16 * a) * LP + 2 * j);
 #pragma unroll
-              for (int a = 0; a < RM; ++a) {
-                const float e = jj == 0 ? pf[a].x : jj == 1 ? pf[a].y : jj == 2 ? pf[a].z : pf[a].w;
-                o[a][d][0] = fmaf(e, v.x, o[a][d][0]);
-                o[a][d][1] = fmaf(e, v.y, o[a][d][1]);
-                o[a][d][2] = fmaf(e, v.z, o[a][d][2]);
-                o[a][d][3] = fmaf(e, v.w, o[a][d][3]);
-              }
-            }
+        for (int d = 0; d < DV; ++d) {
+          const ulonglong2 v0 = *reinterpret_cast<const ulonglong2*>(sKV + j * LD + d * 64 + tx * 4);
+          const ulonglong2 v1 = *reinterpret_cast<const ulonglong2*>(sKV + (j + 1) * LD + d * 64 + tx * 4);
+#pragma unroll
+          for (int a = 0; a < RM; ++a) {
+            o[a][d][0] = fma2(pf[a].x, v0.x, o[a][d][0]);
+            o[a][d][1] = fma2(pf[a].x, v0.y, o[a][d][1]);
+            o[a][d][0] = fma2(pf[a].y, v1.x, o[a][d][0]);
+            o[a][d][1] = fma2(pf[a].y, v1.y, o[a][d][1]);
+          }
         }
       }
     }
@@ -208,8 +217,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
         const int64_t pr = static_cast<int64_t>(w.slot) * p.rows + r;
 #pragma unroll
         for (int d = 0; d < DV; ++d)
-          *reinterpret_cast<float4*>(p.part_O + pr * HD + d * 64 + tx * 4) =
-              make_float4(o[a][d][0], o[a][d][1], o[a][d][2], o[a][d][3]);
+          *reinterpret_cast<ulonglong2*>(p.part_O + pr * HD + d * 64 + tx * 4) = make_ulonglong2(o[a][d][0], o[a][d][1]);
         if (tx == 0) {
           p.part_ml[2 * pr] = m[a];
           p.part_ml[2 * pr + 1] = l[a];
@@ -222,7 +230,12 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) dst[d * 64 + tx * 4 + x] = Elt<T>::from_f(o[a][d][x] * inv);
+          for (int x = 0; x < 2; ++x) {
+            float e0, e1;
+            unpair(o[a][d][x], e0, e1);
+            dst[d * 64 + tx * 4 + 2 * x] = Elt<T>::from_f(e0 * inv);
+            dst[d * 64 + tx * 4 + 2 * x + 1] = Elt<T>::from_f(e1 * inv);
+          }
         if (tx == 0) p.lse[t * p.H + h] = m[a] * 0.6931471805599453f + logf(l[a]);
       }
     }
@@ -266,20 +279,16 @@ cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t
 template <typename T, int HD, int RM>
 static cudaError_t attention_simt(const PagedAttnParams& p, cudaStream_t st) {
   constexpr int R = 16 * RM;
-  constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + R * (kSimtKeys + 4)) * 4;
+  constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + R * (2 * kSimtKeys + 4)) * 4;
   cudaError_t e = allow_smem(paged_attention_simt_kernel<T, HD, RM>, smem);
   if (e != cudaSuccess) return e;
   paged_attention_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
   return launched();
 }
 
-cudaError_t launch_paged_attention_simt(int dtype, const PagedAttnParams& p, cudaStream_t st) {
+cudaError_t launch_paged_attention_simt(const PagedAttnParams& p, cudaStream_t st) {
   if (p.workers == 0) return cudaSuccess;
   const bool wide = p.rows == 64;
-  if (dtype == BF16) {
-    if (p.hd == 128) return wide ? attention_simt<__nv_bfloat16, 128, 4>(p, st) : attention_simt<__nv_bfloat16, 128, 1>(p, st);
-    return wide ? attention_simt<__nv_bfloat16, 64, 4>(p, st) : attention_simt<__nv_bfloat16, 64, 1>(p, st);
-  }
   if (p.hd == 128) return wide ? attention_simt<float, 128, 4>(p, st) : attention_simt<float, 128, 1>(p, st);
   return wide ? attention_simt<float, 64, 4>(p, st) : attention_simt<float, 64, 1>(p, st);
 }
@@ -385,10 +394,8 @@ static cudaError_t mass_simt(const PagedMassParams& p, cudaStream_t st) {
   return launched();
 }
 
-cudaError_t launch_paged_mass_simt(int dtype, const PagedMassParams& p, cudaStream_t st) {
+cudaError_t launch_paged_mass_simt(const PagedMassParams& p, cudaStream_t st) {
   if (p.workers == 0) return cudaSuccess;
-  if (dtype == BF16)
-    return p.hd == 128 ? mass_simt<__nv_bfloat16, 128, 4>(p, st) : mass_simt<__nv_bfloat16, 64, 4>(p, st);
   return p.hd == 128 ? mass_simt<float, 128, 4>(p, st) : mass_simt<float, 64, 4>(p, st);
 }
 

@@ -257,6 +257,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
     }
     at = up4(at);
     p.ws_bytes = 0;
+    const int keys = p.dtype == SF_DTYPE_BF16 ? kPagedKB : kPagedKeysF32;   // of a block
     for (int k = 0; k < 2; ++k) {
       std::vector<PagedItem> tiles;
       std::vector<int> units;
@@ -276,9 +277,9 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
             it.ntok = std::min(t.per_tile[k], q_lens[b] - t0);
             it.slot = -1;
             const int hi = std::max(0, mask.hi(t0 + it.ntok - 1));
-            const int end = (hi + kPagedKB - 1) / kPagedKB;
-            it.lo_blk = std::min(mask.lo(t0) / kPagedKB, end);
-            it.sink_blks = std::min((std::min(p.sinks, hi) + kPagedKB - 1) / kPagedKB, it.lo_blk);
+            const int end = (hi + keys - 1) / keys;
+            it.lo_blk = std::min(mask.lo(t0) / keys, end);
+            it.sink_blks = std::min((std::min(p.sinks, hi) + keys - 1) / keys, it.lo_blk);
             it.i1 = it.sink_blks + end - it.lo_blk;
             it.q0 = q0;
             it.q_len = q_lens[b];
@@ -467,7 +468,7 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
     else if (plan->dtype == SF_DTYPE_BF16)
       e = launch_paged_attention_chunk(p, st);
     else
-      e = launch_paged_attention_simt(plan->dtype, p, st);
+      e = launch_paged_attention_simt(p, st);
     if (e == cudaSuccess) e = launch_paged_merge(plan->dtype, p, st);
     if (e != cudaSuccess) return status(e, "paged_attention");
   }
@@ -506,7 +507,7 @@ int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool
   p.scale = scale;
   p.err = plan->err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = plan->dtype == SF_DTYPE_BF16 ? launch_paged_mass_tc(p, st) : launch_paged_mass_simt(plan->dtype, p, st);
+  cudaError_t e = plan->dtype == SF_DTYPE_BF16 ? launch_paged_mass_tc(p, st) : launch_paged_mass_simt(p, st);
   if (e == cudaSuccess) e = launch_paged_mass_merge(p, st);
   return status(e, "paged_attention_mass");
 }

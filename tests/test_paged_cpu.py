@@ -24,13 +24,13 @@ def build(q_lens, kv_lens, **kw):
     return c, words.tolist()
 
 
-def visible_blocks(q, n, i, block, window, sinks):
-    """Blocks of 128 keys that token i sees a key of."""
+def visible_blocks(q, n, i, block, window, sinks, keys=128):
+    """Blocks of 128 (or ``keys``) keys that token i sees a key of."""
     hi = n if block == 0 else min(n, n - q + (i // block + 1) * block)
     lo = max(0, n - q + i - window + 1) if window else 0
     out = set()
-    for b in range(-(-max(hi, 0) // 128)):
-        a, e = b * 128, min(hi, b * 128 + 128)
+    for b in range(-(-max(hi, 0) // keys)):
+        a, e = b * keys, min(hi, b * keys + keys)
         if max(a, lo) < e or (window and a < min(sinks, e)):
             out.add(b)
     return out
@@ -50,7 +50,7 @@ def test_a_plan_covers_every_row_and_key_once(seed):
     assert c.T == sum(q) and bool(c.short_chunk) == any(a > b for a, b in zip(q, n))
     assert w[c.tokens:c.tokens + 2 * c.T] == [x for b in range(len(q)) for i in range(q[b])
                                               for x in (b, n[b] - q[b] + i)]
-    rows = set()
+    rows, keys = set(), 128 if c.dtype else 64
     for part in c.attn:
         if part.n_items == 0:
             continue
@@ -75,11 +75,11 @@ def test_a_plan_covers_every_row_and_key_once(seed):
                 used += [slot] if slot >= 0 else []
             sink, lo = pieces[0][3:]
             blocks = [i if i < sink else i - sink + lo for i in range(at)]
-            assert len(set(blocks)) == len(blocks) and all(b * 128 < n[seq] for b in blocks)
+            assert len(set(blocks)) == len(blocks) and all(b * keys < n[seq] for b in blocks)
             for t in range(t0, t0 + nt):
                 assert (seq, kvh, t) not in rows
                 rows.add((seq, kvh, t))
-                assert visible_blocks(q[seq], n[seq], t, block, window, sinks) <= set(blocks)
+                assert visible_blocks(q[seq], n[seq], t, block, window, sinks, keys) <= set(blocks)
         assert used == list(range(part.slots))
         merged = [w[part.merges + MERGE * x:][:MERGE] for x in range(part.n_merges)]
         assert [s for m in merged for s in range(m[3], m[3] + m[4])] == used
