@@ -7,9 +7,12 @@
 // O += P V with an RM x hd/16 register tile.  K and V share one buffer so that two CTAs fit an
 // SM and one's loads run under the other's products.
 //
-// Products are taken two at a time (fma.rn.f32x2): the kernel is bound by issue slots and shared
-// memory, not by the FMA pipe (45% busy with single ones).  Scores add up even and odd dims apart;
-// for P V each weight is stored twice, side by side.
+// Products are taken two at a time (fma.rn.f32x2): half the issue slots for the same FMA rate.
+// Scores add up even and odd dims apart; for P V each weight is stored twice, side by side.
+//
+// Measured (12 / 2 heads of 128, 704 tokens over 800 to 2100 keys, block-causal): 254 us, 24
+// TFLOP/s of the 70 the FMA pipes could do; single products took 265 us.  What bounds it is the
+// loads' latency with two CTAs of 8 warps on an SM: shared memory has no room for a second buffer.
 #include "paged_tc.cuh"
 
 namespace sf {
