@@ -297,10 +297,15 @@ cudaError_t launch_paged_attention_simt(const PagedAttnParams& p, cudaStream_t s
 }
 
 // ------------------------------------------------------------------ weight accumulation
-__device__ __forceinline__ float* mass_slot(const PagedMassParams& p, int seq, int kvh, int key) {
-  const int page = paged_page(p.pool, seq, key >> p.pool.page_shift, p.err);
-  return p.pool.mass + ((static_cast<int64_t>(page) * p.Hkv + kvh) << p.pool.page_shift) +
-         (key & ((1 << p.pool.page_shift) - 1));
+// a key's accumulated weight; a page outside the pool is flagged, and nothing is written
+__device__ __forceinline__ void add_mass(const PagedMassParams& p, int seq, int kvh, int key, float sum) {
+  const int page = p.pool.table[seq * p.pool.table_stride + (key >> p.pool.page_shift)];
+  if (page < 0 || page >= p.pool.num_pages) {
+    flag_error(p.err, SF_DEV_ERR_INDEX);
+    return;
+  }
+  p.pool.mass[ ((static_cast<int64_t>(page) * p.Hkv + kvh) << p.pool.page_shift) +
+              (key & ((1 << p.pool.page_shift) - 1))] += sum;
 }
 
 // A key's weight over all rows that see it: sum of exp(s - lse).  A CTA owns a key block and
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedM
           if (w.slot >= 0)
             p.part[static_cast<int64_t>(w.slot) * kMassBlocks * kPagedKB + j - w.kb0 * kPagedKB] = sum;
           else
-            *mass_slot(p, w.seq, w.kvh, j) += sum;
+            add_mass(p, w.seq, w.kvh, j, sum);
         }
       }
     }
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kMassBlocks * kPagedKB) paged_mass_merge_kerne
   if (f >= l) return;                                   // no token sees it
   float sum = 0.f;
   for (int i = 0; i < w.n; ++i) sum += p.part[static_cast<int64_t>(w.slot0 + i) * kMassBlocks * kPagedKB + threadIdx.x];
-  *mass_slot(p, w.seq, w.kvh, key) += sum;
+  add_mass(p, w.seq, w.kvh, key, sum);
 }
 
 cudaError_t launch_paged_mass_merge(const PagedMassParams& p, cudaStream_t st) {

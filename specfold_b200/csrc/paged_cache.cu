@@ -97,6 +97,16 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* s_warp) {
   return v + (warp > 0 ? s_warp[warp - 1] : 0);
 }
 
+// {cached keys, keys that stay} of a sequence; what the host's bounds do not cover is flagged and
+// cut to them (a budget too small for sinks + recent: everything up to it stays)
+__device__ __forceinline__ void evict_lens(const PagedEvictParams& p, int b, int* n, int* keep) {
+  const int a = p.lens[2 * b], k = p.lens[2 * b + 1];
+  *n = min(max(a, 0), p.max_len);
+  *keep = min(max(k, 0), p.max_keep);
+  if (*n > *keep && *keep < p.sinks + p.recent) *n = *keep;
+  if ((*n != a || *keep != k) && threadIdx.x == 0) flag_error(p.err, SF_DEV_ERR_INDEX);
+}
+
 __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedEvictParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -108,7 +118,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedEvictPar
   const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int h = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = p.lens[2 * b], keep = p.lens[2 * b + 1];
+  int n, keep;
+  evict_lens(p, b, &n, &keep);
   int32_t* out = p.kept + (static_cast<int64_t>(b) * p.Hkv + h) * p.kept_stride;
   const int tid = rank * kSelThreads + threadIdx.x, all = C * kSelThreads;
   pdl_trigger();                                         // the move may line up
@@ -302,7 +313,9 @@ __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvictParams p) {
   constexpr int vpk = 2 * vpr;                          // vectors of a key
   __shared__ int64_t s_src[kMoveKeys], s_dst[kMoveKeys];
   const int bh = blockIdx.y, b = bh / p.Hkv, h = bh % p.Hkv;
-  const int stay = min(p.lens[2 * b], p.lens[2 * b + 1]);
+  int n, keep;
+  evict_lens(p, b, &n, &keep);
+  const int stay = min(n, keep);
   const int base = blockIdx.x * kMoveKeys, keys = min(kMoveKeys, stay - base);
   if (keys <= 0) return;
   pdl_wait();

@@ -68,6 +68,7 @@ int check_plan(const sf_paged_plan* p, const int32_t* q_lens, const int32_t* kv_
   if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
     return bad("paged plan: page size %d must be a power of two in [16, 256]", p->page_size);
   if (p->block < 0 || p->window < 0 || p->sinks < 0) return bad("paged plan: block, window and sinks must not be negative");
+  if (p->window > (1 << 30)) return bad("paged plan: a window of %d is no limit: pass 0", p->window);
   int64_t T = 0;
   for (int b = 0; b < p->B; ++b) {
     if (q_lens[b] < 0 || kv_lens[b] < 0) return bad("paged plan: sequence %d has a negative length", b);

@@ -217,6 +217,37 @@ def test_a_page_outside_the_pool_is_reported(dtype):
     with pytest.raises(_lib.SpecFoldError, match="index out of range"):
         plan.check()
     assert torch.equal(k[bt.table[1, 2]], before[bt.table[1, 2]])     # nothing was written there
+    # weights: those of the keys on the missing page are left out, no other page gets them
+    plan, want, got = plan_of(bt), mass.clone(), mass.clone()
+    q, lse = bt.queries(bt.wide.cuda()), torch.full((71, 8), 3.0, device="cuda")
+    K.paged_attention_mass(q, k, bt.table.cuda(), lse, want, plan_of(bt))
+    K.paged_attention_mass(q, k, table.cuda(), lse, got, plan)
+    with pytest.raises(_lib.SpecFoldError, match="index out of range"):
+        plan.check()
+    gone = bt.table[1, 2].item()
+    assert torch.equal(got[gone], mass[gone])
+    keep = torch.arange(mass.shape[0]) != gone
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_eviction_lengths_beyond_the_hosts_bounds_are_cut():
+    """Lengths on the device that contradict what the call was sized for are reported, and
+    nothing outside its buffers is touched."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k = torch.randn(16, 2, 16, 64, generator=g, device="cuda")
+    v, mass = torch.randn_like(k), torch.rand(16, 2, 16, generator=g, device="cuda")
+    src = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    dst = torch.arange(8, 14, dtype=torch.int32, device="cuda").view(2, 3)
+    for lens in ([[900, 40], [64, 40]], [[64, 900], [64, 40]], [[64, 3], [64, 40]], [[-5, 40], [64, 40]]):
+        plan = K.EvictPlan([64, 64], 40, kv_heads=2, page_size=16, sinks=4, recent=4)
+        plan._lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        spare = k[14:].clone()
+        kept = K.paged_evict(k, v, mass, src, dst, plan)
+        with pytest.raises(_lib.SpecFoldError, match="index out of range"):
+            plan.check()
+        assert torch.equal(k[14:], spare)
+        assert int(kept.max()) < 64 and int(kept.min()) >= -1
+        assert kept[1, 0].tolist()[:4] == [0, 1, 2, 3]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])

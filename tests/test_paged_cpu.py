@@ -115,7 +115,7 @@ GOOD = dict(dtype=1, H=8, Hkv=2, hd=128, page_size=64, block=1)
     (dict(dtype=2), b"dtype"), (dict(hd=96), b"head_dim"), (dict(H=7), b"heads"), (dict(H=34), b"heads"),
     (dict(Hkv=0), b"heads"), (dict(page_size=8), b"page size"), (dict(page_size=48), b"page size"),
     (dict(page_size=512), b"page size"), (dict(block=-1), b"negative"), (dict(window=-1), b"negative"),
-    (dict(sinks=-1), b"negative")])
+    (dict(sinks=-1), b"negative"), (dict(window=(1 << 30) + 1), b"window")])
 def test_plan_refusals(wrong, said):
     lib = _lib.load()
     q = torch.tensor([1], dtype=torch.int32)
