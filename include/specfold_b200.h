@@ -363,6 +363,7 @@ typedef struct sf_paged_plan {
   /* set by the caller */
   int32_t dtype, B, H, Hkv, hd, page_size, block, window, sinks;
   int32_t sms;                       /* SMs to spread the work over; 0: the current device's */
+  int32_t skip_mass;                 /* nonzero: leave out what sf_paged_attention_mass needs */
   /* set by sf_paged_plan_build */
   int32_t T, max_kv, short_chunk;    /* short_chunk: some q_len > kv_len (nothing to append) */
   int32_t tokens;                    /* offset of the {sequence, position} list */

@@ -53,7 +53,7 @@ class SfPagedList(C.Structure):
 
 class SfPagedPlan(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("dtype", "B", "H", "Hkv", "hd", "page_size", "block", "window",
-                                         "sinks", "sms", "T", "max_kv", "short_chunk", "tokens")] + [
+                                         "sinks", "sms", "skip_mass", "T", "max_kv", "short_chunk", "tokens")] + [
         ("attn", SfPagedList * 2), ("mass", SfPagedList), ("words", c_int64), ("ws_bytes", c_size_t),
         ("dev", c_void_p), ("ws", c_void_p), ("err", c_void_p),
     ]

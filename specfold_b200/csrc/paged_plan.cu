@@ -339,7 +339,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       const int tile = std::max(1, t.mass_rows / G);
       int q0 = 0;
       for (int b = 0; b < p.B; q0 += q_lens[b], ++b) {
-        if (q_lens[b] == 0) continue;
+        if (q_lens[b] == 0 || p.skip_mass) continue;
         const PagedMask mask{p.block, p.window, p.sinks, q_lens[b], kv_lens[b]};
         for (int h = 0; h < p.Hkv; ++h)
           for (int kb = 0; kb * kPagedKB < kv_lens[b]; kb += kMassBlocks) {
@@ -479,6 +479,7 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
 int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* q, int64_t q_tok_stride,
                             int64_t q_head_stride, const float* lse, float scale, void* stream) {
   int rc = check_ready("paged_attention_mass", plan);
+  if (rc == SF_OK && plan->skip_mass) rc = bad("paged_attention_mass: the plan was made without it");
   if (rc != SF_OK || plan->mass.n_items == 0) return rc;
   if ((rc = check_pool("paged_attention_mass", pool, plan->dtype, plan->hd, plan->page_size, plan->max_kv, false, true)) != SF_OK ||
       (rc = check_rows("paged_attention_mass", plan, q, q_tok_stride, q_head_stride)) != SF_OK)

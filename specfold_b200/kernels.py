@@ -356,11 +356,12 @@ class PagedPlan(_OnStream):
     ``q_lens[b]`` new tokens of sequence b see its ``kv_lens[b]`` cached keys (the new ones
     included): all up to the end of their own block of ``block`` tokens (1: causal, N:
     block-causal, 0: all), and with ``window`` > 0 only those less than ``window`` positions
-    back and the first ``sinks``."""
+    back and the first ``sinks``.  ``mass`` False leaves out what paged_attention_mass needs (for
+    a large batch of single tokens most of a plan)."""
 
     def __init__(self, q_lens: Sequence[int], kv_lens: Sequence[int], *, heads: int, kv_heads: int,
                  head_dim: int, page_size: int, dtype: torch.dtype = torch.bfloat16, block: int = 1,
-                 window: int = 0, sinks: int = 0, device="cuda"):
+                 window: int = 0, sinks: int = 0, mass: bool = True, device="cuda"):
         q, n = _int32(q_lens), _int32(kv_lens)
         if q.numel() != n.numel():
             raise ValueError(f"{q.numel()} chunk lengths for {n.numel()} cache lengths")
@@ -369,7 +370,7 @@ class PagedPlan(_OnStream):
         lib = _lib.load()
         c = _lib.SfPagedPlan(dtype=_lib.SF_DTYPE_BF16 if dtype == torch.bfloat16 else _lib.SF_DTYPE_F32,
                              B=q.numel(), H=heads, Hkv=kv_heads, hd=head_dim, page_size=page_size,
-                             block=block, window=window, sinks=sinks)
+                             block=block, window=window, sinks=sinks, skip_mass=not mass)
         device = _cuda_device(device)
         c.sms = torch.cuda.get_device_properties(device).multi_processor_count
         cap = lib.sf_paged_plan_words(ctypes.byref(c), q.data_ptr(), n.data_ptr())

@@ -114,7 +114,8 @@ class PagedKVCache:
         more = [self._need(n) - len(self._pages[s]) for s, n in zip(seqs, lens)]
         plan = K.PagedPlan(q_lens, lens, heads=heads, kv_heads=self.num_kv_heads,
                            head_dim=self.head_dim, page_size=self.page_size, dtype=self.dtype,
-                           block=block, window=window, sinks=sinks, device=self.device)
+                           block=block, window=window, sinks=sinks, mass=self._mass is not None,
+                           device=self.device)
         fresh = self._take(sum(more))
         for s, n, m in zip(seqs, lens, more):
             self._pages[s] += [fresh.pop() for _ in range(m)]

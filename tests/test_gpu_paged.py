@@ -329,6 +329,10 @@ def test_refusals():
         K.paged_attention_mass(q, k, table, lse, mass.double(), plan)
     with pytest.raises(ValueError):
         K.paged_attention_mass(q, k, table, lse.half(), mass, plan)
+    light = K.PagedPlan([1, 9], [90, 30], heads=4, kv_heads=2, head_dim=128, page_size=64, block=0, mass=False)
+    K.paged_attention(q, k, v, table, light)
+    with pytest.raises(_lib.SpecFoldError, match="made without"):
+        K.paged_attention_mass(q, k, table, lse, mass, light)
     more = K.PagedPlan([5], [3], heads=4, kv_heads=2, head_dim=128, page_size=64)
     new = torch.zeros(5, 2, 128, dtype=BF, device="cuda")
     with pytest.raises(_lib.SpecFoldError, match="more new tokens"):
