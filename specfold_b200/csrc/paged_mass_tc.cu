@@ -19,7 +19,7 @@
 //
 // Measured: 28 / 4 heads, 4051 tokens over 5300 and 8192 keys, 0.167 TFLOP, 6.5e8 exponentials: 236
 // us, 1.5 times what the special-function units need; 32 tokens over 1000 to 8192 keys of 8 heads,
-// 235 MB: 58 us (4.1 TB/s).  A polynomial for some of the exponentials did not help (289 to 328 us
+// 235 MB: 53 us (4.4 TB/s).  A polynomial for some of the exponentials did not help (289 to 328 us
 // where none took 292, before there were two threads per key).
 #include "paged_tc.cuh"
 
@@ -30,11 +30,11 @@ constexpr int kMassThreads = 640;
 template <int HD>
 struct MassSmem {
   static constexpr int kTile = HD / 64 * kPagedBox;      // 128 rows
-  static constexpr int kStages = 3;                      // of keys, of queries
+  static constexpr int kKeys = 4, kQueries = 2;          // stages of keys, of queries
   static constexpr int kRows = 4;                        // stages of lse
-  static constexpr int k = 0;                            // [kStages][kTile]
-  static constexpr int q = k + kStages * kTile;          // [kStages][kTile]
-  static constexpr int lse = q + kStages * kTile;        // [kRows][128] floats
+  static constexpr int k = 0;                            // [kKeys][kTile]
+  static constexpr int q = k + kKeys * kTile;            // [kQueries][kTile]
+  static constexpr int lse = q + kQueries * kTile;        // [kRows][128] floats
   static constexpr int half = lse + kRows * 512;         // [2 blocks][2][128] sums of rows 64-127
   static constexpr int bars = half + 4 * 512;
   static constexpr int bytes = bars + 256 + 1024;        // + alignment of the base
@@ -55,16 +55,16 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     paged_mass_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       PagedMassParams p) {
   typedef MassSmem<HD> L;
-  constexpr int KCH = HD / 64, NS = L::kStages, NR = L::kRows;
+  constexpr int KCH = HD / 64, NK = L::kKeys, NQ = L::kQueries, NR = L::kRows;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                        ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bars);
-  uint64_t* k_full = bars;                               // [NS]
-  uint64_t* k_empty = bars + NS;                         // [NS]
-  uint64_t* q_full = bars + 2 * NS;                      // [NS]
-  uint64_t* q_empty = bars + 3 * NS;                     // [NS]
-  uint64_t* r_full = bars + 4 * NS;                      // [NR]
+  uint64_t* k_full = bars;                               // [NK]
+  uint64_t* k_empty = bars + NK;                         // [NK]
+  uint64_t* q_full = bars + 2 * NK;                      // [NQ]
+  uint64_t* q_empty = q_full + NQ;                       // [NQ]
+  uint64_t* r_full = q_empty + NQ;                       // [NR]
   uint64_t* r_empty = r_full + NR;                       // [NR]
   uint64_t* s_full = r_empty + NR;                       // [2 blocks][2 buffers]
   uint64_t* s_empty = s_full + 4;
@@ -76,9 +76,11 @@ __global__ void __launch_bounds__(kMassThreads, 1)
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
-    for (int s = 0; s < NS; ++s) {
+    for (int s = 0; s < NK; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < NQ; ++s) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 1);
     }
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     fence_mbar_init();
   }
   // rows of a query tile past its G * tokens are never loaded: their scores must be finite
-  for (int i = threadIdx.x; i < NS * L::kTile / 16; i += kMassThreads)
+  for (int i = threadIdx.x; i < NQ * L::kTile / 16; i += kMassThreads)
     reinterpret_cast<uint4*>(sm + L::q)[i] = make_uint4(0, 0, 0, 0);
   fence_async_shared();
   if (warp == 1) {
@@ -113,38 +115,51 @@ __global__ void __launch_bounds__(kMassThreads, 1)
   bool ok = true;
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
-    for (int it = first; ok && it < last; ++it) {
-      const PagedMassItem m = p.items[it];
+    // one item ahead: its record, and the pages of its two blocks
+    struct Pair {
+      KeyPages a, b;
+      bool has_a, has_b;
+    };
+    auto pages = [&](const PagedMassItem& m) {
       const PagedMask mask{p.block, p.window, p.sinks, m.q_len, m.kv_len};
       PagedItem w{};
       w.seq = m.seq;
-      w.kvh = m.kvh;
-      for (int x = m.i0; ok && x < m.i1; ++x, ++qn) {
-        if (x == m.i0)
-          for (int kb = m.kb0; ok && kb < m.kb0 + kMassBlocks; ++kb) {
-            const PagedRange range = mask.block_range(kb);
-            if (kb * kPagedKB >= m.kv_len || range.hi == 0) continue;
-            const uint32_t s = kn % NS;
-            ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[s], ((kn / NS) & 1) ^ 1, p.err, abort_flag));
-            if (!ok) break;
-            load_key_block(sm + L::k + s * L::kTile, &tmK, &k_full[s], KeyPages(p.pool, w, range, kb, KCH, lane, p.err),
-                           m.kvh, lane);
-            ++kn;
-          }
-        const uint32_t s = qn % NS;
-        ok = ok && __all_sync(0xffffffffu, wait_or_abort(&q_empty[s], ((qn / NS) & 1) ^ 1, p.err, abort_flag));
+      const bool second = (m.kb0 + 1) * kPagedKB < m.kv_len;
+      const PagedRange ra = mask.block_range(m.kb0), rb = second ? mask.block_range(m.kb0 + 1) : PagedRange{0, 0, 0};
+      return Pair{KeyPages(p.pool, w, ra, m.kb0, KCH, lane, p.err), KeyPages(p.pool, w, rb, m.kb0 + 1, KCH, lane, p.err),
+                  ra.hi > 0, rb.hi > 0};
+    };
+    auto load_keys = [&](const KeyPages& k, int kvh) {
+      const uint32_t s = kn % NK;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[s], ((kn / NK) & 1) ^ 1, p.err, abort_flag));
+      if (!ok) return;
+      load_key_block(sm + L::k + s * L::kTile, &tmK, &k_full[s], k, kvh, lane);
+      ++kn;
+    };
+    PagedMassItem m = p.items[first < last ? first : 0];
+    Pair now = pages(m);
+    for (int it = first; ok && it < last; ++it) {
+      const PagedMassItem next = p.items[it + 1 < last ? it + 1 : it];
+      if (now.has_a) load_keys(now.a, m.kvh);
+      if (ok && now.has_b) load_keys(now.b, m.kvh);
+      for (int x = m.i0; ok && x < m.i1; ++x) {
+        const uint32_t s = qn % NQ;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[s], ((qn / NQ) & 1) ^ 1, p.err, abort_flag));
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&q_full[s], KCH * tq * p.G * 128);
         __syncwarp();
         if (lane < KCH)
           tma_load_3d(sm + L::q + s * L::kTile + lane * kPagedBox, &tmQ, &q_full[s], lane * 64, m.kvh * p.G,
                       m.q0 + m.t0 + x * tq);
+        ++qn;
       }
+      m = next;
+      now = pages(m);
     }
     if (!ok && lane == 0) {                              // no load may be in flight at exit
       *abort_flag = 1;
-      for (uint32_t x = kn > NS ? kn - NS : 0; x < kn; ++x) mbar_wait(&k_full[x % NS], (x / NS) & 1, p.err);
-      for (uint32_t x = qn > NS ? qn - NS : 0; x < qn; ++x) mbar_wait(&q_full[x % NS], (x / NS) & 1, p.err);
+      for (uint32_t x = kn > NK ? kn - NK : 0; x < kn; ++x) mbar_wait(&k_full[x % NK], (x / NK) & 1, p.err);
+      for (uint32_t x = qn > NQ ? qn - NQ : 0; x < qn; ++x) mbar_wait(&q_full[x % NQ], (x / NQ) & 1, p.err);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
@@ -159,18 +174,18 @@ __global__ void __launch_bounds__(kMassThreads, 1)
 #pragma unroll
         for (int y = 0; ok && y < 2; ++y) {
           if (blk[y].f >= blk[y].l) continue;
-          ks[y] = kn % NS;
-          ok = wait_or_abort(&k_full[ks[y]], (kn / NS) & 1, p.err, abort_flag);
+          ks[y] = kn % NK;
+          ok = wait_or_abort(&k_full[ks[y]], (kn / NK) & 1, p.err, abort_flag);
           k_lo[y] = ((smem_u32(sm + L::k) + ks[y] * L::kTile) >> 4) | (1u << 16);
           ++kn;
         }
         for (int x = m.i0; ok && x < m.i1; ++x, ++qn) {
-          const uint32_t s = qn % NS;
+          const uint32_t s = qn % NQ;
           const int t = m.t0 + x * tq, t_end = min(t + tq, m.t1);
           const int cols = ((t_end - t) * p.G + 15) / 16 * 16;
           const uint32_t id = idesc_bf16(128, 16) + (static_cast<uint32_t>(cols / 8 - 2) << 17);
           const uint32_t q_lo = ((smem_u32(sm + L::q) + s * L::kTile) >> 4) | (1u << 16);
-          ok = wait_or_abort(&q_full[s], (qn / NS) & 1, p.err, abort_flag);
+          ok = wait_or_abort(&q_full[s], (qn / NQ) & 1, p.err, abort_flag);
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             if (!ok || !blk[y].meets(t, t_end)) continue;

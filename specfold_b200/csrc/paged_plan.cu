@@ -32,6 +32,11 @@ int64_t up4(int64_t x) { return (x + 3) & ~int64_t{3}; }
 // single tokens, small blocks), two of them (long ones).  fp32: 16 and 64 rows.
 struct Tiling {
   int rows[2], tokens[2], per_tile[2], workers[2], mass_workers, mass_rows;
+  // A tile of at most `whole` key blocks is not cut where every tile can have a CTA: pieces need a
+  // second launch for their join, which costs about what that many blocks take.  (One token over 7
+  // blocks of 2 kv heads: 11.0 us on the device in 14 pieces, 18.2 in two, 2 us a block; the join's
+  // launch takes the host 3 us.)
+  int whole[2];
 };
 Tiling tiling(const sf_paged_plan& p) {
   const int G = p.H / p.Hkv;
@@ -45,6 +50,8 @@ Tiling tiling(const sf_paged_plan& p) {
     t.workers[0] = t.workers[1] = p.sms;
     t.mass_workers = p.sms;
     t.mass_rows = 128;
+    t.whole[0] = 4;
+    t.whole[1] = 3;
     return t;
   }
   t.rows[0] = 16;
@@ -56,6 +63,8 @@ Tiling tiling(const sf_paged_plan& p) {
   t.workers[0] = t.workers[1] = 2 * p.sms;
   t.mass_workers = 2 * p.sms;
   t.mass_rows = 64;
+  t.whole[0] = 4;
+  t.whole[1] = 2;
   return t;
 }
 
@@ -103,13 +112,25 @@ struct Cut {
 
 // Deals things out in order: each worker takes its share of their units (and `extra` per thing),
 // and what does not fit goes on with the next one.
-void deal(const std::vector<int>& units, int extra, int workers, std::vector<Piece>* pieces,
+void deal(const std::vector<int>& units, int extra, int workers, int whole, std::vector<Piece>* pieces,
           std::vector<int32_t>* first, std::vector<Cut>* cuts, int* slots) {
   int64_t total = 0;
-  for (int u : units) total += u + extra;
+  int top = 0;
+  for (int u : units) {
+    total += u + extra;
+    top = std::max(top, u);
+  }
+  *slots = 0;
+  if (static_cast<int64_t>(units.size()) <= workers && top <= whole) {
+    for (size_t x = 0; x < units.size(); ++x) {
+      first->push_back(static_cast<int32_t>(x));
+      pieces->push_back({static_cast<int>(x), 0, units[x], -1});
+    }
+    first->push_back(static_cast<int32_t>(units.size()));
+    return;
+  }
   const int64_t w = std::max<int64_t>(1, std::min<int64_t>(workers, total));
   first->push_back(0);
-  *slots = 0;
   int64_t done = 0, worker = 0;   // dealt out; this worker's share ends at (worker + 1) * total / w
   for (size_t x = 0; x < units.size(); ++x) {
     int at = 0, n = 0;
@@ -296,7 +317,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       for (const PagedItem& it : tiles) l.max_rows = std::max(l.max_rows, it.ntok * G);
       if (!tiles.empty()) {
         int slots = 0;
-        deal(units, 1, t.workers[k], &pieces, &first, &cuts, &slots);
+        deal(units, 1, t.workers[k], t.whole[k], &pieces, &first, &cuts, &slots);
         l.slots = slots;
         l.n_items = static_cast<int32_t>(pieces.size());
         l.workers = static_cast<int32_t>(first.size()) - 1;
@@ -361,7 +382,7 @@ int sf_paged_plan_build(sf_paged_plan* plan, const int32_t* q_lens, const int32_
       if (!pairs.empty()) {
         int slots = 0;
         // loading two key blocks takes about as long as two tiles
-        deal(units, 2, t.mass_workers, &pieces, &first, &cuts, &slots);
+        deal(units, 2, t.mass_workers, 1, &pieces, &first, &cuts, &slots);
         l.slots = slots;
         l.n_items = static_cast<int32_t>(pieces.size());
         l.workers = static_cast<int32_t>(first.size()) - 1;
