@@ -59,7 +59,7 @@ cudaError_t launch_paged_append(int dtype, const PagedAppendParams& p, cudaStrea
 // the weights' order-preserving bits (11, 11 and 10 of them) finds the m-th largest value and
 // how many of its equals are taken; a count over the positions then places every survivor.
 //
-// Measured: 8200 keys of 4 heads of 24 sequences, 21 us; 32768 keys of 8 heads, 22 us (the weights
+// Measured: 8200 keys of 4 heads of 24 sequences, 16 us; 32768 keys of 8 heads, 19 us (the weights
 // are 3 and 1 MB: it is the latency of three passes, each a count, a cluster barrier and a scan).
 // One CTA per head that read the weights again in every pass took 55 us for the longer.
 //
@@ -156,25 +156,16 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(PagedEvictPar
   for (int pass = 0; pass < 3; ++pass) {
     uint32_t* mine = hist[pass & 1];
     const uint32_t field = (1u << bits[pass]) - 1;
-    // equal bins of a warp are counted together: a heavy tail has few leading bits
+    // (counting equal bins of a warp together first was slower: 21 us for the selection, 16 without)
     auto count = [&](uint32_t k, bool live) {
-      live = live && (k & mask) == prefix;
-      const unsigned who = __ballot_sync(0xffffffffu, live);
-      if (!live) return;
-      const uint32_t bin = (k >> shifts[pass]) & field;
-      const unsigned same = __match_any_sync(who, bin);
-      if (lane == __ffs(same) - 1) atomicAdd(&mine[bin], __popc(same));
+      if (live && (k & mask) == prefix) atomicAdd(&mine[(k >> shifts[pass]) & field], 1u);
     };
 #pragma unroll
     for (int j = 0; j < kSelKeys; ++j)
-      if (j < turns) {
-        count(held[j], begin + j * kSelThreads + threadIdx.x < end);
-        __syncwarp();
-      }
+      if (j < turns) count(held[j], begin + j * kSelThreads + threadIdx.x < end);
     for (int j = kSelKeys; j < turns; ++j) {
       const int i = begin + j * kSelThreads + threadIdx.x;
       count(i < end ? read(i) : 0, i < end);
-      __syncwarp();
     }
     cluster.sync();                                      // every CTA's counts are there
     // thread t owns bins 2047 - 2t and 2046 - 2t: a scan from the largest bin down
@@ -354,7 +345,7 @@ __global__ void __launch_bounds__(256) paged_move_kernel(PagedEvictParams p) {
 cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_t st) {
   if (p.B == 0) return cudaSuccess;
   // CTAs of a cluster: at most 2 keys a thread, as long as all clusters run side by side (a CTA
-  // fills an SM: for 96 heads of 8200 keys the selection took 25 us with two CTAs each, 21 with one)
+  // fills an SM: for 96 heads of 8200 keys the selection took 4 us more with two CTAs each than with one)
   const int stay = p.max_len < p.max_keep ? p.max_len : p.max_keep;
   int C = 1;
   while (C < 8 && p.max_len > C * 2 * kSelThreads && 2 * C * p.B * p.Hkv <= p.sms) C *= 2;
