@@ -89,7 +89,7 @@ struct ChunkSmem {
   static constexpr int ring = q + 2 * kTile;             // [kStages][kTile]
   static constexpr int ml = ring + kStages * kTile;      // [2 tiles][m (log2 units), l][128]
   static constexpr int bars = ml + 2 * 2 * 128 * 4;
-  static constexpr int bytes = bars + (2 * kStages + 24) * 8 + 8;
+  static constexpr int bytes = bars + (2 * kStages + 26) * 8 + 8;
 };
 
 template <int HD>
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int KCH = HD / 64, NS = L::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bars);
-  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 24);
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 26);
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
   if (smem_u32(sm) & 1023) {                             // the swizzled tiles need it; all threads see it
     flag_error(p.err, SF_DEV_ERR_TMEM);
@@ -114,10 +114,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* o_free = q_full + 6;
   uint64_t* ml_full = q_full + 8;
   uint64_t* ml_free = q_full + 10;
-  uint64_t* pv_done = q_full + 12;
-  uint64_t* drain = q_full + 14;
-  uint64_t* s_full = q_full + 16;                        // [2 tiles][2 halves]
-  uint64_t* p_full = q_full + 20;
+  uint64_t* drain = q_full + 12;
+  uint64_t* s_full = q_full + 14;                        // [2 tiles][2 halves]
+  uint64_t* p_full = q_full + 18;
+  uint64_t* pv_done = q_full + 22;
 
   pdl_trigger();                                         // the join of cut tiles may line up
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -132,10 +132,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
-      mbar_init(&pv_done[t], 1);
       for (int h = 0; h < 2; ++h) {
         mbar_init(&s_full[2 * t + h], 1);
         mbar_init(&p_full[2 * t + h], 4);
+        mbar_init(&pv_done[2 * t + h], 1);
       }
       mbar_init(&o_done[t], 1);
       mbar_init(&drain[t], 1);
@@ -240,9 +240,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           umma_f16_ts(tO, tS + h * 64 + kk * 8, desc(v_lo + kk * 128), id_pv, (!due_begin || h > 0 || kk > 0) ? 1u : 0u);
         return true;
       };
+      // Ahead of what half h commits: the last P V of the other half that was committed must be seen
+      // to be done, so that a softmax warp that has this half's scores finds its barrier at most one
+      // phase behind.  (That P V came before the products just issued, which hide the wait.)
+      auto settle = [&](int h) -> bool {
+        return wait(&pv_done[2 * t + (h ^ 1)], h == 1 && due_stage != NS ? par : par ^ 1);
+      };
       // after an item's last block O is done; the stage of V is free
       auto commit_pv = [&](int h) {
-        umma_commit(&pv_done[t]);
+        umma_commit(&pv_done[2 * t + h]);
         if (h == 0) return;
         umma_commit(&empty[due_stage]);
         if (due_end) umma_commit(&o_done[t]);
@@ -271,6 +277,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               for (int kk = 0; kk < HD / 16; ++kk)
                 umma_f16(tS + h * 64, desc(q_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2),
                          desc(k_lo + (kk >> 2) * (kPagedBox >> 4) + (kk & 3) * 2), id_s, kk > 0 ? 1u : 0u);
+            }
+            ok = settle(h);
+            if (!ok) break;
+            if (active) {
               umma_commit(&s_full[2 * t + h]);
               if (h == 1) {
                 umma_commit(&empty[stage]);
@@ -430,8 +440,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             l *= alpha;
             if (valid && !(mx < INFINITY)) l = NAN;      // an infinite or NaN score in the row
             if (i > w.i0 || half > 0) {
-              // the P V of the half before, the last to add to O, must be done
-              wait_or_abort(&pv_done[t], half ^ 1, p.err, &abort_flag);
+              // the P V of the half before, the last to add to O, must be done: phase n of the first
+              // half's barrier, n - 1 of the second's.  The parity means no other: the phase before was
+              // over when these scores were committed (settle), the one after needs this row's P.
+              wait_or_abort(&pv_done[2 * t + (half ^ 1)], (n & 1) ^ half ^ 1, p.err, &abort_flag);
               __syncwarp();
               tc_fence_after();
 #pragma unroll 1

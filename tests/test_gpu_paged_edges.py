@@ -1,0 +1,140 @@
+"""The paged cache's kernels where their pipelines and their inputs have edges: steps of many key
+blocks and items against the definitions in float64 on the device."""
+import math
+
+import pytest
+import torch
+
+from specfold_b200 import kernels as K
+from tests.paged_reference import U32, UB, UW
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+class Step:
+    """One step's inputs on the device.  Pages are dealt in no order; ``q``, ``k[b]`` and ``v[b]``
+    (rows of sequence b, in order) may be changed before ``pages()`` is called."""
+
+    def __init__(self, q_lens, kv_lens, H, Hkv, hd=128, ps=64, dtype=BF, block=1, window=0, sinks=0, seed=0):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.q_lens, self.kv_lens, self.H, self.Hkv, self.hd, self.ps = q_lens, kv_lens, H, Hkv, hd, ps
+        self.dtype, self.block, self.window, self.sinks, self.scale = dtype, block, window, sinks, hd ** -0.5
+        self.q = torch.randn(sum(q_lens), H, hd, generator=g, device="cuda").to(dtype)
+        self.k = [torch.randn(n, Hkv, hd, generator=g, device="cuda").to(dtype) for n in kv_lens]
+        self.v = [torch.randn(n, Hkv, hd, generator=g, device="cuda").to(dtype) for n in kv_lens]
+        need = [-(-n // ps) for n in kv_lens]
+        order = torch.randperm(sum(need) + 1, generator=g, device="cuda").to(torch.int32)
+        self.table = torch.full((len(kv_lens), max(need + [1])), -1, dtype=torch.int32, device="cuda")
+        at = 0
+        for b, m in enumerate(need):
+            self.table[b, :m] = order[at:at + m]
+            at += m
+        self.num_pages = sum(need) + 1
+
+    def pages(self):
+        """(k_pages, v_pages); slots that hold no key are NaN."""
+        out = []
+        for rows in (self.k, self.v):
+            p = torch.full((self.num_pages, self.Hkv, self.ps, self.hd), math.nan, dtype=self.dtype, device="cuda")
+            for b, r in enumerate(rows):
+                j = torch.arange(len(r), device="cuda")
+                p[self.table[b, j // self.ps].long(), :, j % self.ps] = r
+            out.append(p)
+        return out
+
+    def plan(self, **kw):
+        return K.PagedPlan(self.q_lens, self.kv_lens, heads=self.H, kv_heads=self.Hkv, head_dim=self.hd,
+                           page_size=self.ps, dtype=self.dtype, block=self.block, window=self.window,
+                           sinks=self.sinks, **kw)
+
+    def sees(self, b):
+        """[q_len, kv_len]: which keys each token of sequence b sees"""
+        q, n = self.q_lens[b], self.kv_lens[b]
+        i, j = torch.arange(q, device="cuda")[:, None], torch.arange(n, device="cuda")
+        see = (j < n - q + (i // self.block + 1) * self.block) if self.block else (j < n).expand(q, n)
+        if self.window:
+            see = see & ((j > n - q + i - self.window) | (j < self.sinks))
+        return see
+
+    def exact(self):
+        """(out, lse, bound on out, bound on lse) in float64; the bounds as in paged_reference."""
+        T, G, bf = sum(self.q_lens), self.H // self.Hkv, self.dtype == BF
+        out = torch.zeros(T, self.H, self.hd, dtype=torch.float64, device="cuda")
+        lse = torch.full((T, self.H), -math.inf, dtype=torch.float64, device="cuda")
+        tol_o, tol_l = torch.zeros_like(out), torch.zeros_like(lse)
+        t0 = 0
+        for b, ql in enumerate(self.q_lens):
+            see, rows = self.sees(b), slice(t0, t0 + ql)
+            t0 += ql
+            some = see.any(1)
+            for h in range(self.H):
+                q, k, v = self.q[rows, h].double(), self.k[b][:, h // G].double(), self.v[b][:, h // G].double()
+                s = (q @ k.T * self.scale).masked_fill(~see, -math.inf)
+                top = s.amax(1, keepdim=True).masked_fill(~some[:, None], 0)
+                w = (s - top).exp()
+                z = w.sum(1, keepdim=True)
+                w = w / z.clamp(min=1e-300)
+                fin = v.isfinite()
+                o = w @ v.masked_fill(~fin, 0)
+                # a value that is not finite decides its column for the tokens that see it
+                x = see.double()
+                pos, neg, nan = (x @ m.double() > 0 for m in (v == math.inf, v == -math.inf, v.isnan()))
+                o = o.masked_fill(pos, math.inf).masked_fill(neg, -math.inf).masked_fill(nan | (pos & neg), math.nan)
+                out[rows, h] = o
+                lse[rows, h] = torch.where(some, (top + z.log())[:, 0], -math.inf)
+                e = self.hd * U32 * self.scale * (q.abs() @ k.abs().T).masked_fill(~see, 0).amax(1)
+                e += 8 * U32 * s.abs().masked_fill(~see, 0).amax(1) + see.sum(1) * U32
+                a = w @ v.masked_fill(~fin, 0).abs()
+                tol_o[rows, h] = (2 * e + (2 * UW + 2.1 * UB if bf else 4 * U32))[:, None] * a
+                tol_l[rows, h] = e + (UW if bf else 4 * U32) + 4 * U32 * lse[rows, h].abs().masked_fill(~some, 0)
+        return out, lse, tol_o, tol_l
+
+
+def within(got, want, tol, what):
+    got = got.double()
+    fin = want.isfinite()
+    assert torch.equal(got.isfinite(), fin), f"{what}: finite elsewhere"
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf]), f"{what}: infinities differ"
+    over = ((got - want).abs() - tol)[fin]
+    assert over.numel() == 0 or float(over.max()) <= 0, f"{what}: {float(over.max()):.3e} over its bound"
+
+
+# ---------------------------------------------------------------------------- rescaled accumulators
+def check_repeatedly(st, what, times=40):
+    """Against float64, and the same bits every time."""
+    k, v = st.pages()
+    plan = st.plan()
+    first = K.paged_attention(st.q, k, v, st.table, plan)
+    o, l, tol_o, tol_l = st.exact()
+    within(first[0], o, tol_o, f"{what}: out")
+    within(first[1], l, tol_l, f"{what}: lse")
+    same = torch.ones((), dtype=torch.bool, device="cuda")
+    for _ in range(times):
+        again = K.paged_attention(st.q, k, v, st.table, plan)
+        same &= (again[0] == first[0]).all() & (again[1] == first[1]).all()
+    plan.check()
+    assert bool(same), what
+
+
+@pytest.mark.parametrize("hd", [128, 64])
+def test_rows_that_outgrow_their_reference(hd):
+    """One head's scores rise by more than 2^60 from each half block to the next, so that its rows
+    move their reference and rescale what they have accumulated in every half; the rows beside
+    them do not, and must lose nothing."""
+    st = Step([64, 128], [1600, 1400], 8, 2, hd=hd, seed=1)
+    for k in st.k:
+        # 64 keys further on, 80 more: 50 nats (72 powers of two) at a scaled query of 8
+        k[:, :, 0] = (torch.arange(len(k), device="cuda") * (80 / 64))[:, None].to(k.dtype)
+    st.q[:, :, 0] = 0
+    st.q[:, [1, 6], 0] = 50 / 80 * hd ** 0.5
+    check_repeatedly(st, "growing scores")
+
+
+@pytest.mark.parametrize("window,sinks,block", [(24, 0, 1), (70, 3, 1), (5, 200, 1), (40, 0, 32)])
+def test_windows_narrower_than_a_tile(window, sinks, block):
+    """Rows of a tile see their first key in different half blocks."""
+    st = Step([256, 128], [1500, 900], 8, 2, window=window, sinks=sinks, block=block, seed=2)
+    check_repeatedly(st, "narrow window")
