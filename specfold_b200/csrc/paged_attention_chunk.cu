@@ -403,17 +403,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       float m = -INFINITY, l = 0.f;
       for (int i = w.i0; i < w.i1; ++i, ++n, ++x) {
         const int k0 = w.block(i) * kPagedKB;
-        // the keys of this block that no row sees hold whatever their pages do: weight 0 times
-        // that must be 0 (thread r clears row r of V; others that do write the same zeros)
-        if ((k0 < range.lo || k0 + kPagedKB > range.hi) && !range.has(k0 + r)) {
-          const uint32_t u = 2 * x + 1;
-          wait_or_abort(&full[u % NS], (u / NS) & 1, p.err, &abort_flag);
-          unsigned char* row = sm + L::ring + (u % NS) * L::kTile + r * 128;
+        // The keys of this block that no row sees hold whatever their pages do: weight 0 times that
+        // must be 0 (thread r clears row r of V; the other tile's writes the same zeros).  Not before
+        // this block's scores are there: tile 1 skips items, and until its issuing warp has come this
+        // far the parity may name an earlier use of the stage.
+        if (k0 < range.lo || k0 + kPagedKB > range.hi) {
+          ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * t], n & 1, p.err, &abort_flag));
+          if (!ok) break;
+          if (!range.has(k0 + r)) {
+            const uint32_t u = 2 * x + 1;
+            wait_or_abort(&full[u % NS], (u / NS) & 1, p.err, &abort_flag);
+            unsigned char* row = sm + L::ring + (u % NS) * L::kTile + r * 128;
 #pragma unroll
-          for (int c = 0; c < KCH; ++c)
+            for (int c = 0; c < KCH; ++c)
 #pragma unroll
-            for (int y = 0; y < 8; ++y) *reinterpret_cast<uint4*>(row + c * kPagedBox + y * 16) = make_uint4(0, 0, 0, 0);
-          fence_async_shared();
+              for (int y = 0; y < 8; ++y) *reinterpret_cast<uint4*>(row + c * kPagedBox + y * 16) = make_uint4(0, 0, 0, 0);
+            fence_async_shared();
+          }
         }
         const bool edge = k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks);
 #pragma unroll 1

@@ -138,3 +138,15 @@ def test_windows_narrower_than_a_tile(window, sinks, block):
     """Rows of a tile see their first key in different half blocks."""
     st = Step([256, 128], [1500, 900], 8, 2, window=window, sinks=sinks, block=block, seed=2)
     check_repeatedly(st, "narrow window")
+
+
+# ---------------------------------------------------------------------------- many items a CTA
+@pytest.mark.parametrize("hd,window,sinks", [(128, 100, 4), (128, 0, 0), (64, 300, 0), (64, 0, 0)])
+def test_ragged_chunks_whose_last_tiles_are_half_empty(hd, window, sinks):
+    """Chunks that end within the first half of a tile pair, several of them in every CTA's share:
+    the pair's second tile sits an item out and begins the next one with keys that no row sees."""
+    g = torch.Generator().manual_seed(hd + window)
+    q = (70 + 64 * torch.randint(0, 3, (48,), generator=g) + torch.randint(0, 20, (48,), generator=g)).tolist()
+    n = [x + int(m) for x, m in zip(q, torch.randint(0, 700 if window else 40, (48,), generator=g))]
+    st = Step(q, n, 32, 8, hd=hd, ps=32, window=window, sinks=sinks, seed=3)
+    check_repeatedly(st, "half-empty tiles")
