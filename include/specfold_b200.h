@@ -397,7 +397,8 @@ typedef struct sf_paged_pool {
 } sf_paged_pool;
 
 /* The new rows of every sequence into its pages, at positions [kv_len - q_len, kv_len);
- * mass_pages, when not NULL, is zeroed there.  k_new / v_new [T][Hkv][hd] with the given token
+ * mass_pages, when not NULL, is zeroed there.  Sequences may share pages, but not those of
+ * their new positions.  k_new / v_new [T][Hkv][hd] with the given token
  * and head strides (elements, 16-byte multiples, alike for both). */
 int sf_paged_kv_append(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* k_new,
                        const void* v_new, int64_t new_tok_stride, int64_t new_head_stride,
@@ -410,8 +411,11 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
                        float scale, void* stream);
 
 /* mass[key] += sum over the tokens that see it and the query heads of its kv head of
- * exp(scale * q . k - lse), lse as sf_paged_attention wrote it.  Each weight is summed in one
- * place in a fixed order: the same inputs give the same bits. */
+ * exp(scale * q . k - lse), lse as sf_paged_attention wrote it.  A sequence's weight for a key
+ * is summed in one place in a fixed order and added in one piece: the same inputs give the same
+ * bits.  A page that several of the step's sequences hold (a shared prefix) gets the weights of
+ * all of them; the order in which they are added, and with it the last bits, may then differ
+ * from call to call. */
 int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool, const void* q,
                             int64_t q_tok_stride, int64_t q_head_stride, const float* lse,
                             float scale, void* stream);

@@ -297,19 +297,20 @@ cudaError_t launch_paged_attention_simt(const PagedAttnParams& p, cudaStream_t s
 }
 
 // ------------------------------------------------------------------ weight accumulation
-// a key's accumulated weight; a page outside the pool is flagged, and nothing is written
+// A key's accumulated weight; a page outside the pool is flagged, and nothing is written.  Atomic:
+// sequences that share the page add to it at the same time.
 __device__ __forceinline__ void add_mass(const PagedMassParams& p, int seq, int kvh, int key, float sum) {
   const int page = p.pool.table[seq * p.pool.table_stride + (key >> p.pool.page_shift)];
   if (page < 0 || page >= p.pool.num_pages) {
     flag_error(p.err, SF_DEV_ERR_INDEX);
     return;
   }
-  p.pool.mass[ ((static_cast<int64_t>(page) * p.Hkv + kvh) << p.pool.page_shift) +
-              (key & ((1 << p.pool.page_shift) - 1))] += sum;
+  atomicAdd(&p.pool.mass[((static_cast<int64_t>(page) * p.Hkv + kvh) << p.pool.page_shift) +
+                         (key & ((1 << p.pool.page_shift) - 1))], sum);
 }
 
 // A key's weight over all rows that see it: sum of exp(s - lse).  A CTA owns a key block and
-// walks the query rows, so each weight is summed in one place, in one order, without atomics.
+// walks the query rows, so each weight is summed in one place, in one order, and added once.
 template <typename T, int HD, int RM>
 __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedMassParams p) {
   constexpr int R = 16 * RM, LD = HD + 4;

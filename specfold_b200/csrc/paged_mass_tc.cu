@@ -4,7 +4,8 @@
 // The scores are computed transposed, S^T = K Q^T with the 128 keys of a block as the rows of the
 // MMA, so that a key is a TMEM lane: a thread adds up its own key's weights over the columns (the
 // query rows), tile after tile, in registers.  A weight is therefore summed in one place, in one
-// order, and written once; no atomics.  lse is a per-column constant: the exponent is one fma.
+// order, and added once (atomically: another sequence may hold the same page).  lse is a per-column
+// constant: the exponent is one fma.
 // A CTA works on two key blocks at a time, so that a query tile, which streams from L2, feeds two
 // products.  A pair whose tiles were cut between CTAs leaves its sums for the merge.
 //   warps 4-11, 12-19 exponentials and sums of the first and of the second block, two threads per
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     const uint64_t scale2 = pair(sl2, sl2);
     uint32_t bn = 0;                                     // this block's scores so far
     // One item ahead: which key is this thread's, the tokens that see it, and where its sum goes
-    // (the page id, then the weight so far, are on their way while the item before is worked on).
+    // (the page id is on its way while the item before is worked on).
     struct Ahead {
       PagedMassItem m;
       int f, l, id;                                      // tokens [f, l) see the key; its page
@@ -282,7 +283,6 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     };
     Ahead cur = begin(first < last ? first : 0);
     float* dst = target(cur);
-    float old = half == 0 && dst != nullptr && cur.m.slot < 0 ? *dst : 0.f;
     float* s_half = reinterpret_cast<float*>(sm + L::half) + y * 256;
     for (int it = first; it < last; ++it) {              // (to the end whatever fails: the halves meet)
       const PagedMassItem& m = cur.m;
@@ -343,16 +343,18 @@ __global__ void __launch_bounds__(kMassThreads, 1)
         }
       }
       float* next_dst = target(next);
-      const float next_old = half == 0 && it + 1 < last && next_dst != nullptr && next.m.slot < 0 ? *next_dst : 0.f;
       float a0, a1;
       unpair(add2(sum0, sum1), a0, a1);
       float* other = s_half + (it - first & 1) * 128 + r;  // two by turns: read while the next is written
       if (half == 1) *other = a0 + a1;
       asm volatile("bar.sync %0, 256;" ::"r"(1 + y) : "memory");
-      if (half == 0 && dst != nullptr && ok) *dst = old + (a0 + a1 + *other);
+      if (half == 0 && dst != nullptr && ok) {
+        const float sum = a0 + a1 + *other;
+        if (m.slot < 0) atomicAdd(dst, sum);
+        else *dst = sum;
+      }
       cur = next;
       dst = next_dst;
-      old = next_old;
     }
     if (!ok) *abort_flag = 1;
   }

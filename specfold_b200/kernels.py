@@ -470,7 +470,7 @@ def paged_kv_append(k_pages: torch.Tensor, v_pages: torch.Tensor, k_new: torch.T
                     mass_pages: Optional[torch.Tensor] = None) -> None:
     """The new tokens' keys and values [T, Hkv, hd] (strided rows, e.g. slices of a fused
     projection's output) into their sequences' pages (sf_paged_kv_append); their accumulated
-    weights start at zero."""
+    weights start at zero.  Sequences may share pages, but not those of their new positions."""
     pool = _paged_pool(k_pages, v_pages, table, mass_pages, plan, plan.dtype)
     tok, head = _paged_rows(k_new, plan.kv_heads, plan, "k_new")
     if _paged_rows(v_new, plan.kv_heads, plan, "v_new") != (tok, head):
@@ -507,7 +507,8 @@ def paged_attention_mass(q: torch.Tensor, k_pages: torch.Tensor, table: torch.Te
                          scale: Optional[float] = None) -> None:
     """Adds to every cached key's accumulated weight what the new tokens' softmax gave it,
     summed over tokens and the query heads of its kv head (sf_paged_attention_mass); ``lse`` is
-    paged_attention's."""
+    paged_attention's.  A page that several sequences of the step hold gets the weights of all
+    (whose order, and so the last bits, may then differ from call to call)."""
     pool = _paged_pool(k_pages, None, table, mass_pages, plan, plan.dtype)
     tok, head = _paged_rows(q, plan.heads, plan, "q")
     if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:

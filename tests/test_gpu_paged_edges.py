@@ -91,6 +91,27 @@ class Step:
                 tol_l[rows, h] = e + (UW if bf else 4 * U32) + 4 * U32 * lse[rows, h].abs().masked_fill(~some, 0)
         return out, lse, tol_o, tol_l
 
+    def exact_mass(self, lse, mass):
+        """(accumulated weights, bound) in float64 after the step's are added to ``mass``, from the
+        given lse; the bound as in paged_reference, its parts added up over a page's holders."""
+        G, acc = self.H // self.Hkv, mass.double()
+        off, adds, terms = (torch.zeros_like(acc) for _ in range(3))
+        t0 = 0
+        for b, ql in enumerate(self.q_lens):
+            see, rows, j = self.sees(b), slice(t0, t0 + ql), torch.arange(self.kv_lens[b], device="cuda")
+            t0 += ql
+            page, at = self.table[b, j // self.ps].long(), j % self.ps
+            for h in range(self.H if ql else 0):
+                q, k, ls = self.q[rows, h].double(), self.k[b][:, h // G].double(), lse[rows, h].double()[:, None]
+                x = q @ k.T * self.scale
+                w = (x - ls).exp().masked_fill(~see, 0)
+                e = self.hd * U32 * self.scale * (q.abs() @ k.abs().T) + 8 * U32 * (x.abs() + ls.abs()) + 8 * U32
+                where = (page, torch.full_like(page, h // G), at)
+                for into, what in ((adds, w.sum(0)), (off, (w * e).masked_fill(~see, 0).sum(0)), (terms, see.double().sum(0))):
+                    into.index_put_(where, what, accumulate=True)
+        tol = off + (terms + 2 * len(self.q_lens)) * U32 * (adds + acc.abs())
+        return acc + adds, tol.masked_fill(terms == 0, 0)
+
 
 def within(got, want, tol, what):
     got = got.double()
@@ -150,3 +171,34 @@ def test_ragged_chunks_whose_last_tiles_are_half_empty(hd, window, sinks):
     n = [x + int(m) for x, m in zip(q, torch.randint(0, 700 if window else 40, (48,), generator=g))]
     st = Step(q, n, 32, 8, hd=hd, ps=32, window=window, sinks=sinks, seed=3)
     check_repeatedly(st, "half-empty tiles")
+
+
+# ---------------------------------------------------------------------------- shared pages
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("q", [1, 40, 150])
+def test_weights_of_a_shared_prefix_add_up(dtype, q):
+    """Every sequence's table begins with the same pages; the weights that all of them give those keys
+    are there afterwards, those of a sequence's own pages in the same bits every time."""
+    B, shared, ps = 12, 10, 32
+    st = Step([q] * B, [400 + q + 13 * b for b in range(B)], 8, 2, ps=ps, dtype=dtype, seed=4)
+    st.table[:, :shared] = st.table[0, :shared]
+    for b in range(1, B):
+        st.k[b][:shared * ps], st.v[b][:shared * ps] = st.k[0][:shared * ps], st.v[0][:shared * ps]
+    k, v = st.pages()
+    plan = st.plan()
+    out, lse = K.paged_attention(st.q, k, v, st.table, plan)
+    o, l, tol_o, tol_l = st.exact()
+    within(out, o, tol_o, "out")
+    within(lse, l, tol_l, "lse")
+    start = torch.rand(k.shape[:3], generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    want, tol = st.exact_mass(lse, start)
+    own = torch.ones(len(k), dtype=torch.bool, device="cuda")
+    own[st.table[0, :shared].long()] = False
+    first = None
+    for _ in range(8):
+        mass = start.clone()
+        K.paged_attention_mass(st.q, k, st.table, lse, mass, plan)
+        within(mass, want, tol, "weights")
+        first = mass if first is None else first
+        assert torch.equal(mass[own], first[own])
+    plan.check()
