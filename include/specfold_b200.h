@@ -411,7 +411,9 @@ int sf_paged_attention(const sf_paged_plan* plan, const sf_paged_pool* pool, con
                        float scale, void* stream);
 
 /* mass[key] += sum over the tokens that see it and the query heads of its kv head of
- * exp(scale * q . k - lse), lse as sf_paged_attention wrote it.  A sequence's weight for a key
+ * exp(scale * q . k - lse), lse as sf_paged_attention wrote it (a token whose lse is
+ * -inf saw nothing and adds nothing; one whose lse is NaN makes the weights of the keys it sees
+ * NaN, and no others).  A sequence's weight for a key
  * is summed in one place in a fixed order and added in one piece: the same inputs give the same
  * bits.  A page that several of the step's sequences hold (a shared prefix) gets the weights of
  * all of them; the order in which they are added, and with it the last bits, may then differ

@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedM
             if (r >= rows) continue;
             const int i = t + r / p.G;
             const float lse = p.lse[static_cast<int64_t>(w.q0 + i) * p.H + w.kvh * p.G + r % p.G] * 1.4426950408889634f;
+            if (lse == -INFINITY) continue;               // a row that saw nothing gives nothing
             const int hi = mask.hi(i), lo = mask.lo(i);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {

@@ -37,7 +37,8 @@ struct MassSmem {
   static constexpr int q = k + kKeys * kTile;            // [kQueries][kTile]
   static constexpr int lse = q + kQueries * kTile;        // [kRows][128] floats
   static constexpr int half = lse + kRows * 512;         // [2 blocks][2][128] sums of rows 64-127
-  static constexpr int bars = half + 4 * 512;
+  static constexpr int odd = half + 4 * 512;             // [kRows] stages with a NaN lse
+  static constexpr int bars = odd + kRows * 4;
   static constexpr int bytes = bars + 256 + 1024;        // + alignment of the base
 };
 
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
   } else if (warp == 2) {
     // ---------------------------------------------------------------- lse of the rows
     float* s_lse = reinterpret_cast<float*>(sm + L::lse);
+    int* s_odd = reinterpret_cast<int*>(sm + L::odd);
     int tok[4], head[4];                                 // of this lane's four rows
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -233,11 +235,14 @@ __global__ void __launch_bounds__(kMassThreads, 1)
           v[j] = INFINITY;                               // a column that is no row: weight 0
           if (tok[j] < n)
             v[j] = p.lse[static_cast<int64_t>(m.q0 + t + tok[j]) * p.H + m.kvh * p.G + head[j]] * 1.4426950408889634f;
+          if (v[j] == -INFINITY) v[j] = INFINITY;        // a row that saw nothing gives nothing
         }
+        const bool odd = __any_sync(0xffffffffu, isnan(v[0]) || isnan(v[1]) || isnan(v[2]) || isnan(v[3]));
         ok = __all_sync(0xffffffffu, wait_or_abort(&r_empty[s], ((qn / NR) & 1) ^ 1, p.err, abort_flag));
         if (!ok) break;
 #pragma unroll
         for (int j = 0; j < 4; ++j) s_lse[s * 128 + lane + 32 * j] = -v[j];
+        if (lane == 0) s_odd[s] = odd;
         __syncwarp();
         if (lane == 0) mbar_arrive(&r_full[s]);
       }
@@ -248,6 +253,7 @@ __global__ void __launch_bounds__(kMassThreads, 1)
     const int y = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t tS = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + y * 256;
     const float* s_lse = reinterpret_cast<const float*>(sm + L::lse);
+    const int* s_odd = reinterpret_cast<const int*>(sm + L::odd);
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint64_t scale2 = pair(sl2, sl2);
     uint32_t bn = 0;                                     // this block's scores so far
@@ -326,12 +332,25 @@ __global__ void __launch_bounds__(kMassThreads, 1)
             }
           };
           const uint32_t tB = tS + b * 128;
+          const int c_end = min(rows, half * 64 + 64);
+          if (s_odd[s]) {                                // -inf + NaN is NaN: only the columns themselves
 #pragma unroll 1
-          for (int c = half * 64; c < min(rows, half * 64 + 64); c += 32) {
-            float v[32];
-            tmem_ld32(tB + c, v);
-            tmem_wait<32>(v);
-            add(v, c);
+            for (int c = half * 64; c < c_end; c += 8) {
+              float v[8];
+              tmem_ld8(tB + c, v);
+              tmem_wait<8>(v);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (c + j >= c_lo && c + j < c_hi) sum0 = add2(sum0, pair(ex2(fmaf(v[j], sl2, s_lse[s * 128 + c + j])), 0.f));
+            }
+          } else {
+#pragma unroll 1
+            for (int c = half * 64; c < c_end; c += 32) {
+              float v[32];
+              tmem_ld32(tB + c, v);
+              tmem_wait<32>(v);
+              add(v, c);
+            }
           }
           tc_fence_before();
           ++bn;

@@ -103,11 +103,12 @@ class Step:
             page, at = self.table[b, j // self.ps].long(), j % self.ps
             for h in range(self.H if ql else 0):
                 q, k, ls = self.q[rows, h].double(), self.k[b][:, h // G].double(), lse[rows, h].double()[:, None]
+                ls = ls.masked_fill(ls == -math.inf, math.inf)         # saw nothing: weight 0
                 x = q @ k.T * self.scale
                 w = (x - ls).exp().masked_fill(~see, 0)
                 e = self.hd * U32 * self.scale * (q.abs() @ k.abs().T) + 8 * U32 * (x.abs() + ls.abs()) + 8 * U32
                 where = (page, torch.full_like(page, h // G), at)
-                for into, what in ((adds, w.sum(0)), (off, (w * e).masked_fill(~see, 0).sum(0)), (terms, see.double().sum(0))):
+                for into, what in ((adds, w.sum(0)), (off, (w * e).masked_fill(~see | (w == 0), 0).sum(0)), (terms, see.double().sum(0))):
                     into.index_put_(where, what, accumulate=True)
         tol = off + (terms + 2 * len(self.q_lens)) * U32 * (adds + acc.abs())
         return acc + adds, tol.masked_fill(terms == 0, 0)
@@ -202,3 +203,26 @@ def test_weights_of_a_shared_prefix_add_up(dtype, q):
         first = mass if first is None else first
         assert torch.equal(mass[own], first[own])
     plan.check()
+
+
+# ---------------------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("window,block", [(0, 1), (0, 8), (30, 1)])
+def test_a_token_that_is_not_finite_spoils_the_keys_it_sees_only(dtype, window, block):
+    """Next to it in the tile are tokens that see other keys; a token whose lse is -inf adds nothing."""
+    st = Step([1, 90, 24], [150, 200, 170], 8, 2, ps=16, dtype=dtype, window=window, block=block, seed=5)
+    st.q[30, 5], st.q[100, 2, 7] = math.nan, math.inf
+    k, v = st.pages()
+    plan = st.plan()
+    out, lse = K.paged_attention(st.q, k, v, st.table, plan)
+    hit = torch.zeros(lse.shape, dtype=torch.bool, device="cuda")
+    hit[30, 5] = hit[100, 2] = True
+    assert torch.equal(lse.isnan(), hit) and torch.equal(out.isnan().all(2), hit) and torch.equal(out.isnan().any(2), hit)
+    lse[50, 1] = lse[0] = -math.inf
+    start = torch.rand(k.shape[:3], generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    mass = start.clone()
+    K.paged_attention_mass(st.q, k, st.table, lse, mass, plan)
+    plan.check()
+    want, tol = st.exact_mass(lse, start)
+    assert bool(want.isnan().any())
+    within(mass, want, tol, "weights")
