@@ -14,8 +14,9 @@
 // fill the 512 columns of TMEM.
 //
 // The softmax's reference need not be the running maximum: any value that no weight outgrows by
-// more than 2^60, and that is no larger than the true maximum, gives the same quotient O / l with
-// the same relative rounding.  So a row takes the maximum of the first half block that it sees a
+// more than 2^8, and that is no larger than the true maximum, gives the same quotient O / l with
+// the same relative rounding, and takes no more than 8 of the 128 powers of two that O has for
+// the values.  So a row takes the maximum of the first half block that it sees a
 // key of, and later halves only check their largest score against it; where a row outgrows it, the
 // reference moves and O is rescaled.
 //
@@ -54,9 +55,9 @@ __device__ __forceinline__ float max64(const float* v) {
   }
   return max3(max3(m[0], m[1], v[15]), max3(m[2], m[3], v[31]), max3(v[47], v[63], v[63]));
 }
-// How far a row may outgrow its reference (see the head of the file): weights up to 2^60, which
-// bf16 and the fp32 sums hold.
-constexpr float kGrowthLog2 = 60.f;
+// How far a row may outgrow its reference (see the head of the file).  (2^60 made O overflow for
+// values above 2^67 and was no faster.)
+constexpr float kGrowthLog2 = 8.f;
 
 // 2^x of a pair on the FMA and integer pipes: x = i + r with |r| <= 1/2, 2^r by the polynomial of
 // degree 4 with p(0) = 1 that is minimax in relative error on that interval (2.8e-6, found by
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           const float mx = max64(v) * sl2;
           if (!__all_sync(0xffffffffu, !valid || mx <= m + kGrowthLog2)) {
-            const bool grew = valid && !(mx <= m + 8.f);
+            const bool grew = valid && !(mx <= m + kGrowthLog2);
             const float alpha = grew ? ex2(m - mx) : 1.f;
             if (grew) m = mx;
             l *= alpha;

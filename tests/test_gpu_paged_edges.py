@@ -155,6 +155,18 @@ def test_rows_that_outgrow_their_reference(hd):
     check_repeatedly(st, "growing scores")
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_large_values_under_growing_scores(dtype):
+    """Scores that rise by 2^2 to 2^50 over the sequence, in steps of any size, and values near 2^100:
+    the accumulators hold them, whatever the softmax's reference was."""
+    st = Step([64, 128, 1, 20], [900, 1400, 3000, 500], 8, 2, dtype=dtype, seed=6)
+    for k in st.k:
+        k[:, :, 0] = (torch.arange(len(k), device="cuda") / len(k))[:, None].to(dtype)
+    st.v = [(v.float() * 2.0 ** 100).to(dtype) for v in st.v]
+    st.q[:, :, 0] = (torch.linspace(2, 50, 213, device="cuda") * math.log(2) * st.hd ** 0.5)[:, None].to(dtype)
+    check_repeatedly(st, "large values", times=5)
+
+
 @pytest.mark.parametrize("window,sinks,block", [(24, 0, 1), (70, 3, 1), (5, 200, 1), (40, 0, 32)])
 def test_windows_narrower_than_a_tile(window, sinks, block):
     """Rows of a tile see their first key in different half blocks."""
