@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int64_t row = tok * p.H + w.kvh * p.G + r % p.G;
         const int64_t prow = static_cast<int64_t>(w.slot) * p.rows + t * 128 + r;
         const float f = w.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        uint64_t finite = pair(0.f, 0.f);                // NaN where O is not
 #pragma unroll 1
         for (int c = 0; c < HD; c += 8) {
           float o[8];
@@ -349,6 +350,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (any) {
             tmem_ld8(tmem + 256 + t * 128 + lane_off + c, o);
             tmem_wait<8>(o);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) finite = fma2(pair(o[j], o[j + 1]), pair(0.f, 0.f), finite);
           }
           if (any && c + 8 == HD) {                      // O is read: the next item may begin
             tc_fence_before();
@@ -377,6 +380,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             p.part_ml[2 * prow + 1] = l;
           } else {
             p.lse[row] = m * 0.6931471805599453f + logf(l);
+          }
+        }
+        float f_even, f_odd;
+        unpair(finite, f_even, f_odd);
+        unsigned todo = __ballot_sync(0xffffffffu, r < rows && f_even + f_odd != 0.f && l < INFINITY);
+        if (todo != 0) {                                 // values that not all rows see?
+          const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
+          const int t0 = w.tok0 + t * tq, t1 = min(w.tok0 + w.ntok, t0 + tq);
+          if (!paged_odd_values<__nv_bfloat16, HD>(p, w, mask.range(w.tok0, w.tok0 + w.ntok), mask.hi(t0), mask.lo(t1 - 1), kPagedKB, lane))
+            todo = 0;
+          __syncwarp();                                  // the rows are read back
+          for (; todo != 0; todo &= todo - 1) {
+            const int x = __ffs(todo) - 1, rx = quarter * 32 + x;
+            paged_repair_row<__nv_bfloat16, HD>(p, w, t0 + rx / p.G, rx % p.G, __shfl_sync(0xffffffffu, m, x),
+                                                __shfl_sync(0xffffffffu, f, x),
+                                                static_cast<__nv_bfloat16*>(p.out) + __shfl_sync(0xffffffffu, row, x) * HD,
+                                                w.slot >= 0 ? p.part_O + __shfl_sync(0xffffffffu, prow, x) * HD : nullptr, kPagedKB, lane);
           }
         }
       }

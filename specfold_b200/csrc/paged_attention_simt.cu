@@ -212,10 +212,19 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
         }
       }
     }
+    unsigned odd = 0;                                   // this thread's rows whose O is not finite
 #pragma unroll
     for (int a = 0; a < RM; ++a) {
       const int r = ty + 16 * a;
       if (r >= rows) continue;
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float e0, e1;
+          unpair(o[a][d][x], e0, e1);
+          odd |= static_cast<unsigned>(l[a] < INFINITY && fmaf(e0, 0.f, e1 * 0.f) != 0.f) << a;
+        }
       if (w.slot >= 0) {
         const int64_t pr = static_cast<int64_t>(w.slot) * p.rows + r;
 #pragma unroll
@@ -240,6 +249,28 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
             dst[d * 64 + tx * 4 + 2 * x + 1] = Elt<T>::from_f(e1 * inv);
           }
         if (tx == 0) p.lse[t * p.H + h] = m[a] * 0.6931471805599453f + logf(l[a]);
+      }
+    }
+    if (__any_sync(0xffffffffu, odd != 0)) {            // values that not all rows see?
+      const int lane = threadIdx.x & 31;
+      __syncwarp();                                     // the rows are read back
+      if (paged_odd_values<T, HD>(p, w, range, mask.hi(w.tok0), mask.lo(w.tok0 + w.ntok - 1), kSimtKeys, lane)) {
+#pragma unroll 1
+        for (int x = 0; x < 2 * RM; ++x) {              // the warp's rows: two of every 16
+          const int a = x >> 1, half = x & 1;
+          const unsigned who = __ballot_sync(0xffffffffu, odd >> a & 1);
+          if ((who >> (16 * half) & 0xffffu) == 0) continue;
+          float ma = m[0], la = l[0];
+#pragma unroll
+          for (int y = 1; y < RM; ++y)
+            if (a == y) ma = m[y], la = l[y];
+          ma = __shfl_sync(0xffffffffu, ma, 16 * half);
+          la = __shfl_sync(0xffffffffu, la, 16 * half);
+          const int r = (ty & ~1) + half + 16 * a;
+          const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + r / p.G) * p.H + w.kvh * p.G + r % p.G;
+          paged_repair_row<T, HD>(p, w, w.tok0 + r / p.G, r % p.G, ma, la == 0.f ? 0.f : 1.f / la, static_cast<T*>(p.out) + row * HD,
+                                  w.slot >= 0 ? p.part_O + (static_cast<int64_t>(w.slot) * p.rows + r) * HD : nullptr, kSimtKeys, lane);
+        }
       }
     }
   }

@@ -339,6 +339,8 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       // where the rows are few, else 32 at a time.
       const int turn = REP * rows * (HD + 1) <= 128 * kRedLd ? HD : 32, ld = turn + 1;
       float* mine = red + (copy * rows + rr) * ld;
+      float finite = 0.f;                                // NaN where an output of this thread's is not finite
+      bool all_finite = true;
 #pragma unroll 1
       for (int c0 = 0; c0 < HD; c0 += turn) {
 #pragma unroll 1
@@ -365,6 +367,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
           float sum = red[row * ld + c];
 #pragma unroll
           for (int y = 1; y < REP; ++y) sum += red[(y * rows + row) * ld + c];
+          finite = fmaf(sum, 0.f, finite);
           if (w.slot < 0) {
             const int64_t t = w.q0 + w.tok0 + row / p.G;
             static_cast<__nv_bfloat16*>(p.out)[(t * p.H + w.kvh * p.G + row % p.G) * HD + c0 + c] =
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
             p.part_O[(slot_row + row) * HD + c0 + c] = sum;
           }
         }
-        vote128(true);
+        all_finite = vote128(finite == 0.f);
       }
       if (valid && copy == 0) {
         if (w.slot < 0) {
@@ -383,6 +386,24 @@ __global__ void __launch_bounds__(kTokThreads, 1)
           p.part_ml[2 * (slot_row + rr)] = M_row;
           p.part_ml[2 * (slot_row + rr) + 1] = L_row;
         }
+      }
+      // Values that not all rows see?  (One token's rows see the same; of its copies only one has the
+      // weight of an infinite value, the others 0.)
+      if (!all_finite && (REP > 1 || (w.ntok > 1 && paged_odd_values<__nv_bfloat16, HD>(p, w, range, hi_min, lo_max, kPagedKB, lane)))) {
+        if (valid && copy == 0) {
+          s_m[rr] = M_row;
+          s_l[rr] = L_row;
+        }
+        vote128(true);
+        for (int x = quarter; x < rows; x += 4) {
+          const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + x / p.G) * p.H + w.kvh * p.G + x % p.G;
+          const float sum = s_l[x];
+          if (sum < INFINITY)
+            paged_repair_row<__nv_bfloat16, HD>(p, w, w.tok0 + x / p.G, x % p.G, s_m[x], sum == 0.f ? 0.f : 1.f / sum,
+                                                static_cast<__nv_bfloat16*>(p.out) + row * HD,
+                                                w.slot >= 0 ? p.part_O + (slot_row + x) * HD : nullptr, kPagedKB, lane);
+        }
+        vote128(true);                                   // (the next item writes s_m)
       }
     }
     if (!ok) *abort_flag = 1;

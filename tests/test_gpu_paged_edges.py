@@ -238,3 +238,30 @@ def test_a_token_that_is_not_finite_spoils_the_keys_it_sees_only(dtype, window, 
     want, tol = st.exact_mass(lse, start)
     assert bool(want.isnan().any())
     within(mass, want, tol, "weights")
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF, 128), (BF, 64), (F32, 128), (F32, 64)])
+@pytest.mark.parametrize("q,n,mask", [
+    ([100, 20, 1, 33], [400, 150, 300, 33], {}), ([100, 64, 7], [300, 64, 500], dict(block=32)),
+    ([70, 9], [200, 90], dict(block=0)), ([150, 20, 1], [500, 300, 90], dict(window=30, sinks=2)),
+    ([40], [3000], {}), ([7, 5], [2000, 1500], {}), ([300], [2600], dict(window=700, sinks=1))])
+def test_values_that_are_not_finite_stay_out_of_tokens_that_do_not_see_them(q, n, mask, dtype, hd):
+    """Infinite and NaN values in keys that some tokens of a tile see and others do not: the ones
+    have what the formula gives, the others finite outputs."""
+    st = Step(q, n, 8, 2, hd=hd, ps=32, dtype=dtype, seed=7, **mask)
+    for b, (ql, nl) in enumerate(zip(q, n)):
+        base, v = nl - ql, st.v[b]
+        v[base + ql // 3, :, 3] = math.nan
+        v[base + ql // 2, 1, 5], v[base + ql // 2, :, 6] = math.inf, -math.inf
+        v[base + 2 * ql // 3, 0, 6] = math.inf
+        v[nl - 1, 0] = math.inf
+        v[1, 1, 11] = -math.inf
+        if base > 10:
+            v[base - 5, :, 9] = math.nan
+    k, v = st.pages()
+    plan = st.plan()
+    out, lse = K.paged_attention(st.q, k, v, st.table, plan)
+    plan.check()
+    want, l, tol_o, tol_l = st.exact()
+    within(out, want, tol_o, "out")
+    within(lse, l, tol_l, "lse")
