@@ -428,7 +428,8 @@ int sf_paged_attention_mass(const sf_paged_plan* plan, const sf_paged_pool* pool
  * +inf).  Their rows and weights move, in the order of their positions, to positions 0, 1, ...
  * of the pages of dst_table, which must not be pages of a source table; kept [B][Hkv]
  * [kept_stride] gets their old positions, -1 after the last.  lens [B][2] int32 on the device
- * with max_len / max_keep its columns' maxima; sinks + recent <= every lens[b][1] that is below
+ * with max_len / max_keep its columns' maxima (give a budget that exceeds its length as that
+ * length: kept and dst_table then need room for what stays, no more); sinks + recent <= every lens[b][1] that is below
  * lens[b][0] (lengths beyond these set SF_DEV_INDEX and are cut to them); kept_stride >= min(max_len, max_keep). */
 int sf_paged_evict(int dtype, const sf_paged_pool* pool, const int32_t* dst_table,
                    int64_t dst_stride, int32_t dst_width, const int32_t* lens, int32_t max_len,

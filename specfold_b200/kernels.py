@@ -408,11 +408,14 @@ class EvictPlan(_OnStream):
         device = _cuda_device(device)
         self.sequences, self.kv_heads, self.page_size = n.numel(), kv_heads, page_size
         self.sinks, self.recent = sinks, recent
-        self.stay = torch.minimum(n, k).tolist()
+        # a budget above its length evicts nothing: what stays is then the length, and a budget that
+        # only a short sequence has does not size the others' rows and tables
+        k = torch.minimum(n, k)
+        self.stay = k.tolist()
         self.max_len = int(n.max()) if n.numel() else 0
-        # budgets above every length evict nothing: sinks + recent then bounds nothing
-        self.max_keep = max(int(k.max()) if n.numel() else 0, sinks + recent)
         self.kept = max(self.stay, default=0)
+        # (where nothing is evicted sinks + recent may be more than stays: it bounds nothing)
+        self.max_keep = max(self.kept, sinks + recent)
         self._lens = torch.stack((n, k), 1).contiguous().to(device)
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
         self._made(device, self._lens, self.err)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from specfold_b200 import kernels as K
-from tests.paged_reference import U32, UB, UW
+from tests.paged_reference import U32, UB, UW, evict_positions
 
 pytestmark = pytest.mark.gpu
 
@@ -265,3 +265,51 @@ def test_values_that_are_not_finite_stay_out_of_tokens_that_do_not_see_them(q, n
     want, l, tol_o, tol_l = st.exact()
     within(out, want, tol_o, "out")
     within(lse, l, tol_l, "lse")
+
+
+# ---------------------------------------------------------------------------- eviction
+def evict(lens, keep, ps=64, Hkv=2, hd=64, sinks=0, recent=0, dtype=BF, seed=0, mass=None, room=0):
+    """An eviction against a sort of the weights: positions kept, rows and weights moved.  The
+    destination table holds what stays, and ``room`` pages more."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    budget = [keep] * len(lens) if isinstance(keep, int) else keep
+    stay = [min(n, m) for n, m in zip(lens, budget)]
+    need, into = ([-(-n // ps) for n in x] for x in (lens, stay))
+    order = torch.randperm(sum(need) + sum(into), generator=g, device="cuda").to(torch.int32)
+    src = torch.full((len(lens), max(need)), -1, dtype=torch.int32, device="cuda")
+    dst = torch.full((len(lens), max(into) + room), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, (x, y) in enumerate(zip(need, into)):
+        src[b, :x], dst[b, :y] = order[at:at + x], order[at + x:at + x + y]
+        at += x + y
+    k, v = (torch.randn(len(order), Hkv, ps, hd, generator=g, device="cuda").to(dtype) for _ in range(2))
+    if mass is None:
+        mass = (torch.rand(len(order), Hkv, ps, generator=g, device="cuda") * 4000).round() / 8
+    else:
+        mass = mass(torch.rand(len(order), Hkv, ps, generator=g, device="cuda"))
+    plan = K.EvictPlan(lens, keep, kv_heads=Hkv, page_size=ps, sinks=sinks, recent=recent)
+    gk, gv, gm = k.clone(), v.clone(), mass.clone()
+    kept = K.paged_evict(gk, gv, gm, src, dst, plan)
+    plan.check()
+    assert kept.shape == (len(lens), Hkv, max(stay))
+    kept = kept.cpu()
+    for b, n in enumerate(lens):
+        j, r = torch.arange(n), torch.arange(stay[b])
+        for h in range(Hkv):
+            w = mass[src[b, j // ps].long().cpu(), h, j % ps].cpu()
+            rank = torch.where(w.isnan(), math.inf, w.double().clamp(max=1e300)).tolist()
+            want = evict_positions(rank, budget[b], sinks, recent)
+            assert kept[b, h].tolist() == want + [-1] * (kept.shape[2] - len(want))
+            x = torch.tensor(want, dtype=torch.long)
+            a, c = (src[b, x // ps].long(), h, x % ps), (dst[b, r // ps].long(), h, r % ps)
+            k[c], v[c], mass[c] = k[a], v[a], mass[a]
+    assert torch.equal(gk, k) and torch.equal(gv, v)
+    assert torch.equal(gm.view(torch.int32), mass.view(torch.int32))
+
+
+@pytest.mark.parametrize("lens,keep,sinks,recent", [
+    ([800, 100], [33, 500], 4, 8), ([10, 5000], [4096, 100], 0, 0), ([64, 65, 3], [64, 3, 900], 1, 1),
+    ([50, 700], [1 << 30, 40], 0, 40), ([20, 30], [500, 40], 90, 90)])
+def test_budgets_that_are_larger_on_shorter_sequences(lens, keep, sinks, recent):
+    evict(lens, keep, sinks=sinks, recent=recent)
+    evict(lens, keep, sinks=sinks, recent=recent, ps=16, room=3)
