@@ -69,8 +69,10 @@ cudaError_t launch_paged_append(int dtype, const PagedAppendParams& p, cudaStrea
 constexpr int kSelThreads = 1024;
 constexpr int kSelKeys = 8;
 
+// bits that order like the weights: zeros of either sign are equal, a NaN of either is above all
 __device__ __forceinline__ uint32_t order_bits(float f) {
-  const uint32_t u = __float_as_uint(f);
+  if (isnan(f)) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(f + 0.f);           // -0 + 0 = 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 

@@ -313,3 +313,16 @@ def evict(lens, keep, ps=64, Hkv=2, hd=64, sinks=0, recent=0, dtype=BF, seed=0, 
 def test_budgets_that_are_larger_on_shorter_sequences(lens, keep, sinks, recent):
     evict(lens, keep, sinks=sinks, recent=recent)
     evict(lens, keep, sinks=sinks, recent=recent, ps=16, room=3)
+
+
+@pytest.mark.parametrize("kind", ["zeros", "nan"])
+@pytest.mark.parametrize("n,keep", [(300, 120), (9000, 3000)])
+def test_zeros_and_nans_of_either_sign(kind, n, keep):
+    """-0 and 0 are equal weights, of which the lowest positions stay; a NaN ranks above +inf
+    whatever its sign."""
+    def mass(u):
+        if kind == "zeros":
+            return torch.where(u < 0.1, u, torch.where(u < 0.5, 0.0, -0.0))
+        bad = torch.where(u < 0.1, 0x7fc00000, torch.where(u < 0.2, -0x400000, 0x7f800000))    # NaN, -NaN, inf
+        return torch.where(u < 0.5, bad.to(torch.int32).view(torch.float32), u)
+    evict([n, n // 2], keep, sinks=2, recent=7, mass=mass)
