@@ -25,6 +25,8 @@ used on one stream at a time.
 
 from __future__ import annotations
 
+import contextlib
+import itertools
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -94,6 +96,17 @@ class PagedKVCache:
             raise MemoryError(f"{n} pages needed, {len(self._free)} of {self.num_pages} free")
         return [self._free.pop() for _ in range(n)]
 
+    @contextlib.contextmanager
+    def _taken(self, counts: Sequence[int]):
+        """Lists of free pages, one of each length; they go back to the pool if the body fails."""
+        fresh = self._take(sum(counts))
+        try:
+            it = iter(fresh)
+            yield [list(itertools.islice(it, n)) for n in counts]
+        except BaseException:
+            self._free.extend(reversed(fresh))
+            raise
+
     def _table(self, rows: List[List[int]]) -> torch.Tensor:
         width = max([len(r) for r in rows] + [1])
         return torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32
@@ -104,7 +117,7 @@ class PagedKVCache:
              window: int = 0, sinks: int = 0) -> PagedStep:
         """Makes room for ``q_lens[i]`` new tokens of ``seqs[i]``, counts them as cached and plans
         the step (``kernels.PagedPlan`` has the mask's meaning).  Nothing changes when the pool
-        is too small (MemoryError)."""
+        is too small (MemoryError) or the step fails in another way."""
         seqs = list(seqs)
         if len(set(seqs)) != len(seqs) or len(seqs) != len(q_lens):
             raise ValueError("a step takes every sequence once, with one chunk length each")
@@ -116,11 +129,12 @@ class PagedKVCache:
                            head_dim=self.head_dim, page_size=self.page_size, dtype=self.dtype,
                            block=block, window=window, sinks=sinks, mass=self._mass is not None,
                            device=self.device)
-        fresh = self._take(sum(more))
-        for s, n, m in zip(seqs, lens, more):
-            self._pages[s] += [fresh.pop() for _ in range(m)]
-            self._len[s] = n
-        return PagedStep(seqs, plan, self._table([self._pages[s] for s in seqs]))
+        with self._taken(more) as fresh:
+            rows = [self._pages[s] + new for s, new in zip(seqs, fresh)]
+            step = PagedStep(seqs, plan, self._table(rows))
+        for s, n, row in zip(seqs, lens, rows):
+            self._pages[s], self._len[s] = row, n
+        return step
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: PagedStep) -> None:
         """The step's new keys and values [T, Hkv, hd] of one layer into their pages."""
@@ -160,8 +174,8 @@ class PagedKVCache:
         """Cuts every sequence to ``keep`` positions, in every layer and kv head by accumulated
         weight: the first ``sinks``, the last ``recent`` and the heaviest others stay, in order.
         Returns per layer the old positions of what stayed, int32 [len(seqs), Hkv, most kept]
-        (-1 after the last).  The survivors move to free pages (MemoryError when there are too few;
-        nothing has changed then) and the old ones are returned."""
+        (-1 after the last).  The survivors move to free pages and the old ones are returned.
+        Nothing has changed when there are too few (MemoryError) or the call fails in another way."""
         if self._mass is None:
             raise ValueError("the cache was made without track_mass")
         seqs = list(seqs)
@@ -172,11 +186,10 @@ class PagedKVCache:
         lens = [self._len[s] for s in seqs]
         plan = K.EvictPlan(lens, keep, kv_heads=self.num_kv_heads, page_size=self.page_size, sinks=sinks,
                            recent=recent, device=self.device)
-        fresh = self._take(sum(map(self._need, plan.stay)))
-        into = [[fresh.pop() for _ in range(self._need(n))] for n in plan.stay]
-        table, dst = self._table([self._pages[s] for s in seqs]), self._table(into)
-        kept = [K.paged_evict(self._store[x, 0], self._store[x, 1], self._mass[x], table, dst, plan)
-                for x in range(self.num_layers)]
+        with self._taken([self._need(n) for n in plan.stay]) as into:
+            table, dst = self._table([self._pages[s] for s in seqs]), self._table(into)
+            kept = [K.paged_evict(self._store[x, 0], self._store[x, 1], self._mass[x], table, dst, plan)
+                    for x in range(self.num_layers)]
         for s, n, new in zip(seqs, plan.stay, into):
             self._free.extend(self._pages[s])
             self._pages[s], self._len[s] = new, n

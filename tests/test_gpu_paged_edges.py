@@ -326,3 +326,53 @@ def test_zeros_and_nans_of_either_sign(kind, n, keep):
         bad = torch.where(u < 0.1, 0x7fc00000, torch.where(u < 0.2, -0x400000, 0x7f800000))    # NaN, -NaN, inf
         return torch.where(u < 0.5, bad.to(torch.int32).view(torch.float32), u)
     evict([n, n // 2], keep, sinks=2, recent=7, mass=mass)
+
+
+# ---------------------------------------------------------------------------- the cache
+def filled_cache(lens, num_pages, layers=2, H=4, Hkv=2, hd=64, seed=0):
+    """A cache whose sequences have these lengths, with random keys, values and weights."""
+    from specfold_b200 import PagedKVCache
+    cache = PagedKVCache(layers, Hkv, hd, num_pages=num_pages, page_size=16, dtype=F32, track_mass=True)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    seqs = [cache.add() for _ in lens]
+    step = cache.step(seqs, lens, heads=H)
+    for x in range(layers):
+        k, v = (torch.randn(sum(lens), Hkv, hd, generator=g, device="cuda") for _ in range(2))
+        cache.append(x, k, v, step)
+    step.check()
+    cache._mass.copy_(torch.rand(cache._mass.shape, generator=g, device="cuda"))
+    return cache, seqs
+
+
+def contents(cache, seq):
+    """[layers, keys and values, Hkv, length, hd] and the weights of a sequence"""
+    pages, n = torch.tensor(cache.pages(seq), dtype=torch.long, device="cuda"), cache.length(seq)
+    rows = cache._store[:, :, pages].transpose(2, 3).flatten(3, 4)[:, :, :, :n]
+    return rows.clone(), cache._mass[:, pages].transpose(1, 2).flatten(2, 3)[..., :n].clone()
+
+
+def test_pages_are_not_lost_when_a_call_fails(monkeypatch):
+    cache, (a, b) = filled_cache([100, 40], 30)
+    free, pages, before = cache.free_pages, cache.pages(a), contents(cache, a)
+    real, calls = K.paged_evict, []
+
+    def fails_in_the_second_layer(*args):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("no")
+        return real(*args)
+
+    monkeypatch.setattr(K, "paged_evict", fails_in_the_second_layer)
+    with pytest.raises(RuntimeError):
+        cache.evict([a, b], 32)
+    monkeypatch.setattr(K, "paged_evict", real)
+    monkeypatch.setattr(cache, "_table", lambda rows: 1 / 0)
+    for call in (lambda: cache.evict([a], 32), lambda: cache.step([a, b], [70, 1], heads=4)):
+        with pytest.raises(ZeroDivisionError):
+            call()
+    monkeypatch.undo()
+    assert cache.free_pages == free and cache.pages(a) == pages and cache.length(a) == 100
+    assert all(torch.equal(x, y) for x, y in zip(contents(cache, a), before))
+    cache.evict([a, b], 32)
+    cache.step([a, b], [70, 1], heads=4).check()
+    assert len(set(cache._free + cache.pages(a) + cache.pages(b))) == 30
