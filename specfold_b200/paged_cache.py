@@ -27,7 +27,7 @@ from __future__ import annotations
 
 import contextlib
 import itertools
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -170,27 +170,47 @@ class PagedKVCache:
                 n += 1
         return n
 
-    def evict(self, seqs: Sequence[int], keep: int, sinks: int = 0, recent: int = 0) -> List[torch.Tensor]:
-        """Cuts every sequence to ``keep`` positions, in every layer and kv head by accumulated
-        weight: the first ``sinks``, the last ``recent`` and the heaviest others stay, in order.
-        Returns per layer the old positions of what stayed, int32 [len(seqs), Hkv, most kept]
-        (-1 after the last).  The survivors move to free pages and the old ones are returned.
-        Nothing has changed when there are too few (MemoryError) or the call fails in another way."""
+    def evict(self, seqs: Sequence[int], keep: Union[int, Sequence[int]], sinks: int = 0, recent: int = 0
+              ) -> List[torch.Tensor]:
+        """Cuts every sequence to ``keep`` (or ``keep[i]``) positions, in every layer and kv head by
+        accumulated weight: the first ``sinks``, the last ``recent`` and the heaviest others stay, in
+        order.  Returns per layer the old positions of what stayed, int32 [len(seqs), Hkv, most
+        kept] (-1 after the last).  A sequence within ``keep`` stays where it is; the survivors of
+        the others move to free pages and the old ones are returned.  Nothing has changed when there
+        are too few (MemoryError; sequence by sequence fewer will do) or the call fails in another
+        way."""
         if self._mass is None:
             raise ValueError("the cache was made without track_mass")
         seqs = list(seqs)
         if len(set(seqs)) != len(seqs):
             raise ValueError("an eviction takes every sequence once")
-        if any(-1 in self._pages[s] for s in seqs):
-            raise ValueError("a sequence with released pages cannot be cut by weight")
         lens = [self._len[s] for s in seqs]
-        plan = K.EvictPlan(lens, keep, kv_heads=self.num_kv_heads, page_size=self.page_size, sinks=sinks,
-                           recent=recent, device=self.device)
+        keep = list(keep) if hasattr(keep, "__len__") else [keep] * len(seqs)
+        if len(keep) != len(seqs):
+            raise ValueError(f"{len(keep)} budgets for {len(seqs)} sequences")
+        over = [i for i, n in enumerate(lens) if n > keep[i]]
+        cut = [seqs[i] for i in over]
+        if any(-1 in self._pages[s] for s in cut):
+            raise ValueError("a sequence with released pages cannot be cut by weight")
+        plan = K.EvictPlan([lens[i] for i in over], [keep[i] for i in over], kv_heads=self.num_kv_heads,
+                           page_size=self.page_size, sinks=sinks, recent=recent, device=self.device)
         with self._taken([self._need(n) for n in plan.stay]) as into:
-            table, dst = self._table([self._pages[s] for s in seqs]), self._table(into)
+            table, dst = self._table([self._pages[s] for s in cut]), self._table(into)
             kept = [K.paged_evict(self._store[x, 0], self._store[x, 1], self._mass[x], table, dst, plan)
                     for x in range(self.num_layers)]
-        for s, n, new in zip(seqs, plan.stay, into):
+            if len(cut) < len(seqs):
+                kept = self._with_whole(kept, [min(n, k) for n, k in zip(lens, keep)], over)
+        for s, n, new in zip(cut, plan.stay, into):
             self._free.extend(self._pages[s])
             self._pages[s], self._len[s] = new, n
         return kept
+
+    def _with_whole(self, kept: List[torch.Tensor], stay: List[int], over: List[int]) -> List[torch.Tensor]:
+        """``kept`` of the sequences ``over`` alone, with the rows of those that stayed whole."""
+        j = torch.arange(max(stay), dtype=torch.int32)
+        whole = torch.where(j < torch.tensor(stay)[:, None], j, -1)[:, None].repeat(1, self.num_kv_heads, 1).to(self.device)
+        rows = torch.tensor(over, dtype=torch.long).to(self.device)
+        out = [whole.clone() for _ in kept]
+        for o, k in zip(out, kept):
+            o[rows, :, :k.shape[2]] = k
+        return out

@@ -376,3 +376,36 @@ def test_pages_are_not_lost_when_a_call_fails(monkeypatch):
     cache.evict([a, b], 32)
     cache.step([a, b], [70, 1], heads=4).check()
     assert len(set(cache._free + cache.pages(a) + cache.pages(b))) == 30
+
+
+def test_sequences_within_their_budget_stay_where_they_are():
+    """An eviction moves, and needs room for, the sequences that are over the budget alone."""
+    lens = [100, 40, 32, 0, 33]                              # 7 + 3 + 2 + 0 + 3 pages
+    cache, seqs = filled_cache(lens, 15 + 4)                 # room for the two that are cut
+    before, pages = [contents(cache, s) for s in seqs], [cache.pages(s) for s in seqs]
+    kept = cache.evict(seqs, 40, sinks=2, recent=4)
+    assert [cache.length(s) for s in seqs] == [40, 40, 32, 0, 33]
+    assert all(cache.pages(s) == p for s, p in zip(seqs[1:], pages[1:])) and cache.free_pages == 19 - 11
+    for x in range(2):
+        assert kept[x].shape == (5, 2, 40) and kept[x].dtype == torch.int32
+        for i, n in enumerate(lens):
+            for h in range(2):
+                want = evict_positions(before[i][1][x, h].tolist(), 40, 2, 4)
+                assert kept[x][i, h].tolist() == want + [-1] * (40 - len(want))
+                now = contents(cache, seqs[i])
+                assert torch.equal(now[0][x, :, h], before[i][0][x, :, h][:, want])
+                assert torch.equal(now[1][x, h], before[i][1][x, h][want])
+    kept = cache.evict(seqs, 60, recent=100)                 # nothing to cut: nothing to hold
+    assert [k.tolist()[4][0] for k in kept] == [list(range(33)) + [-1] * 7] * 2
+    released = cache.add()
+    cache.step([released], [70], heads=4).check()
+    cache.release(released, 20)
+    assert [k.shape for k in cache.evict([released], 80)] == [(1, 2, 70)] * 2
+    with pytest.raises(ValueError, match="released"):
+        cache.evict([released], 60)
+    a, b = seqs[0], seqs[2]
+    kept = cache.evict([a, b], [50, 7])                      # budgets of their own
+    assert (cache.length(a), cache.length(b)) == (40, 7)
+    assert kept[0].shape == (2, 2, 40) and kept[0][0, 1].tolist() == list(range(40)) and int(kept[0][1, 0, 7]) == -1
+    with pytest.raises(ValueError, match="budgets"):
+        cache.evict([a, b], [50])
