@@ -293,16 +293,7 @@ cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t
   const dim3 grid((p.rows + 7) / 8, p.n_merges);
   // lines up behind the pieces' kernel (which lets it) and waits for its end on the device
   auto go = [&](auto* kernel) {
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    const cudaError_t e = launch_attr(kernel, grid, dim3(256), 0, st, false, true, p);
     return e == cudaSuccess ? launched() : e;
   };
   if (dtype == BF16)

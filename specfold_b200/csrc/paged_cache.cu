@@ -365,16 +365,9 @@ cudaError_t launch_paged_evict(int dtype, const PagedEvictParams& p, cudaStream_
   if (e == cudaSuccess) e = launched();
   if (e != cudaSuccess || stay == 0) return e;
   const dim3 grid((stay + kMoveKeys - 1) / kMoveKeys, p.B * p.Hkv);
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
-  if (dtype == BF16)
-    e = p.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_move_kernel<__nv_bfloat16, 16>, p)
-                    : cudaLaunchKernelEx(&cfg, paged_move_kernel<__nv_bfloat16, 8>, p);
-  else
-    e = p.hd == 128 ? cudaLaunchKernelEx(&cfg, paged_move_kernel<float, 32>, p)
-                    : cudaLaunchKernelEx(&cfg, paged_move_kernel<float, 16>, p);
+  auto move = [&](auto* kernel) { return launch_attr(kernel, grid, dim3(256), 0, st, false, true, p); };
+  if (dtype == BF16) e = p.hd == 128 ? move(paged_move_kernel<__nv_bfloat16, 16>) : move(paged_move_kernel<__nv_bfloat16, 8>);
+  else e = p.hd == 128 ? move(paged_move_kernel<float, 32>) : move(paged_move_kernel<float, 16>);
   return e == cudaSuccess ? launched() : e;
 }
 

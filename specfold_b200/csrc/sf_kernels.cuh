@@ -15,12 +15,13 @@ constexpr int kMaxGateSmem = 227 * 1024;
 // one finishes; it calls pdl_wait() before touching what that kernel produces), plus the
 // cooperative attribute when the kernel's CTAs wait on one another.  If the driver
 // refuses the combination, the launch is repeated without the programmatic attribute.
-// The programmatic attribute is set only with SF_PDL=1 in the environment (read once).
+// The programmatic attribute is set only with SF_PDL=1 in the environment (read once), or where
+// the caller asks for it: a kernel that only ever follows one that calls pdl_trigger().
 bool pdl_enabled();
 
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                             cudaStream_t st, bool cooperative, Args&&... args) {
+inline cudaError_t launch_attr(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t st, bool cooperative, bool programmatic, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -29,7 +30,7 @@ inline cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
   cudaLaunchAttribute attr[2];
   int na = 0;
   attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[na].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[na].val.programmaticStreamSerializationAllowed = programmatic ? 1 : 0;
   ++na;
   if (cooperative) {
     attr[na].id = cudaLaunchAttributeCooperative;
@@ -46,6 +47,12 @@ inline cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
     e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
   }
   return e;
+}
+
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_ex(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t st, bool cooperative, Args&&... args) {
+  return launch_attr(kernel, grid, block, smem, st, cooperative, pdl_enabled(), std::forward<Args>(args)...);
 }
 
 // records msg for sf_last_error() and returns code
