@@ -20,58 +20,40 @@ namespace sf {
 constexpr int kSimtThreads = 256;
 constexpr int kSimtKeys = kPagedKeysF32;
 
-template <typename T>
-__device__ __forceinline__ void simt_store_row(float* dst, const T* src, int e);
-template <>
-__device__ __forceinline__ void simt_store_row<float>(float* dst, const float* src, int e) {
-  *reinterpret_cast<float4*>(dst + e) = *reinterpret_cast<const float4*>(src + e);
-}
-template <>
-__device__ __forceinline__ void simt_store_row<__nv_bfloat16>(float* dst, const __nv_bfloat16* src,
-                                                              int e) {
-  float f[8];
-  load_vec(src + e, f);
-  *reinterpret_cast<float4*>(dst + e) = make_float4(f[0], f[1], f[2], f[3]);
-  *reinterpret_cast<float4*>(dst + e + 4) = make_float4(f[4], f[5], f[6], f[7]);
-}
-
 // keys [k0, k0 + 64) of a sequence into shared memory [64][HD + 4]; keys outside `range`, which
 // no row of the tile sees, are zero: their slots may never have been written (0 * NaN is NaN),
 // their pages may be gone
-template <typename T, int HD>
+template <int HD>
 __device__ __forceinline__ void simt_load_keys(float* dst, const void* pages, const PagedPool& pool,
                                                int seq, int kvh, int k0, PagedRange range, int* err) {
-  constexpr int VPR = HD / Elt<T>::kVec;
+  constexpr int VPR = HD / 4;
   for (int i = threadIdx.x; i < kSimtKeys * VPR; i += kSimtThreads) {
-    const int r = i / VPR, e = (i % VPR) * Elt<T>::kVec;
+    const int r = i / VPR, e = (i % VPR) * 4;
     const int key = k0 + r;
     float* d = dst + r * (HD + 4);
     if (range.has(key)) {
       const int page = paged_page(pool, seq, key >> pool.page_shift, err);
-      const T* src = static_cast<const T*>(pages) + page * pool.page_stride + kvh * pool.head_stride +
-                     (key & ((1 << pool.page_shift) - 1)) * pool.row_stride;
-      simt_store_row<T>(d, src, e);
+      const float* src = static_cast<const float*>(pages) + page * pool.page_stride + kvh * pool.head_stride +
+                         (key & ((1 << pool.page_shift) - 1)) * pool.row_stride;
+      *reinterpret_cast<float4*>(d + e) = *reinterpret_cast<const float4*>(src + e);
     } else {
-#pragma unroll
-      for (int x = 0; x < Elt<T>::kVec; x += 4)
-        *reinterpret_cast<float4*>(d + e + x) = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(d + e) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
 }
 
-template <typename T, int HD, int RM>
+template <int HD, int RM>
 __device__ __forceinline__ void simt_load_q(float* sQ, const void* q, int64_t q_tok, int64_t q_head,
                                             int row0, int kvh, int G, int rows) {
-  constexpr int VPR = HD / Elt<T>::kVec;
+  constexpr int VPR = HD / 4;
   for (int i = threadIdx.x; i < 16 * RM * VPR; i += kSimtThreads) {
-    const int r = i / VPR, e = (i % VPR) * Elt<T>::kVec;
+    const int r = i / VPR, e = (i % VPR) * 4;
     float* d = sQ + r * (HD + 4);
     if (r < rows) {
-      simt_store_row<T>(d, static_cast<const T*>(q) + (row0 + r / G) * q_tok + (kvh * G + r % G) * q_head, e);
+      const float* src = static_cast<const float*>(q) + (row0 + r / G) * q_tok + (kvh * G + r % G) * q_head;
+      *reinterpret_cast<float4*>(d + e) = *reinterpret_cast<const float4*>(src + e);
     } else {
-#pragma unroll
-      for (int x = 0; x < Elt<T>::kVec; x += 4)
-        *reinterpret_cast<float4*>(d + e + x) = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(d + e) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
 }
@@ -121,7 +103,7 @@ __device__ __forceinline__ float half_warp_sum(float v) {
   return v;
 }
 
-template <typename T, int HD, int RM>
+template <int HD, int RM>
 __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(PagedAttnParams p) {
   constexpr int R = 16 * RM, LD = HD + 4, LP = 2 * kSimtKeys + 4;
   constexpr int DV = HD / 64;                           // float4 groups of O per thread
@@ -152,11 +134,11 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
     }
     const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
     __syncthreads();                                    // the previous item's reads are done
-    simt_load_q<T, HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + w.tok0, w.kvh, p.G, rows);
+    simt_load_q<HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + w.tok0, w.kvh, p.G, rows);
     for (int i = w.i0; i < w.i1; ++i) {
       const int k0 = w.block(i) * kSimtKeys;
       __syncthreads();
-      simt_load_keys<T, HD>(sKV, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
+      simt_load_keys<HD>(sKV, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
       __syncthreads();
       float s[RM][4];
       simt_scores<HD, RM>(sQ, sKV, s);
@@ -190,7 +172,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
         }
       }
       __syncthreads();                                  // K read, P written
-      simt_load_keys<T, HD>(sKV, p.pool.v, p.pool, w.seq, w.kvh, k0, range, p.err);
+      simt_load_keys<HD>(sKV, p.pool.v, p.pool, w.seq, w.kvh, k0, range, p.err);
       __syncthreads();
       // a row of P is written and read by the same half-warp's 16 threads
 #pragma unroll 4
@@ -238,15 +220,15 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
         const int64_t t = w.q0 + w.tok0 + r / p.G;
         const int h = w.kvh * p.G + r % p.G;
         const float inv = l[a] == 0.f ? 0.f : 1.f / l[a];   // a NaN sum stays one
-        T* dst = static_cast<T*>(p.out) + (t * p.H + h) * HD;
+        float* dst = static_cast<float*>(p.out) + (t * p.H + h) * HD;
 #pragma unroll
         for (int d = 0; d < DV; ++d)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             float e0, e1;
             unpair(o[a][d][x], e0, e1);
-            dst[d * 64 + tx * 4 + 2 * x] = Elt<T>::from_f(e0 * inv);
-            dst[d * 64 + tx * 4 + 2 * x + 1] = Elt<T>::from_f(e1 * inv);
+            dst[d * 64 + tx * 4 + 2 * x] = e0 * inv;
+            dst[d * 64 + tx * 4 + 2 * x + 1] = e1 * inv;
           }
         if (tx == 0) p.lse[t * p.H + h] = m[a] * 0.6931471805599453f + logf(l[a]);
       }
@@ -254,7 +236,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
     if (__any_sync(0xffffffffu, odd != 0)) {            // values that not all rows see?
       const int lane = threadIdx.x & 31;
       __syncwarp();                                     // the rows are read back
-      if (paged_odd_values<T, HD>(p, w, range, mask.hi(w.tok0), mask.lo(w.tok0 + w.ntok - 1), kSimtKeys, lane)) {
+      if (paged_odd_values<float, HD>(p, w, range, mask.hi(w.tok0), mask.lo(w.tok0 + w.ntok - 1), kSimtKeys, lane)) {
 #pragma unroll 1
         for (int x = 0; x < 2 * RM; ++x) {              // the warp's rows: two of every 16
           const int a = x >> 1, half = x & 1;
@@ -268,7 +250,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
           la = __shfl_sync(0xffffffffu, la, 16 * half);
           const int r = (ty & ~1) + half + 16 * a;
           const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + r / p.G) * p.H + w.kvh * p.G + r % p.G;
-          paged_repair_row<T, HD>(p, w, w.tok0 + r / p.G, r % p.G, ma, la == 0.f ? 0.f : 1.f / la, static_cast<T*>(p.out) + row * HD,
+          paged_repair_row<float, HD>(p, w, w.tok0 + r / p.G, r % p.G, ma, la == 0.f ? 0.f : 1.f / la, static_cast<float*>(p.out) + row * HD,
                                   w.slot >= 0 ? p.part_O + (static_cast<int64_t>(w.slot) * p.rows + r) * HD : nullptr, kSimtKeys, lane);
         }
       }
@@ -301,21 +283,21 @@ cudaError_t launch_paged_merge(int dtype, const PagedAttnParams& p, cudaStream_t
   return p.hd == 128 ? go(paged_merge_kernel<float, 128>) : go(paged_merge_kernel<float, 64>);
 }
 
-template <typename T, int HD, int RM>
+template <int HD, int RM>
 static cudaError_t attention_simt(const PagedAttnParams& p, cudaStream_t st) {
   constexpr int R = 16 * RM;
   constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + R * (2 * kSimtKeys + 4)) * 4;
-  cudaError_t e = allow_smem(paged_attention_simt_kernel<T, HD, RM>, smem);
+  cudaError_t e = allow_smem(paged_attention_simt_kernel<HD, RM>, smem);
   if (e != cudaSuccess) return e;
-  paged_attention_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
+  paged_attention_simt_kernel<HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
   return launched();
 }
 
 cudaError_t launch_paged_attention_simt(const PagedAttnParams& p, cudaStream_t st) {
   if (p.workers == 0) return cudaSuccess;
   const bool wide = p.rows == 64;
-  if (p.hd == 128) return wide ? attention_simt<float, 128, 4>(p, st) : attention_simt<float, 128, 1>(p, st);
-  return wide ? attention_simt<float, 64, 4>(p, st) : attention_simt<float, 64, 1>(p, st);
+  if (p.hd == 128) return wide ? attention_simt<128, 4>(p, st) : attention_simt<128, 1>(p, st);
+  return wide ? attention_simt<64, 4>(p, st) : attention_simt<64, 1>(p, st);
 }
 
 // ------------------------------------------------------------------ weight accumulation
@@ -333,7 +315,7 @@ __device__ __forceinline__ void add_mass(const PagedMassParams& p, int seq, int 
 
 // A key's weight over all rows that see it: sum of exp(s - lse).  A CTA owns a key block and
 // walks the query rows, so each weight is summed in one place, in one order, and added once.
-template <typename T, int HD, int RM>
+template <int HD, int RM>
 __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedMassParams p) {
   constexpr int R = 16 * RM, LD = HD + 4;
   extern __shared__ __align__(16) float sm[];
@@ -353,13 +335,13 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_mass_simt_kernel(PagedM
         const int k0 = kb * kPagedKB + sub * kSimtKeys;
         if (k0 >= range.hi) break;
         __syncthreads();
-        simt_load_keys<T, HD>(sK, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
+        simt_load_keys<HD>(sK, p.pool.k, p.pool, w.seq, w.kvh, k0, range, p.err);
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
         for (int x = w.i0; x < w.i1; ++x) {
           const int t = w.t0 + x * tile;
           const int rows = min(tile, w.t1 - t) * p.G;
           __syncthreads();
-          simt_load_q<T, HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + t, w.kvh, p.G, rows);
+          simt_load_q<HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + t, w.kvh, p.G, rows);
           __syncthreads();
           float s[RM][4];
           simt_scores<HD, RM>(sQ, sK, s);
@@ -416,19 +398,19 @@ cudaError_t launch_paged_mass_merge(const PagedMassParams& p, cudaStream_t st) {
   return launched();
 }
 
-template <typename T, int HD, int RM>
+template <int HD, int RM>
 static cudaError_t mass_simt(const PagedMassParams& p, cudaStream_t st) {
   constexpr int R = 16 * RM;
   constexpr int smem = (R * (HD + 4) + kSimtKeys * (HD + 4) + 16 * kSimtKeys) * 4;
-  cudaError_t e = allow_smem(paged_mass_simt_kernel<T, HD, RM>, smem);
+  cudaError_t e = allow_smem(paged_mass_simt_kernel<HD, RM>, smem);
   if (e != cudaSuccess) return e;
-  paged_mass_simt_kernel<T, HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
+  paged_mass_simt_kernel<HD, RM><<<p.workers, kSimtThreads, smem, st>>>(p);
   return launched();
 }
 
 cudaError_t launch_paged_mass_simt(const PagedMassParams& p, cudaStream_t st) {
   if (p.workers == 0) return cudaSuccess;
-  return p.hd == 128 ? mass_simt<float, 128, 4>(p, st) : mass_simt<float, 64, 4>(p, st);
+  return p.hd == 128 ? mass_simt<128, 4>(p, st) : mass_simt<64, 4>(p, st);
 }
 
 }  // namespace sf
