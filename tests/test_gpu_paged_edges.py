@@ -186,6 +186,18 @@ def test_ragged_chunks_whose_last_tiles_are_half_empty(hd, window, sinks):
     check_repeatedly(st, "half-empty tiles")
 
 
+# ---------------------------------------------------------------------------- many pieces of a tile
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("q,n,H,pieces", [(1, 32768, 4, 70), (1, 9000, 2, 33), (5, 40000, 12, 70), (48, 20000, 6, 40)])
+def test_one_request_over_a_long_cache(q, n, H, pieces, dtype):
+    """One tile per kv head, cut into more pieces than a warp has lanes, whose join takes several turns."""
+    st = Step([q], [n], H, 2 if H > 2 else 1, ps=128, dtype=dtype, seed=9)
+    st.k[0][::97] *= 2                                       # maxima in every piece
+    plan = st.plan()._c
+    assert max(x.slots / x.n_merges for x in plan.attn if x.n_merges) >= pieces
+    check_repeatedly(st, "long cache", times=5)
+
+
 # ---------------------------------------------------------------------------- shared pages
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("q", [1, 40, 150])
@@ -326,6 +338,13 @@ def test_zeros_and_nans_of_either_sign(kind, n, keep):
         bad = torch.where(u < 0.1, 0x7fc00000, torch.where(u < 0.2, -0x400000, 0x7f800000))    # NaN, -NaN, inf
         return torch.where(u < 0.5, bad.to(torch.int32).view(torch.float32), u)
     evict([n, n // 2], keep, sinks=2, recent=7, mass=mass)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_more_keys_than_a_selecting_block_holds(dtype):
+    """So many heads that each is one CTA's, some with more keys than its registers hold (8192)."""
+    lens = [20000, 8300, 16385, 9000, 12000, 700, 8192, 8193, 30000, 1]
+    evict(lens, 5000, Hkv=8, sinks=3, recent=100, dtype=dtype)
 
 
 # ---------------------------------------------------------------------------- the cache
