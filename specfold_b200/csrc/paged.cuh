@@ -259,89 +259,64 @@ __device__ __forceinline__ void paged_join_row(const PagedAttnParams& p, const P
   if (lane == 0) p.lse[row] = m * 0.6931471805599453f + logf(l);
 }
 
-// What a tile's product P V cannot do: a key that some of its rows do not see has weight 0 in
-// them, and 0 times an infinite or NaN value is NaN.  Rows whose O is not finite although their l
-// is are looked at again when the tile has such a value (odd_values), and the columns in question
-// are added up from the keys that the row sees (repair_row).  Rare and slow, and nothing that runs
-// where the values are finite.  Both are for a whole warp; keys: of a block.
+// Keys that only some rows of a tile see have weight 0 in the others, and 0 times an infinite or NaN
+// value is NaN.  Such values are taken out of the tile in shared memory (only keys of that kind are
+// looked at) and decide their columns here, at the output of the rows that see them: one warp adds up
+// the values that are not finite of the keys that a token sees.  `some`: of those that not all rows of
+// the item see (beyond hi_min, or before lo_max and no sink), else of all.  keys: of a block; need:
+// which of the lane's columns are asked for.
 template <typename T, int HD>
-__device__ __forceinline__ bool paged_odd_values(const PagedAttnParams& p, const PagedItem& w, const PagedRange& range,
-                                                 int hi_min, int lo_max, int keys, int lane) {
-  constexpr int E = HD / 32;
-  bool odd = false;
+__device__ __forceinline__ void paged_odd_values(const PagedAttnParams& p, const PagedItem& w, int tok, bool some,
+                                                 int hi_min, int lo_max, int keys, int lane, unsigned need,
+                                                 float (&sum)[HD / 32]) {
+  constexpr int E = HD / 32, AHEAD = 8;
+  const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
+  const int hi = mask.hi(tok), lo = mask.lo(tok), sinks = p.window > 0 ? p.sinks : 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[e] = 0.f;
 #pragma unroll 1
   for (int i = w.i0; i < w.i1; ++i) {
     const int k0 = w.block(i) * keys;
-    if (k0 + keys <= hi_min && (k0 >= lo_max || k0 + keys <= range.sinks)) continue;   // all rows see all of it
+    if (some && k0 + keys <= hi_min && (k0 >= lo_max || k0 + keys <= sinks)) continue;
 #pragma unroll 1
-    for (int j = k0; j < k0 + keys; ++j) {
-      if (!range.has(j) || (j < hi_min && (j >= lo_max || j < range.sinks))) continue;
-      const int page = paged_page(p.pool, w.seq, j >> p.pool.page_shift, p.err);
-      const T* v = static_cast<const T*>(p.pool.v) + page * p.pool.page_stride + w.kvh * p.pool.head_stride +
-                   (j & ((1 << p.pool.page_shift) - 1)) * p.pool.row_stride + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) odd |= !(fabsf(Elt<T>::to_f(v[e])) < INFINITY);
-    }
-  }
-  return __any_sync(0xffffffffu, odd);
-}
-// Row (tok, g) of the item, whose weights refer to m (log2 units) and whose output is O * f: in
-// out, or in part where that is given.
-template <typename T, int HD>
-__device__ __forceinline__ void paged_repair_row(const PagedAttnParams& p, const PagedItem& w, int tok, int g, float m,
-                                                 float f, T* out, float* part, int keys, int lane) {
-  constexpr int E = HD / 32, AHEAD = 4;
-  const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
-  const int hi = mask.hi(tok), lo = mask.lo(tok), sinks = p.window > 0 ? p.sinks : 0;
-  const float sl2 = p.scale * 1.4426950408889634f, ref = m == -INFINITY ? 0.f : m;
-  const T* qr = static_cast<const T*>(p.q) + (w.q0 + tok) * p.q_tok + (w.kvh * p.G + g) * p.q_head + lane * E;
-  float q[E], o[E];
-  bool need[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = Elt<T>::to_f(qr[e]);
-    o[e] = 0.f;
-    need[e] = !(fabsf(part != nullptr ? part[lane * E + e] : Elt<T>::to_f(out[lane * E + e])) < INFINITY);
-  }
-  bool open = true;                                      // (a column that is not finite again stays so)
-#pragma unroll 1
-  for (int i = w.i1 - 1; open && i >= w.i0; --i) {       // the row's own tokens first
-    const int k0 = w.block(i) * keys;
-#pragma unroll 1
-    for (int j0 = k0 + keys - AHEAD; open && j0 >= k0; j0 -= AHEAD) {
-      float s[AHEAD], v[AHEAD][E];
+    for (int j0 = k0; j0 < k0 + keys; j0 += AHEAD) {       // (in one page)
+      bool take[AHEAD], any = false;
 #pragma unroll
       for (int y = 0; y < AHEAD; ++y) {
         const int j = j0 + y;
-        const bool see = j < hi && (j >= lo || j < sinks);
-        int64_t at = 0;
-        if (see)
-          at = paged_page(p.pool, w.seq, j >> p.pool.page_shift, p.err) * p.pool.page_stride +
-               w.kvh * p.pool.head_stride + (j & ((1 << p.pool.page_shift) - 1)) * p.pool.row_stride + lane * E;
-        s[y] = see ? 0.f : -INFINITY;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          v[y][e] = see ? Elt<T>::to_f(static_cast<const T*>(p.pool.v)[at + e]) : 0.f;
-          if (see) s[y] = fmaf(q[e], Elt<T>::to_f(static_cast<const T*>(p.pool.k)[at + e]), s[y]);
-        }
+        take[y] = j < hi && (j >= lo || j < sinks) && !(some && j < hi_min && (j >= lo_max || j < sinks));
+        any |= take[y];
       }
+      if (!any) continue;
+      const T* row = static_cast<const T*>(p.pool.v) +
+                     paged_page(p.pool, w.seq, j0 >> p.pool.page_shift, p.err) * p.pool.page_stride + w.kvh * p.pool.head_stride +
+                     (j0 & ((1 << p.pool.page_shift) - 1)) * p.pool.row_stride + lane * E;
+      float v[AHEAD][E];
 #pragma unroll
-      for (int y = 0; y < AHEAD; ++y) {
-        const float c = Elt<T>::rnd(exp2f(fmaf(warp_sum(s[y]), sl2, -ref)));
+      for (int y = 0; y < AHEAD; ++y)
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(c, v[y][e], o[e]);
+        for (int e = 0; e < E; ++e) v[y][e] = take[y] ? Elt<T>::to_f(row[y * p.pool.row_stride + e]) : 0.f;
+      bool open = false;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int y = 0; y < AHEAD; ++y)
+          if (!(fabsf(v[y][e]) < INFINITY)) sum[e] += v[y][e];
+        open |= (need >> e & 1) && !isnan(sum[e]);
       }
-      bool more = false;
-#pragma unroll
-      for (int e = 0; e < E; ++e) more |= need[e] && fabsf(o[e]) < INFINITY;
-      open = __any_sync(0xffffffffu, more);
+      if (!__any_sync(0xffffffffu, open)) return;          // (NaN stays NaN)
     }
   }
+}
+// ... into an output row (or its partial, where given): added, or in its place
+template <typename T, int HD>
+__device__ __forceinline__ void paged_put_odd(const float (&sum)[HD / 32], bool add, T* out, float* part, int lane) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (!need[e]) continue;
-    if (part != nullptr) part[lane * E + e] = o[e];
-    else out[lane * E + e] = Elt<T>::from_f(f == 0.f ? 0.f : o[e] * f);
+  for (int e = 0; e < HD / 32; ++e) {
+    const int c = lane * (HD / 32) + e;
+    if (sum[e] == 0.f) continue;
+    if (part != nullptr) part[c] = add ? part[c] + sum[e] : sum[e];
+    else out[c] = Elt<T>::from_f(add ? Elt<T>::to_f(out[c]) + sum[e] : sum[e]);
   }
 }
 

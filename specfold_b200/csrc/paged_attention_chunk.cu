@@ -7,6 +7,9 @@
 //   warps 8-11       output: O out of TMEM, normalised, written
 //   warp 12          TMA: queries, and K and V blocks through a ring of 32 KB stages
 //   warps 13, 14     issue tcgen05.mma, one warp per tile
+//   warp 15          V blocks that not all rows see all of: rows that no row sees (whose pages hold
+//                    whatever they do) are cleared, values that are not finite are taken out of those
+//                    that only some see (weight 0 times either must be 0)
 // A key block is worked on in two halves of 64 keys, each with its own S [128 x 64] in TMEM (its
 // weights P, in bf16, take the place of its first 32 columns).  While the softmax is on one half,
 // the tensor core adds P V of the other and writes the other's next S = Q K^T, so that the softmax
@@ -32,6 +35,7 @@
 namespace sf {
 
 constexpr int kChunkThreads = 512;
+constexpr int kOddItems = 16;          // more than the items between the V warp and the output
 
 // Of every 8 pairs of weights, this many take the polynomial instead of the special-function unit
 // (none 921 us, one 888, two 891, three 921 for the case above: an exponential costs the FMA pipe
@@ -90,7 +94,7 @@ struct ChunkSmem {
   static constexpr int ring = q + 2 * kTile;             // [kStages][kTile]
   static constexpr int ml = ring + kStages * kTile;      // [2 tiles][m (log2 units), l][128]
   static constexpr int bars = ml + 2 * 2 * 128 * 4;
-  static constexpr int bytes = bars + (2 * kStages + 26) * 8 + 8;
+  static constexpr int bytes = bars + (3 * kStages + 26) * 8 + kOddItems * 4 + 8;
 };
 
 template <int HD>
@@ -101,7 +105,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int KCH = HD / 64, NS = L::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::bars);
-  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 2 * NS + 26);
+  // [x % kOddItems] x, where the V of the CTA's x-th item (with blocks) lost values
+  volatile uint32_t* odd_items = reinterpret_cast<volatile uint32_t*>(bars + 3 * NS + 26);
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 3 * NS + 26 + kOddItems / 2);
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(&tmem_slot + 1);
   if (smem_u32(sm) & 1023) {                             // the swizzled tiles need it; all threads see it
     flag_error(p.err, SF_DEV_ERR_TMEM);
@@ -109,7 +115,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   }
   uint64_t* full = bars;                                 // [NS]
   uint64_t* empty = bars + NS;                           // [NS]
-  uint64_t* q_full = bars + 2 * NS;                      // [2] and so on: one per tile
+  uint64_t* fit = bars + 2 * NS;                         // [NS] looked at by the V warp
+  uint64_t* q_full = bars + 3 * NS;                      // [2] and so on: one per tile
   uint64_t* q_empty = q_full + 2;
   uint64_t* o_done = q_full + 4;
   uint64_t* o_free = q_full + 6;
@@ -129,6 +136,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 2);                           // both tiles
+      mbar_init(&fit[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
@@ -144,6 +152,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&ml_full[t], 4);
       mbar_init(&ml_free[t], 4);
     }
+    for (int x = 0; x < kOddItems; ++x) odd_items[x] = ~0u;
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -231,7 +240,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (!wait(&o_free[t], (par >> 1) ^ 1)) return false;
             par ^= 2;
           }
-          if (!wait(&full[due_stage], due_phase)) return false;
+          if (!wait(&full[due_stage], due_phase) || !wait(&fit[due_stage], due_phase)) return false;
         }
         if (!wait(&p_full[2 * t + h], par)) return false;
         tc_fence_after();
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             due_end = left == 1;
           } else {
             due_stage = NS;
-            ok = wait(&full[stage], phase);
+            ok = wait(&full[stage], phase) && wait(&fit[stage], phase);
             mbar_arrive(&empty[stage]);
           }
           advance();
@@ -314,16 +323,66 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (!ok) abort_flag = 1;
       umma_commit(&drain[t]);
       mbar_wait(&drain[t], 0, p.err);
+    } else if (warp == 15) {
+      // -------------------------------------------------------------- V
+      uint32_t u = 0;                                    // ring units (every one is waited for, so that
+                                                         // no parity is mistaken)
+      uint32_t nth = 0;                                  // items with blocks
+      bool ok = true;
+      for (int it = first; ok && it < last; ++it) {
+        const PagedItem w = p.items[it];
+        if (w.i0 == w.i1) continue;
+        ++nth;
+        const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
+        const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
+        const int hi_min = mask.hi(w.tok0), lo_max = mask.lo(w.tok0 + w.ntok - 1);
+        for (int i = w.i0; ok && i < w.i1; ++i) {
+          const int k0 = w.block(i) * kPagedKB;
+          for (int kv = 0; kv < 2; ++kv, ++u) {
+            const int s = u % NS;
+            ok = __all_sync(0xffffffffu, wait_or_abort(&full[s], (u / NS) & 1, p.err, &abort_flag));
+            if (!ok) break;
+            if (kv == 1 && (k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks))) {
+              bool odd = false;
+              // four rows at a time, 16 bytes a lane
+#pragma unroll 2
+              for (int r = lane / 8; r < kPagedKB; r += 4) {
+                const int j = k0 + r;
+                const bool seen = range.has(j);
+                if (seen && j < hi_min && (j >= lo_max || j < range.sinks)) continue;
+                uint4* at = reinterpret_cast<uint4*>(sm + L::ring + s * L::kTile + r * 128) + lane % 8;
+#pragma unroll
+                for (int c = 0; c < KCH; ++c) {
+                  uint4 d = make_uint4(0, 0, 0, 0);
+                  bool write = !seen;
+                  if (seen) {
+                    d = at[c * (kPagedBox / 16)];
+                    write = drop_odd(d);
+                    odd |= write;
+                  }
+                  if (write) at[c * (kPagedBox / 16)] = d;
+                }
+              }
+              if (__any_sync(0xffffffffu, odd) && lane == 0) odd_items[nth % kOddItems] = nth;
+              fence_async_shared();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&fit[s]);
+          }
+        }
+      }
+      if (!ok) abort_flag = 1;
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- output
     const int quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    uint32_t on[2] = {0, 0};
+    uint32_t on[2] = {0, 0}, nth = 0;
     bool ok = true;
     for (int it = first; ok && it < last; ++it) {
       const PagedItem w = p.items[it];
       const bool any = w.i1 > w.i0;
+      nth += any;
       for (int t = 0; ok && t < (w.ntok > tq ? 2 : 1); ++t) {
         const int rows = (min(w.ntok, (t + 1) * tq) - t * tq) * p.G;
         float m = -INFINITY, l = 0.f;
@@ -342,7 +401,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int64_t row = tok * p.H + w.kvh * p.G + r % p.G;
         const int64_t prow = static_cast<int64_t>(w.slot) * p.rows + t * 128 + r;
         const float f = w.slot >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        uint64_t finite = pair(0.f, 0.f);                // NaN where O is not
 #pragma unroll 1
         for (int c = 0; c < HD; c += 8) {
           float o[8];
@@ -350,8 +408,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (any) {
             tmem_ld8(tmem + 256 + t * 128 + lane_off + c, o);
             tmem_wait<8>(o);
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) finite = fma2(pair(o[j], o[j + 1]), pair(0.f, 0.f), finite);
           }
           if (any && c + 8 == HD) {                      // O is read: the next item may begin
             tc_fence_before();
@@ -382,21 +438,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             p.lse[row] = m * 0.6931471805599453f + logf(l);
           }
         }
-        float f_even, f_odd;
-        unpair(finite, f_even, f_odd);
-        unsigned todo = __ballot_sync(0xffffffffu, r < rows && f_even + f_odd != 0.f && l < INFINITY);
-        if (todo != 0) {                                 // values that not all rows see?
+        if (any && odd_items[nth % kOddItems] == nth) {  // values that decide their columns
           const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
-          const int t0 = w.tok0 + t * tq, t1 = min(w.tok0 + w.ntok, t0 + tq);
-          if (!paged_odd_values<__nv_bfloat16, HD>(p, w, mask.range(w.tok0, w.tok0 + w.ntok), mask.hi(t0), mask.lo(t1 - 1), kPagedKB, lane))
-            todo = 0;
           __syncwarp();                                  // the rows are read back
-          for (; todo != 0; todo &= todo - 1) {
-            const int x = __ffs(todo) - 1, rx = quarter * 32 + x;
-            paged_repair_row<__nv_bfloat16, HD>(p, w, t0 + rx / p.G, rx % p.G, __shfl_sync(0xffffffffu, m, x),
-                                                __shfl_sync(0xffffffffu, f, x),
-                                                static_cast<__nv_bfloat16*>(p.out) + __shfl_sync(0xffffffffu, row, x) * HD,
-                                                w.slot >= 0 ? p.part_O + __shfl_sync(0xffffffffu, prow, x) * HD : nullptr, kPagedKB, lane);
+          float sum[HD / 32];
+          for (int x = 0, seen = -1; x < 32 && quarter * 32 + x < rows; ++x) {
+            const int rx = quarter * 32 + x, tx = w.tok0 + t * tq + rx / p.G;
+            if (tx != seen)
+              paged_odd_values<__nv_bfloat16, HD>(p, w, tx, true, mask.hi(w.tok0), mask.lo(w.tok0 + w.ntok - 1), kPagedKB, lane, ~0u, sum);
+            seen = tx;
+            paged_put_odd<__nv_bfloat16, HD>(
+                sum, true, static_cast<__nv_bfloat16*>(p.out) + (static_cast<int64_t>(w.q0 + tx) * p.H + w.kvh * p.G + rx % p.G) * HD,
+                w.slot >= 0 ? p.part_O + (static_cast<int64_t>(w.slot) * p.rows + t * 128 + rx) * HD : nullptr, lane);
           }
         }
       }
@@ -408,11 +461,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
     const float sl2 = p.scale * 1.4426950408889634f;     // scores in log2 units
-    uint32_t n = 0, items = 0, x = 0;                    // this tile's blocks, items; blocks of the stream
+    uint32_t n = 0, items = 0;                           // this tile's blocks, items
     bool ok = true;
     for (int it = first; ok && it < last; ++it) {
       const PagedItem w = p.items[it];
-      if (t == 1 && w.ntok <= tq) x += w.i1 - w.i0;
       if (w.i0 == w.i1 || (t == 1 && w.ntok <= tq)) continue;
       const PagedMask mask{p.block, p.window, p.sinks, w.q_len, w.kv_len};
       const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
@@ -422,26 +474,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int hi = mask.hi(tok), lo = mask.lo(tok);
       const int hi_min = mask.hi(t0), lo_max = mask.lo(t1 - 1);
       float m = -INFINITY, l = 0.f;
-      for (int i = w.i0; i < w.i1; ++i, ++n, ++x) {
+      for (int i = w.i0; i < w.i1; ++i, ++n) {
         const int k0 = w.block(i) * kPagedKB;
-        // The keys of this block that no row sees hold whatever their pages do: weight 0 times that
-        // must be 0 (thread r clears row r of V; the other tile's writes the same zeros).  Not before
-        // this block's scores are there: tile 1 skips items, and until its issuing warp has come this
-        // far the parity may name an earlier use of the stage.
-        if (k0 < range.lo || k0 + kPagedKB > range.hi) {
-          ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * t], n & 1, p.err, &abort_flag));
-          if (!ok) break;
-          if (!range.has(k0 + r)) {
-            const uint32_t u = 2 * x + 1;
-            wait_or_abort(&full[u % NS], (u / NS) & 1, p.err, &abort_flag);
-            unsigned char* row = sm + L::ring + (u % NS) * L::kTile + r * 128;
-#pragma unroll
-            for (int c = 0; c < KCH; ++c)
-#pragma unroll
-              for (int y = 0; y < 8; ++y) *reinterpret_cast<uint4*>(row + c * kPagedBox + y * 16) = make_uint4(0, 0, 0, 0);
-            fence_async_shared();
-          }
-        }
         const bool edge = k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {

@@ -42,6 +42,27 @@ __device__ __forceinline__ void simt_load_keys(float* dst, const void* pages, co
   }
 }
 
+// Takes values that are not finite out of the keys that not all rows see (not in [all_lo, all_hi), and
+// no sink), each thread out of what it loaded; whether there were any.
+template <int HD>
+__device__ __forceinline__ bool simt_drop_odd(float* dst, int k0, int sinks, int all_lo, int all_hi) {
+  constexpr int VPR = HD / 4;
+  bool odd = false;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kSimtKeys * VPR; i += kSimtThreads) {
+    const int r = i / VPR, key = k0 + r;
+    if (key < all_hi && (key >= all_lo || key < sinks)) continue;
+    float* x = dst + r * (HD + 4) + (i % VPR) * 4;
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (!(fabsf(x[y]) < INFINITY)) {
+        x[y] = 0.f;
+        odd = true;
+      }
+  }
+  return odd;
+}
+
 template <int HD, int RM>
 __device__ __forceinline__ void simt_load_q(float* sQ, const void* q, int64_t q_tok, int64_t q_head,
                                             int row0, int kvh, int G, int rows) {
@@ -103,14 +124,31 @@ __device__ __forceinline__ float half_warp_sum(float v) {
   return v;
 }
 
+// The values that were left out of an item decide their columns.  (A call: registers are short above.)
+template <int HD>
+__device__ __noinline__ void simt_put_odd(const PagedAttnParams& p, int item, int all_lo, int all_hi) {
+  const PagedItem w = p.items[item];
+  const int lane = threadIdx.x & 31;
+  float sum[HD / 32];
+  for (int tok = threadIdx.x >> 5; tok < w.ntok; tok += kSimtThreads / 32) {
+    paged_odd_values<float, HD>(p, w, w.tok0 + tok, true, all_hi, all_lo, kSimtKeys, lane, ~0u, sum);
+    for (int g = 0; g < p.G; ++g) {
+      const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + tok) * p.H + w.kvh * p.G + g;
+      paged_put_odd<float, HD>(sum, true, static_cast<float*>(p.out) + row * HD,
+                               w.slot >= 0 ? p.part_O + (static_cast<int64_t>(w.slot) * p.rows + tok * p.G + g) * HD : nullptr, lane);
+    }
+  }
+}
+
 template <int HD, int RM>
-__global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(PagedAttnParams p) {
+__global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(const __grid_constant__ PagedAttnParams p) {
   constexpr int R = 16 * RM, LD = HD + 4, LP = 2 * kSimtKeys + 4;
   constexpr int DV = HD / 64;                           // float4 groups of O per thread
   extern __shared__ __align__(16) float sm[];
   float* sQ = sm;                                       // [R][LD]
   float* sKV = sQ + R * LD;                             // [64][LD]
   float* sP = sKV + kSimtKeys * LD;                     // [R][LP], every weight twice
+  __shared__ int s_all[3];                              // all rows see keys [0], [1); values were left out
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float sl2 = p.scale * 1.4426950408889634f;
   const int last = p.first[blockIdx.x + 1];
@@ -134,6 +172,11 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
     }
     const PagedRange range = mask.range(w.tok0, w.tok0 + w.ntok);
     __syncthreads();                                    // the previous item's reads are done
+    if (threadIdx.x == 0) {
+      s_all[0] = mask.lo(w.tok0 + w.ntok - 1);
+      s_all[1] = mask.hi(w.tok0);
+      s_all[2] = 0;
+    }
     simt_load_q<HD, RM>(sQ, p.q, p.q_tok, p.q_head, w.q0 + w.tok0, w.kvh, p.G, rows);
     for (int i = w.i0; i < w.i1; ++i) {
       const int k0 = w.block(i) * kSimtKeys;
@@ -173,6 +216,8 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
       }
       __syncthreads();                                  // K read, P written
       simt_load_keys<HD>(sKV, p.pool.v, p.pool, w.seq, w.kvh, k0, range, p.err);
+      if ((k0 + kSimtKeys > s_all[1] || k0 < s_all[0]) && simt_drop_odd<HD>(sKV, k0, p.window > 0 ? p.sinks : 0, s_all[0], s_all[1]))
+        s_all[2] = 1;
       __syncthreads();
       // a row of P is written and read by the same half-warp's 16 threads
 #pragma unroll 4
@@ -194,19 +239,10 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
         }
       }
     }
-    unsigned odd = 0;                                   // this thread's rows whose O is not finite
 #pragma unroll
     for (int a = 0; a < RM; ++a) {
       const int r = ty + 16 * a;
       if (r >= rows) continue;
-#pragma unroll
-      for (int d = 0; d < DV; ++d)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float e0, e1;
-          unpair(o[a][d][x], e0, e1);
-          odd |= static_cast<unsigned>(l[a] < INFINITY && fmaf(e0, 0.f, e1 * 0.f) != 0.f) << a;
-        }
       if (w.slot >= 0) {
         const int64_t pr = static_cast<int64_t>(w.slot) * p.rows + r;
 #pragma unroll
@@ -233,28 +269,8 @@ __global__ void __launch_bounds__(kSimtThreads, 2) paged_attention_simt_kernel(P
         if (tx == 0) p.lse[t * p.H + h] = m[a] * 0.6931471805599453f + logf(l[a]);
       }
     }
-    if (__any_sync(0xffffffffu, odd != 0)) {            // values that not all rows see?
-      const int lane = threadIdx.x & 31;
-      __syncwarp();                                     // the rows are read back
-      if (paged_odd_values<float, HD>(p, w, range, mask.hi(w.tok0), mask.lo(w.tok0 + w.ntok - 1), kSimtKeys, lane)) {
-#pragma unroll 1
-        for (int x = 0; x < 2 * RM; ++x) {              // the warp's rows: two of every 16
-          const int a = x >> 1, half = x & 1;
-          const unsigned who = __ballot_sync(0xffffffffu, odd >> a & 1);
-          if ((who >> (16 * half) & 0xffffu) == 0) continue;
-          float ma = m[0], la = l[0];
-#pragma unroll
-          for (int y = 1; y < RM; ++y)
-            if (a == y) ma = m[y], la = l[y];
-          ma = __shfl_sync(0xffffffffu, ma, 16 * half);
-          la = __shfl_sync(0xffffffffu, la, 16 * half);
-          const int r = (ty & ~1) + half + 16 * a;
-          const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + r / p.G) * p.H + w.kvh * p.G + r % p.G;
-          paged_repair_row<float, HD>(p, w, w.tok0 + r / p.G, r % p.G, ma, la == 0.f ? 0.f : 1.f / la, static_cast<float*>(p.out) + row * HD,
-                                  w.slot >= 0 ? p.part_O + (static_cast<int64_t>(w.slot) * p.rows + r) * HD : nullptr, kSimtKeys, lane);
-        }
-      }
-    }
+    __syncthreads();
+    if (s_all[2]) simt_put_odd<HD>(p, it, s_all[0], s_all[1]);
   }
 }
 

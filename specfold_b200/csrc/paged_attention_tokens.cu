@@ -239,8 +239,10 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       const int hi = mask.hi(tok), lo = mask.lo(tok);
       const int hi_min = mask.hi(w.tok0), lo_max = mask.lo(w.tok0 + w.ntok - 1);
       float m = -INFINITY, l = 0.f;
+      bool finite = true;                                // what this thread saw of V and of the output
       for (int i = w.i0; i < w.i1; ++i, ++n) {
         const int k0 = w.block(i) * kPagedKB;
+        const bool edge = k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks);
         ok = __all_sync(0xffffffffu, ok && wait_or_abort(&s_full[n & 1], (n >> 1) & 1, p.err, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
 #pragma unroll
           for (int c = 0; c < NC; c += 32) tmem_ld32(tmem + (n & 1) * 128 + lane_off + copy * NC + c, v + c);
           tmem_wait<NC>(v);
-          if (k0 + kPagedKB > hi_min || (k0 < lo_max && k0 + kPagedKB > range.sinks)) {
+          if (edge) {
             const int h = hi - k0 - copy * NC, b = lo - k0 - copy * NC, f = range.sinks - k0 - copy * NC;
 #pragma unroll
             for (int j = 0; j < NC; ++j)
@@ -260,17 +262,29 @@ __global__ void __launch_bounds__(kTokThreads, 1)
           for (int j = 0; j < NC; ++j) mx = fmaxf(mx, v[j]);
           mx *= sl2;
         }
-        // the keys of this block that no row sees hold whatever their pages do: weight 0 times
-        // that must be 0 (thread r clears row r of V)
-        const bool edge = k0 < range.lo || k0 + kPagedKB > range.hi;
-        if (edge && !range.has(k0 + r)) {
+        // The keys of this block that no row sees hold whatever their pages do, and those that only
+        // some see may hold values that are not finite: weight 0 times either must be 0 (thread r
+        // clears row r of V, or takes such values out of it).
+        const int key = k0 + r;
+        const bool seen = range.has(key);
+        if (edge && !(seen && key < hi_min && (key >= lo_max || key < range.sinks))) {
           const uint32_t u = 2 * n + 1;
           ok = mbar_wait(&full[u % NS], (u / NS) & 1, p.err);
-          unsigned char* row = sm + L::ring + (u % NS) * L::kTile + r * 128;
+          uint4* row = reinterpret_cast<uint4*>(sm + L::ring + (u % NS) * L::kTile + r * 128);
 #pragma unroll
           for (int c = 0; c < KCH; ++c)
 #pragma unroll
-            for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(row + c * kPagedBox + x * 16) = make_uint4(0, 0, 0, 0);
+            for (int x = 0; x < 8; ++x) {
+              uint4 d = make_uint4(0, 0, 0, 0);
+              uint4* at = row + c * (kPagedBox / 16) + ((x + r) & 7);   // (the rows' banks apart)
+              bool write = !seen;
+              if (seen) {
+                d = *at;
+                write = drop_odd(d);
+                finite &= !write;
+              }
+              if (write) *at = d;
+            }
           fence_async_shared();
         }
         // the P V before reads P and adds to O
@@ -339,8 +353,6 @@ __global__ void __launch_bounds__(kTokThreads, 1)
       // where the rows are few, else 32 at a time.
       const int turn = REP * rows * (HD + 1) <= 128 * kRedLd ? HD : 32, ld = turn + 1;
       float* mine = red + (copy * rows + rr) * ld;
-      float finite = 0.f;                                // NaN where an output of this thread's is not finite
-      bool all_finite = true;
 #pragma unroll 1
       for (int c0 = 0; c0 < HD; c0 += turn) {
 #pragma unroll 1
@@ -367,7 +379,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
           float sum = red[row * ld + c];
 #pragma unroll
           for (int y = 1; y < REP; ++y) sum += red[(y * rows + row) * ld + c];
-          finite = fmaf(sum, 0.f, finite);
+          finite &= fabsf(sum) < INFINITY;
           if (w.slot < 0) {
             const int64_t t = w.q0 + w.tok0 + row / p.G;
             static_cast<__nv_bfloat16*>(p.out)[(t * p.H + w.kvh * p.G + row % p.G) * HD + c0 + c] =
@@ -376,7 +388,7 @@ __global__ void __launch_bounds__(kTokThreads, 1)
             p.part_O[(slot_row + row) * HD + c0 + c] = sum;
           }
         }
-        all_finite = vote128(finite == 0.f);
+        finite = vote128(finite);
       }
       if (valid && copy == 0) {
         if (w.slot < 0) {
@@ -387,23 +399,27 @@ __global__ void __launch_bounds__(kTokThreads, 1)
           p.part_ml[2 * (slot_row + rr) + 1] = L_row;
         }
       }
-      // Values that not all rows see?  (One token's rows see the same; of its copies only one has the
-      // weight of an infinite value, the others 0.)
-      if (!all_finite && (REP > 1 || (w.ntok > 1 && paged_odd_values<__nv_bfloat16, HD>(p, w, range, hi_min, lo_max, kPagedKB, lane)))) {
-        if (valid && copy == 0) {
-          s_m[rr] = M_row;
-          s_l[rr] = L_row;
+      // Values that decide their columns.  (Of a row's copies only one has the weight of such a value,
+      // the others 0: infinity became NaN, so the sum takes the output's place, unless the scores were NaN.)
+      if (!finite) {
+        vote128(true);                                   // lse is read back
+        float sum[HD / 32];
+        for (int tok = quarter; tok < w.ntok; tok += 4) {
+          const int64_t row0 = static_cast<int64_t>(w.q0 + w.tok0 + tok) * p.H + w.kvh * p.G;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + row0 * HD;
+          float* part = w.slot >= 0 ? p.part_O + (slot_row + tok * p.G) * HD : nullptr;
+          unsigned need = w.ntok == 1 ? 0u : ~0u;        // one token: nothing was left out of V
+          for (int g = 0; w.ntok == 1 && g < p.G; ++g)
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) {
+              const int at = g * HD + lane * (HD / 32) + e;
+              need |= static_cast<unsigned>(!(fabsf(part != nullptr ? part[at] : __bfloat162float(out[at])) < INFINITY)) << e;
+            }
+          paged_odd_values<__nv_bfloat16, HD>(p, w, w.tok0 + tok, REP == 1, hi_min, lo_max, kPagedKB, lane, need, sum);
+          for (int g = 0; g < p.G; ++g)
+            if (part != nullptr || !isnan(p.lse[row0 + g]))
+              paged_put_odd<__nv_bfloat16, HD>(sum, REP == 1, out + g * HD, part != nullptr ? part + g * HD : nullptr, lane);
         }
-        vote128(true);
-        for (int x = quarter; x < rows; x += 4) {
-          const int64_t row = static_cast<int64_t>(w.q0 + w.tok0 + x / p.G) * p.H + w.kvh * p.G + x % p.G;
-          const float sum = s_l[x];
-          if (sum < INFINITY)
-            paged_repair_row<__nv_bfloat16, HD>(p, w, w.tok0 + x / p.G, x % p.G, s_m[x], sum == 0.f ? 0.f : 1.f / sum,
-                                                static_cast<__nv_bfloat16*>(p.out) + row * HD,
-                                                w.slot >= 0 ? p.part_O + (slot_row + x) * HD : nullptr, kPagedKB, lane);
-        }
-        vote128(true);                                   // (the next item writes s_m)
       }
     }
     if (!ok) *abort_flag = 1;

@@ -121,6 +121,18 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, in
   }
 }
 
+// Values that are not finite become 0; whether there were any.  (An exponent of ones is carried into
+// the bit above it.)
+__device__ __forceinline__ bool drop_odd(uint32_t& x) {
+  const uint32_t t = ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  if (t != 0) x &= ~((t & 0x8000u ? 0xffffu : 0u) | (t & 0x80000000u ? 0xffff0000u : 0u));
+  return t != 0;
+}
+__device__ __forceinline__ bool drop_odd(uint4& d) {
+  return static_cast<int>(drop_odd(d.x)) | static_cast<int>(drop_odd(d.y)) | static_cast<int>(drop_odd(d.z)) |
+         static_cast<int>(drop_odd(d.w));
+}
+
 constexpr int kPagedBox = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzled
 
 // What a lane of the loading warp fetches of a key block: box lane / chunks (a page, or half of a

@@ -69,7 +69,7 @@ class Step:
             see, rows = self.sees(b), slice(t0, t0 + ql)
             t0 += ql
             some = see.any(1)
-            for h in range(self.H):
+            for h in range(self.H if see.numel() else 0):
                 q, k, v = self.q[rows, h].double(), self.k[b][:, h // G].double(), self.v[b][:, h // G].double()
                 s = (q @ k.T * self.scale).masked_fill(~see, -math.inf)
                 top = s.amax(1, keepdim=True).masked_fill(~some[:, None], 0)
@@ -82,7 +82,7 @@ class Step:
                 x = see.double()
                 pos, neg, nan = (x @ m.double() > 0 for m in (v == math.inf, v == -math.inf, v.isnan()))
                 o = o.masked_fill(pos, math.inf).masked_fill(neg, -math.inf).masked_fill(nan | (pos & neg), math.nan)
-                out[rows, h] = o
+                out[rows, h] = o.masked_fill(z.isnan(), math.nan)
                 lse[rows, h] = torch.where(some, (top + z.log())[:, 0], -math.inf)
                 e = self.hd * U32 * self.scale * (q.abs() @ k.abs().T).masked_fill(~see, 0).amax(1)
                 e += 8 * U32 * s.abs().masked_fill(~see, 0).amax(1) + see.sum(1) * U32
@@ -428,3 +428,18 @@ def test_sequences_within_their_budget_stay_where_they_are():
     assert kept[0].shape == (2, 2, 40) and kept[0][0, 1].tolist() == list(range(40)) and int(kept[0][1, 0, 7]) == -1
     with pytest.raises(ValueError, match="budgets"):
         cache.evict([a, b], [50])
+
+
+def test_a_value_that_is_not_finite_holds_nobody_up():
+    """One NaN late in a chunk over a long cache, and one in a long cache of single tokens: no wait of
+    the kernels runs out, and the tokens before it stay finite."""
+    st = Step([2048, 1, 1], [131072, 3000, 131072], 16, 8, ps=256, seed=8)
+    st.v[0][131072 - 1000, :, 3] = math.nan
+    st.v[2][700, :, 5] = math.nan
+    k, v = st.pages()
+    plan = st.plan()
+    out, lse = K.paged_attention(st.q, k, v, st.table, plan)
+    plan.check()
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    hit[1048:2048, :, 3] = hit[2049, :, 5] = True
+    assert torch.equal(out.isnan(), hit) and bool(lse.isfinite().all())
