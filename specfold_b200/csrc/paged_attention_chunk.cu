@@ -23,13 +23,15 @@
 // key of, and later halves only check their largest score against it; where a row outgrows it, the
 // reference moves and O is rescaled.
 //
-// Measured (32 / 8 heads of 128, 4096 tokens over 16384 cached keys, 0.96 TFLOP): 888 us, 1.08
+// Measured (32 / 8 heads of 128, 4096 tokens over 16384 cached keys, 0.96 TFLOP): 885 us, 1.09
 // PFLOP/s, 66% of a cuBLAS burst and 80% of what cuBLAS sustains under the same 1000 W cap (this
 // kernel runs there at 1.59 of 1.965 GHz).  Without the softmax's work the same loads and products
 // take 639 us.  A whole block at a time, with the running maximum of every block, took 1316 us; a
 // separate issuing warp per tile, elected so that the compiler knows it is one thread, was worth a
 // quarter of that (a commit holds its thread until the tensor core has run what came before it).
-// Windowed ragged chunks (40 / 8 heads, window 1000, 5600 tokens): 210 us.
+// Windowed ragged chunks (40 / 8 heads, window 1000, 5600 tokens): 214 us.
+// The waits that keep parities unmistakable are in the issuing warps, whose products hide them: in
+// the softmax warps one more wait a half cost the first case 932 to 949 us.
 #include "paged_tc.cuh"
 
 namespace sf {

@@ -10,9 +10,10 @@
 // Products are taken two at a time (fma.rn.f32x2): half the issue slots for the same FMA rate.
 // Scores add up even and odd dims apart; for P V each weight is stored twice, side by side.
 //
-// Measured (12 / 2 heads of 128, 704 tokens over 800 to 2100 keys, block-causal): 254 us, 24
-// TFLOP/s of the 70 the FMA pipes could do; single products took 265 us.  What bounds it is the
-// loads' latency with two CTAs of 8 warps on an SM: shared memory has no room for a second buffer.
+// Measured (12 / 2 heads of 128, 704 tokens over 800 to 2100 keys, block-causal): 264 us, 23
+// TFLOP/s of the 70 the FMA pipes could do; single products took 4% longer, and 2% go to the look at
+// values that only some rows see.  The FMA pipes are 48% busy, the shared-memory pipe 62%: loads are
+// waited for with two CTAs of 8 warps on an SM, and there is no room for a second buffer.
 #include "paged_tc.cuh"
 
 namespace sf {

@@ -17,9 +17,9 @@
 // The rescaling of O waits until a row's maximum has grown by 2^8: until then the weights are
 // merely up to 2^8 instead of 1, relative to the same reference in l and O, and lose nothing.
 //
-// Measured (32 / 8 heads of 128): 64 single tokens over 1100 to 16384 keys, 1.52 GB, in 290 us (5.2
-// TB/s, 81% of a plain copy's rate); 32 tokens that see a window of 4096 and 4 first keys, 244 MB,
-// in 57 us.  In the steady state a CTA takes 2200 cycles a block; the rest is the first loads'
+// Measured (32 / 8 heads of 128): 64 single tokens over 1100 to 16384 keys, 1.52 GB, in 297 us (5.1
+// TB/s, 79% of a plain copy's rate); 32 tokens that see a window of 4096 and 4 first keys, 244 MB,
+// in 60 us.  In the steady state a CTA takes 2200 cycles a block; the rest is the first loads'
 // latency (page id, keys, 5000 cycles) and each item's output.  One token over 777 keys: 11 us on
 // the device, the latency of the chain item, page id, keys, softmax, output, join.
 #include "paged_tc.cuh"

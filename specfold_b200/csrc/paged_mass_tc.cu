@@ -11,16 +11,16 @@
 //   warps 4-11, 12-19 exponentials and sums of the first and of the second block, two threads per
 //                     key: rows 0-63 and 64-127 of a tile.  Two warps on each scheduler for either
 //                     block hide each other's waits for TMEM and for the special-function unit: with
-//                     one thread per key the largest case took 292 us, with two 236
+//                     one thread per key the largest case took 292 us, with two a fifth less
 //   warp 0            TMA: key blocks and query tiles, through rings of their own
 //   warp 1            tcgen05.mma, two S^T buffers of 128 columns for each block (all of TMEM)
 //   warp 2            lse of the tile's rows into shared memory
 // Bound: for chunks by the special-function unit, one exponential per (row, key): 1024 cycles for
 // a 128 x 128 tile against 512 of products; for single tokens by the bytes of the keys.
 //
-// Measured: 28 / 4 heads, 4051 tokens over 5300 and 8192 keys, 0.167 TFLOP, 6.5e8 exponentials: 236
-// us, 1.5 times what the special-function units need; 32 tokens over 1000 to 8192 keys of 8 heads,
-// 235 MB: 53 us (4.4 TB/s).  A polynomial for some of the exponentials did not help (289 to 328 us
+// Measured: 28 / 4 heads, 4051 tokens over 5300 and 8192 keys, 0.167 TFLOP, 6.5e8 exponentials: 249
+// us, 1.6 times what the special-function units need; 32 tokens over 1000 to 8192 keys of 8 heads,
+// 235 MB: 55 us (4.3 TB/s).  A polynomial for some of the exponentials did not help (289 to 328 us
 // where none took 292, before there were two threads per key).
 #include "paged_tc.cuh"
 
